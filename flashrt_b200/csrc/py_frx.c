@@ -43,6 +43,12 @@ static int ints(PyObject* const* a, Py_ssize_t n, Py_ssize_t want, i64* v) {
     }
 
 BIND(route_topk, 10, frx_route_topk(S(0), P(1), I(2), I(3), I(4), P(5), P(6), P(7), P(8), I(9)))
+BIND(route_topk_backward, 8, frx_route_topk_backward(S(0), P(1), P(2), P(3), I(4), I(5), I(6), P(7)))
+BIND(moe_sort, 10, frx_moe_sort(S(0), P(1), I(2), I(3), I(4), P(5), P(6), P(7), P(8), Z(9)))
+BIND(moe_sort_rows, 11, frx_moe_sort_rows(S(0), P(1), v[2], I(3), P(4), I(5), I(6), I(7), P(8), v[9], v[10]))
+BIND(moe_sort_rows_backward, 11, frx_moe_sort_rows_backward(S(0), P(1), v[2], v[3], I(4), P(5), I(6), I(7), I(8), P(9), v[10]))
+BIND(moe_unsort_rows, 12, frx_moe_unsort_rows(S(0), P(1), v[2], v[3], I(4), P(5), P(6), I(7), I(8), I(9), P(10), v[11]))
+BIND(moe_unsort_rows_backward, 15, frx_moe_unsort_rows_backward(S(0), P(1), v[2], P(3), v[4], v[5], I(6), P(7), P(8), I(9), I(10), I(11), P(12), v[13], P(14)))
 BIND(router_logits, 9, frx_router_logits(S(0), P(1), P(2), P(3), I(4), I(5), I(6), P(7), P(8)))
 BIND(quantize_q8, 6, frx_quantize_q8(S(0), P(1), I(2), I(3), P(4), P(5)))
 BIND(moe_decode, 17, frx_moe_decode(P(0), Z(1), I(2), P(3), I(4), I(5), P(6), P(7), P(8), P(9), I(10), I(11), P(12), P(13), P(14), Z(15), S(16)))
@@ -58,9 +64,22 @@ BIND(gemv_moe_q2_0, 11, frx_gemv_moe_q2_0(P(0), P(1), P(2), P(3), P(4), I(5), v[
 BIND(gemv_matvec, 9, frx_gemv_matvec((uint32_t)v[0], P(1), P(2), P(3), v[4], v[5], I(6), P(7), S(8)))
 BIND(gemm_moe_prepare, 12, frx_gemm_moe_prepare(P(0), (uint32_t)v[1], I(2), P(3), I(4), P(5), v[6], I(7), v[8], P(9), Z(10), S(11)))
 BIND(gemm_moe_run, 6, frx_gemm_moe_run(P(0), P(1), v[2], P(3), v[4], S(5)))
+BIND(mxfp4_quantize, 8, frx_mxfp4_quantize(S(0), P(1), v[2], I(3), I(4), I(5), P(6), P(7)))
+BIND(mxfp4_dequantize, 8, frx_mxfp4_dequantize(S(0), P(1), P(2), I(3), I(4), I(5), P(6), v[7]))
+BIND(mxfp4_matmul, 10, frx_mxfp4_matmul(S(0), P(1), P(2), I(3), I(4), P(5), I(6), P(7), v[8], I(9)))
+BIND(mxfp4_moe_matmul, 15,
+     frx_mxfp4_moe_matmul(S(0), P(1), P(2), I(3), I(4), P(5), I(6), I(7), P(8), P(9), I(10), I(11), P(12), v[13], I(14)))
+BIND(mxfp4_moe_layer, 19,
+     frx_mxfp4_moe_layer(S(0), P(1), P(2), P(3), I(4), I(5), I(6), P(7), v[8], I(9), P(10), P(11), I(12), I(13), P(14), v[15], I(16), P(17), Z(18)))
 
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {ENTRY(route_topk),
+                                ENTRY(route_topk_backward),
+                                ENTRY(moe_sort),
+                                ENTRY(moe_sort_rows),
+                                ENTRY(moe_sort_rows_backward),
+                                ENTRY(moe_unsort_rows),
+                                ENTRY(moe_unsort_rows_backward),
                                 ENTRY(router_logits),
                                 ENTRY(quantize_q8),
                                 ENTRY(moe_decode),
@@ -76,6 +95,11 @@ static PyMethodDef methods[] = {ENTRY(route_topk),
                                 ENTRY(gemv_matvec),
                                 ENTRY(gemm_moe_prepare),
                                 ENTRY(gemm_moe_run),
+                                ENTRY(mxfp4_quantize),
+                                ENTRY(mxfp4_dequantize),
+                                ENTRY(mxfp4_matmul),
+                                ENTRY(mxfp4_moe_matmul),
+                                ENTRY(mxfp4_moe_layer),
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_frxpy", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__frxpy(void) { return PyModule_Create(&module); }

@@ -56,6 +56,13 @@ SIGNATURES = {
     "frx_arena_total_bytes": (_sz, [_vp]),
     "frx_arena_load_planar": (_i, [_vp, _i, _i, _i, _vp, _sz, _vp]),
     "frx_route_topk": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i]),
+    "frx_route_topk_backward": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "frx_moe_sort_workspace_bytes": (_sz, [_i, _i, _i]),
+    "frx_moe_sort": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz]),
+    "frx_moe_sort_rows": (_i, [_vp, _vp, _i64, _i, _vp, _i, _i, _i, _vp, _i64, _i64]),
+    "frx_moe_sort_rows_backward": (_i, [_vp, _vp, _i64, _i64, _i, _vp, _i, _i, _i, _vp, _i64]),
+    "frx_moe_unsort_rows": (_i, [_vp, _vp, _i64, _i64, _i, _vp, _vp, _i, _i, _i, _vp, _i64]),
+    "frx_moe_unsort_rows_backward": (_i, [_vp, _vp, _i64, _vp, _i64, _i64, _i, _vp, _vp, _i, _i, _i, _vp, _i64, _vp]),
     "frx_quantize_q8": (_i, [_vp, _vp, _i, _i, _vp, _vp]),
     "frx_moe_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "frx_moe_decode_workspace_offset": (_sz, [_i, _i, _i, _i, C.c_char_p]),
@@ -132,6 +139,15 @@ SIGNATURES = {
     "frx_gemm_moe_prepare": (_i, [_vp, C.c_uint32, _i, _vp, _i, _vp, _i64, _i, _i64, _vp, _sz, _vp]),
     "frx_gemm_moe_run": (_i, [_vp, _vp, _i64, _vp, _i64, _vp]),
     "frx_gemm_moe": (_i, [C.c_uint32, _vp, _i64, _i, _vp, _i, _vp, _i64, _i, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "frx_mxfp4_quantize": (_i, [_vp, _vp, _i64, _i, _i, _i, _vp, _vp]),
+    "frx_mxfp4_dequantize": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _i64]),
+    "frx_mxfp4_packed_bytes": (_sz, [_i, _i]),
+    "frx_mxfp4_pack": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
+    "frx_mxfp4_unpack": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp]),
+    "frx_mxfp4_matmul": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _vp, _i64, _i]),
+    "frx_mxfp4_moe_matmul": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _i64, _i]),
+    "frx_mxfp4_moe_layer_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "frx_mxfp4_moe_layer": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _i, _i, _vp, _i64, _i, _vp, _sz]),
     "frx_convert_q8_0_to_q2_0": (_i, [_vp, _vp, _sz, _vp]),
 }
 

@@ -232,6 +232,136 @@ def quantize_q8(x: torch.Tensor, stream=None):
     return q, d
 
 
+# ---- tokens sorted by expert, and back -----------------------------------------------------------
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # FRX_F32, FRX_BF16, FRX_F16
+
+
+def _on_device(*ts):
+    """The tensors are on the current device, whose stream the call goes to."""
+    dev = _current_device() if _current_device else None
+    for t in ts:
+        if t is not None and not (t.is_cuda and t.get_device() == dev):
+            raise FrxError(_l.ERR_ARG, "tensors must be CUDA tensors of the current device")
+
+
+def _typed(name: str, t: torch.Tensor, dtype, shape=None) -> None:
+    """t is contiguous, of this type, and of this shape if one is given."""
+    if t.dtype != dtype or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise FrxError(_l.ERR_ARG, f"{name}: a contiguous {dtype} tensor{'' if shape is None else f' of shape {tuple(shape)}'} is wanted")
+
+
+def _matrix(name: str, t: torch.Tensor, dtype=None, shape=None) -> int:
+    """How many elements the rows of t are apart: rows are contiguous, and may lie apart."""
+    if t.dim() != 2 or t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype) or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise FrxError(_l.ERR_ARG, f"{name}: rows of {'float32, bfloat16 or float16' if dtype is None else dtype}{'' if shape is None else f', {tuple(shape)},'} are wanted")
+    rows, n = t.shape
+    if rows <= 1:
+        ld = n
+    else:
+        ld = t.stride(0)
+    if (n > 1 and t.stride(1) != 1) or ld < n:
+        raise FrxError(_l.ERR_ARG, f"{name}: the elements of a row must be contiguous and rows must not overlap")
+    return ld
+
+
+def _ids(name: str, t: torch.Tensor, shape=None) -> None:
+    if t.dim() != 2:
+        raise FrxError(_l.ERR_ARG, f"{name}: int32 [tokens][experts per token] is wanted")
+    _typed(name, t, torch.int32, shape)
+
+
+def moe_sort_workspace_bytes(T: int, K: int, E: int) -> int:
+    return int(lib.frx_moe_sort_workspace_bytes(T, K, E))
+
+
+def moe_sort(ids: torch.Tensor, E: int, ws: torch.Tensor | None = None, stream=None):
+    """The plan that sorts the slots of ids int32 [T][K] by expert (frx_moe_sort): offsets int32 [E + 1], slot_of int32 [T * K],
+    row_of int32 [T][K]; -1 where a slot has no row (its id is negative) or a row no slot."""
+    _on_device(ids, ws)
+    _ids("ids", ids)
+    T, K = ids.shape
+    if ws is None:
+        ws = ids.new_empty(moe_sort_workspace_bytes(T, K, E) + 256, dtype=torch.uint8)
+    offsets, slot_of, row_of = ids.new_empty(max(E, 0) + 1), ids.new_empty(T * K), torch.empty_like(ids)
+    wp, wb = _ws_span(ws)
+    check(fast.moe_sort(_raw_stream(stream), ids.data_ptr(), T, K, E, offsets.data_ptr(), slot_of.data_ptr(), row_of.data_ptr(), wp, wb))
+    return offsets, slot_of, row_of
+
+
+def moe_sort_rows(x: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """xs[row_of[t][k]] = x[t]: x [T][n] float32, bfloat16 or float16 -> xs [T * K][n]. Rows that no slot has are left as they were."""
+    _on_device(x, row_of, out)
+    ldx = _matrix("x", x)
+    _ids("row_of", row_of)
+    (T, n), K = x.shape, row_of.shape[1]
+    _ids("row_of", row_of, (T, K))
+    if out is None:
+        out = x.new_empty(T * K, n)
+    ldo = _matrix("out", out, x.dtype, (out.shape[0], n))
+    check(fast.moe_sort_rows(_raw_stream(stream), x.data_ptr(), ldx, DTYPES[x.dtype], row_of.data_ptr(), T, K, n, out.data_ptr(), ldo, out.shape[0]))
+    return out
+
+
+def moe_sort_rows_backward(gxs: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """gx[t] = sum over k of gxs[row_of[t][k]]: the gradient of moe_sort_rows."""
+    _on_device(gxs, row_of, out)
+    ldg = _matrix("gxs", gxs)
+    _ids("row_of", row_of)
+    (T, K), (rows, n) = row_of.shape, gxs.shape
+    if out is None:
+        out = gxs.new_empty(T, n)
+    ldo = _matrix("out", out, gxs.dtype, (T, n))
+    check(fast.moe_sort_rows_backward(_raw_stream(stream), gxs.data_ptr(), ldg, rows, DTYPES[gxs.dtype], row_of.data_ptr(), T, K, n, out.data_ptr(), ldo))
+    return out
+
+
+def moe_unsort_rows(ys: torch.Tensor, wts: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """out[t] = sum over k of wts[t][k] * ys[row_of[t][k]]: sorted rows back to their tokens, with the routing weights applied. A token
+    none of whose slots has a row gets zeros."""
+    _on_device(ys, wts, row_of, out)
+    ldy = _matrix("ys", ys)
+    _ids("row_of", row_of)
+    (T, K), (rows, n) = row_of.shape, ys.shape
+    _typed("wts", wts, torch.float32, (T, K))
+    if out is None:
+        out = ys.new_empty(T, n)
+    ldo = _matrix("out", out, ys.dtype, (T, n))
+    check(fast.moe_unsort_rows(_raw_stream(stream), ys.data_ptr(), ldy, rows, DTYPES[ys.dtype], wts.data_ptr(), row_of.data_ptr(), T, K, n, out.data_ptr(), ldo))
+    return out
+
+
+def moe_unsort_rows_backward(gout: torch.Tensor, ys: torch.Tensor, wts: torch.Tensor, row_of: torch.Tensor, gys: torch.Tensor | None = None, stream=None):
+    """The gradients of moe_unsort_rows: gys [rows][n] (rows that no slot has are left as they were) and gwts float32 [T][K] (0 for a slot
+    without a row)."""
+    _on_device(gout, ys, wts, row_of, gys)
+    ldy = _matrix("ys", ys)
+    _ids("row_of", row_of)
+    (T, K), (rows, n) = row_of.shape, ys.shape
+    ldg = _matrix("gout", gout, ys.dtype, (T, n))
+    _typed("wts", wts, torch.float32, (T, K))
+    if gys is None:
+        gys = ys.new_empty(rows, n)
+    ldgy = _matrix("gys", gys, ys.dtype, (rows, n))
+    gwts = torch.empty_like(wts)
+    check(fast.moe_unsort_rows_backward(_raw_stream(stream), gout.data_ptr(), ldg, ys.data_ptr(), ldy, rows, DTYPES[ys.dtype], wts.data_ptr(), row_of.data_ptr(), T, K, n,
+                                        gys.data_ptr(), ldgy, gwts.data_ptr()))
+    return gys, gwts
+
+
+def moe_route_topk_backward(gwts: torch.Tensor, wts: torch.Tensor, ids: torch.Tensor, E: int, stream=None) -> torch.Tensor:
+    """The gradient of moe_route_topk: glogits float32 [T][E] from the gradient gwts [T][k] of its weights. `ids` are the chosen experts as the
+    router gave them: slots dropped later keep theirs and have the gradient 0 (moe_unsort_rows_backward gives it)."""
+    _on_device(gwts, wts, ids)
+    _ids("ids", ids)
+    T, k = ids.shape
+    _typed("wts", wts, torch.float32, (T, k))
+    _typed("gwts", gwts, torch.float32, (T, k))
+    gl = wts.new_empty(T, max(E, 0))
+    check(fast.route_topk_backward(_raw_stream(stream), gwts.data_ptr(), wts.data_ptr(), ids.data_ptr(), T, E, k, gl.data_ptr()))
+    return gl
+
+
 # ---- the layer ---------------------------------------------------------------------------------
 
 def moe_decode_workspace_bytes(T: int, K: int, n: int, ff: int) -> int:

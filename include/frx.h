@@ -47,6 +47,9 @@ enum {
     FRX_ERR_DEVICE = 5     /* a kernel reported an error (bad expert id, a wait that ran out) */
 };
 
+/* Element types of rows, where a call takes several (`dtype` arguments). */
+enum { FRX_F32 = 0, FRX_BF16 = 1, FRX_F16 = 2 };
+
 int frx_version(void);
 const char* frx_last_error(void);
 
@@ -185,6 +188,40 @@ int frx_arena_load_planar(frx_arena* a, int layer, int expert0, int count, const
  * maximum), tie there and go to the lower index, while here the larger logit wins. */
 int frx_route_topk(frx_stream_t stream, const float* logits, int T, int E, int k, int32_t* ids, float* wts,
                    uint32_t* counts, uint32_t* tail_counts, int tail_from);
+
+/* The gradient of frx_route_topk: with w the weights that it gave (the softmax over a token's chosen logits) and gwts [T][k] the
+ * gradient that arrives at them, glogits[t][ids[t][j]] = w_j * (gwts_j - sum_i w_i * gwts_i), and 0 at the experts that were not
+ * chosen. All of glogits [T][E] is written. ids as frx_route_topk wrote them: a slot whose token was dropped later (an expert
+ * over its capacity) keeps its id here and has the gradient 0 in gwts. An id outside [0, E) has no logit, and an expert named
+ * twice gets the sum of both. E <= 1024, k <= 32. No counterpart in the reference, which does not train. */
+int frx_route_topk_backward(frx_stream_t stream, const float* gwts, const float* wts, const int32_t* ids, int T, int E, int k, float* glogits);
+
+/* ---- tokens sorted by expert, and back (the reference groups inside moe_q2::run and gemm::moe_prepare and has no such entry)
+ * For programs that run experts of their own between the two. A slot s = t * K + k is one of the T * K (token, expert) pairs; rows
+ * are numbered expert after expert, within an expert in slot order.
+ * frx_moe_sort: ids [T][K] -> offsets [E + 1] (the rows of expert e are offsets[e] .. offsets[e + 1] - 1), row_of [T][K] (the row of a
+ * slot) and slot_of [T * K] (the slot of a row). A slot with a negative id (a dropped or padded one, an expert that lives elsewhere)
+ * has no row: row_of is -1 there, and slot_of is -1 for the rows behind offsets[E]. An id of E or more has no row either and is reported by
+ * frx_workspace_status. The same ids give the same plan bit for bit. K <= 32, E <= 4096, T * K < 2^31; ws 16-byte aligned. */
+size_t frx_moe_sort_workspace_bytes(int T, int K, int E);
+int frx_moe_sort(frx_stream_t stream, const int32_t* ids, int T, int K, int E, int32_t* offsets, int32_t* slot_of, int32_t* row_of, void* ws,
+                 size_t ws_bytes);
+/* The rows: of n elements of `dtype`, ld* elements apart (ld >= n; any alignment of an element: rows that are 16-byte aligned and a
+ * multiple of 16 bytes long are moved 16 bytes at a time). `rows` is how many rows the sorted buffer has; slots with no row in it
+ * (row_of < 0 or >= rows) are left out of everything. Rows that no slot has are not written. Buffers do not overlap. Sums are formed in 32 bits, in
+ * k order, and rounded once.
+ *   sort_rows:            xs[row_of[t][k]] = x[t]
+ *   sort_rows_backward:   gx[t] = sum_k gxs[row_of[t][k]]
+ *   unsort_rows:          out[t] = sum_k wts[t][k] * ys[row_of[t][k]]
+ *   unsort_rows_backward: gys[row_of[t][k]] = wts[t][k] * gout[t], gwts[t][k] = <gout[t], ys[row_of[t][k]]> (float; 0 without a row) */
+int frx_moe_sort_rows(frx_stream_t stream, const void* x, int64_t ldx, int dtype, const int32_t* row_of, int T, int K, int n, void* xs, int64_t ldxs,
+                      int64_t rows);
+int frx_moe_sort_rows_backward(frx_stream_t stream, const void* gxs, int64_t ldgxs, int64_t rows, int dtype, const int32_t* row_of, int T, int K,
+                               int n, void* gx, int64_t ldgx);
+int frx_moe_unsort_rows(frx_stream_t stream, const void* ys, int64_t ldys, int64_t rows, int dtype, const float* wts, const int32_t* row_of, int T,
+                        int K, int n, void* out, int64_t ldo);
+int frx_moe_unsort_rows_backward(frx_stream_t stream, const void* gout, int64_t ldg, const void* ys, int64_t ldys, int64_t rows, int dtype,
+                                 const float* wts, const int32_t* row_of, int T, int K, int n, void* gys, int64_t ldgys, float* gwts);
 
 /* ---- activation quantizer: q2_0::quantize_q8 (quant/q2_0/q2_0.cpp:101-117) ----
  * Per 32 values: d = amax / 127, q = roundf(x / d) (half away from zero), d stored after a
@@ -514,6 +551,47 @@ int frx_gemm_moe_run(const frx_gemm_moe_plan* plan, const void* W, int64_t exper
 int frx_gemm_moe(uint32_t ggml_type, const void* W, int64_t expert_stride_bytes, int n_experts, const float* x, int x_per_slot,
                  const int32_t* ids, int64_t T, int K, float* y, int64_t ncols, int64_t nrows, void* ws, size_t ws_bytes,
                  frx_stream_t stream);
+
+/* ---- MXFP4: the OCP microscaling format of 4 bits, which the tensor cores multiply as it is. For experts (or dense layers) in that format
+ * beside the Q2_0 ones; the reference has no counterpart.
+ * Blocks of 32 values along a row share a scale 2^e, held as the byte e + 127: e = floor(log2(largest magnitude)) - 2, at least -127. An element
+ * is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign (E2M1: sign, two bits of exponent, one of mantissa), the value / 2^e to nearest, ties to the
+ * even code, beyond 6 the 6. Codes [rows][n / 2] bytes, the earlier element in the low half; scales [rows][n / 32] bytes. A block with
+ * a NaN or an infinity in it has the scale byte 255 and codes 0: all its values are NaN. Codes are 16-byte aligned (4-byte for the dequantizer),
+ * scales 4-byte aligned in the product. n % 32 == 0; in the product and the layer n % 128 == 0. */
+/* x [T] rows of n elements of dtype, ldx elements apart (any alignment of an element; 16-byte aligned rows are faster) -> codes, scales */
+int frx_mxfp4_quantize(frx_stream_t stream, const void* x, int64_t ldx, int dtype, int T, int n, void* codes, void* scales);
+/* and the values that they stand for, FRX_F32 or FRX_BF16 (both hold each of them exactly; the scale bytes 253 and 254, which the
+ * quantizer never gives, can leave their range) */
+int frx_mxfp4_dequantize(frx_stream_t stream, const void* codes, const void* scales, int T, int n, int dtype, void* x, int64_t ldx);
+/* The layout of a product's matrices, made once when they are loaded. codes [E][rows][n / 2], scales [E][rows][n / 32] -> E packed matrices of
+ * frx_mxfp4_packed_bytes(rows, n) bytes. A packed matrix is tiles of 128 rows (the last one filled up with zeros), a tile is the units
+ * u = 0 .. n / 128 - 1 of 128 columns, a unit is 8,704 bytes, which one bulk copy brings into shared memory as the tensor core reads it:
+ *   [0, 8192):    four planes c of 32 columns, 16 bytes of codes a row: columns 128 u + 32 c .. + 31 of row r at 2048 c + 16 r;
+ *   [8192, 8704): the scale of the same block at 16 (r % 32) + 4 (r / 32) + c.
+ * unpack is the inverse. E * tiles * units < 2^31. */
+size_t frx_mxfp4_packed_bytes(int rows, int n);
+int frx_mxfp4_pack(frx_stream_t stream, const void* codes, const void* scales, int E, int rows, int n, void* packed);
+int frx_mxfp4_unpack(frx_stream_t stream, const void* packed, int E, int rows, int n, void* codes, void* scales);
+/* y[t] = W x[t]: x [T] rows of n values in MXFP4, W one packed matrix [rows][n], y [T] rows of `rows` elements of dtype, ldy apart. Products are
+ * exact, sums are formed in 32 bits on the tensor cores and rounded once to dtype. Any T and any number of rows. */
+int frx_mxfp4_matmul(frx_stream_t stream, const void* codes, const void* scales, int T, int n, const void* packed, int rows, void* y, int64_t ldy,
+                     int dtype);
+/* The same by expert: for the rows r = offsets[e] .. offsets[e + 1] - 1 of expert e (frx_moe_sort) y[r] = W_e x[slot_of[r] / K], or W_e x[r] where
+ * slot_of is null (then K is 1). x has T rows, y has S. The sorted rows of x are never written anywhere: they are read through slot_of. Rows of y that no
+ * expert has (behind offsets[E]) are not written. offsets are taken to lie in [0, S], ascending, and slot_of to name rows of x: what lies outside is left
+ * out (such a row of y holds anything). E <= 4096. */
+int frx_mxfp4_moe_matmul(frx_stream_t stream, const void* codes, const void* scales, int T, int n, const void* packed, int E, int rows,
+                         const int32_t* offsets, const int32_t* slot_of, int K, int S, void* y, int64_t ldy, int dtype);
+/* The expert layer with experts in MXFP4, from the routing to the combined rows in one call:
+ *   out[t] = sum over k of wts[t][k] * W_down Q(silu(W_gate Q(x_t)) * (W_up Q(x_t))) of expert ids[t][k], Q the quantizer above.
+ * w_gate, w_up: E packed matrices [ff][n], w_down: E packed [n][ff]. x, out: rows of n elements of their dtype, ld* apart. Slots with a negative id take
+ * no part (a token without any gets zeros); an id of E or more is left out too and reported by frx_workspace_status. The experts' rows are kept in
+ * bfloat16 where out is, else in float. The hidden rows' codes are those of sums in 32 bits: where such a sum lies within its error of a border between
+ * two codes, the code may be either. Any T; K <= 32, E <= 4096, n and ff multiples of 128 up to 2^20, T * K < 2^31. ws 16-byte aligned. */
+size_t frx_mxfp4_moe_layer_workspace_bytes(int T, int K, int n, int ff, int E);
+int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_up, const void* w_down, int E, int n, int ff, const void* x, int64_t ldx,
+                        int x_dtype, const int32_t* ids, const float* wts, int T, int K, void* out, int64_t ldo, int out_dtype, void* ws, size_t ws_bytes);
 
 /* convert_q8_0_to_q2_0 (arch/qwen4exp/mtp.hpp:40, mtp.cu:129-215) on the device: nblocks64 pairs of
  * Q8_0 blocks {fp16 d; 32 int8} (68 bytes) -> ggml Q2_0 blocks (18 bytes): for each 64 values the
