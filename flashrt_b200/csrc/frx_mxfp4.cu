@@ -1,11 +1,13 @@
 // MXFP4: the quantizer, the way back, the layout that the product reads, the product (dense, and grouped by expert), and
 // the expert layer made of them.
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 #include "frx_mx.cuh"
 #include "frx_rows.cuh"
 #include "frx_sort.cuh"
+#include "frx_umma.cuh"
 
 namespace frx {
 namespace {
@@ -105,112 +107,470 @@ __global__ void __launch_bounds__(kMxTileRows) k_mx_pack(uint4* __restrict__ cod
         scales[at] = *scale;
 }
 
-// ---- product
+// ---- product on the tensor cores
+//
+// A tile is 256 matrix rows (two row tiles of 128: the M of the instruction, or the gate and the up tile of 128 hidden rows) by
+// up to 112 y rows of one expert (its N), so weights are read once per 112 rows and an expert with few rows costs what its weights
+// cost. kind::mxf4 multiplies 64 columns per instruction with the block scales in tensor memory. A stage of the ring is 128 columns:
+// per row tile one 8,704-byte unit of the packed layout, brought by one bulk copy, and the y rows' codes (64 bytes each) and scale
+// words, gathered by cp.async through slot_of. Tensor memory: two sets of accumulators (2 x 2 x 112 columns), so that a tile's
+// epilogue runs beside the next tile's products, and four sets of scales (16 columns each).
+constexpr int kTok = 112;                 // y rows of a tile at most
+constexpr int kRowTiles = 2;              // row tiles of a tile
+constexpr int kStageW = kRowTiles * kMxUnitBytes, kStageB = 4 * kTok * 16, kStageBytes = kStageW + kStageB + 512;
+constexpr int kMaxStages = 8, kLag = 4;   // stages; a stage's gathered rows are handed on kLag stages after their copies were issued
+constexpr int kWarpsEpi = 8, kWarpW = 8, kWarpMma = 9, kWarpAct = 10, kWarpsAct = 4;
+constexpr int kMxThreads = 32 * (kWarpAct + kWarpsAct);
+constexpr int kColsAcc = kRowTiles * kTok, kColScale = 2 * kColsAcc, kScaleSets = 4, kColsScale = 16;
+static_assert(kColScale + kScaleSets * kColsScale <= 512, "tensor memory has 512 columns");
+static_assert(kTok % 16 == 0 && kTok <= 128, "the tokens' scales of a unit are one block of 512 bytes");
+// barriers, 8 bytes each, then the abort flag, the address of the tensor memory and the scan's sums
+constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBars = kBarDFree + 2;
+constexpr int kSmemHead = 256 + 64;
+
+enum { kYf32 = FRX_F32, kYbf16 = FRX_BF16, kYf16 = FRX_F16, kYswiglu = 3 };
+
 struct MxProduct {
-    const uint8_t* w;        // packed matrices
+    const uint8_t* w[2];     // packed matrices; the second: the up matrices of the SwiGLU form
     const uint8_t* codes;    // activations [x_rows][n / 2]
     const uint8_t* scales;   // [x_rows][n / 32]
     const int32_t* offsets;  // [E + 1] rows of every expert; null: one matrix, all rows
     const int32_t* slot_of;  // the x row of sorted row r is slot_of[r] / K; null: r
     void* y;
+    uint8_t* y_scales;       // SwiGLU form
     int64_t ldy;
+    int* status;             // of a workspace, or null
+    unsigned long long wait_ns;
     int E, rows, n, K, x_rows, S;   // rows: of a matrix; S: rows of y
-    int y_type;
+    int stages;
 };
 
-__device__ __forceinline__ void store_y(const MxProduct& p, int64_t r, int row, float v) {
-    if (p.y_type == FRX_F32)
-        static_cast<float*>(p.y)[r * p.ldy + row] = v;
-    else if (p.y_type == FRX_BF16)
-        static_cast<__nv_bfloat16*>(p.y)[r * p.ldy + row] = __float2bfloat16_rn(v);
-    else
-        static_cast<__half*>(p.y)[r * p.ldy + row] = __float2half_rn(v);
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Instruction descriptor of kind::mxf4 with scales of 32: A and B E2M1 (1), scales UE8M0, both K-major, D fp32 128 x n; the byte pair of
+// the scale words that belongs to these 64 columns is part of it.
+__device__ __forceinline__ uint32_t mx_idesc(int n, int pair) {
+    return (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (1u << 23) | (uint32_t(kMxTileRows >> 4) << 24) | (uint32_t(2 * pair) << 4) | (uint32_t(2 * pair) << 29);
+}
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+        : "memory");
+}
+// 512 bytes (32 rows of 16) to four columns of tensor memory, the same in all four quarters of its lanes. In order with the MMAs of the issuing thread.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// 16 columns of this warp's lanes from two places, complete on return
+__device__ __forceinline__ void tmem_ld16x2(uint32_t a0, uint32_t a1, uint32_t (&v)[16], uint32_t (&w)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+          "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]), "=r"(w[8]), "=r"(w[9]),
+          "=r"(w[10]), "=r"(w[11]), "=r"(w[12]), "=r"(w[13]), "=r"(w[14]), "=r"(w[15])
+        : "r"(a0), "r"(a1)
+        : "memory");
 }
 
-// A thread per matrix row and eight y rows.
-__global__ void __launch_bounds__(kMxTileRows) k_mx_product(const MxProduct p) {
-    __shared__ int item[3];
+// The tiles of a block, one after the other: expert after expert, within one row pair after row pair, within these the blocks of y rows
+// (so that blocks that share weights run at the same time). tile_end[e]: tiles of the experts up to e; first[e]: the expert's first row.
+struct MxWalk {
+    const int *tile_end, *first;
+    int E, pairs, tile, e;
+    int rp, row0, live, width;   // row pair, first y row, y rows, their number rounded up to 16
+    __device__ __forceinline__ void begin(const int* ends, const int* rows, int experts, int row_pairs) {
+        tile_end = ends;
+        first = rows;
+        E = experts;
+        pairs = row_pairs;
+        tile = int(blockIdx.x) - int(gridDim.x);
+        e = 0;
+    }
+    __device__ __forceinline__ bool next() {
+        tile += int(gridDim.x);
+        const int lane = threadIdx.x & 31;
+        while (e < E) {   // 32 experts at a time: those that end at or before the tile
+            const unsigned done = __ballot_sync(0xffffffffu, e + lane < E && tile_end[e + lane] <= tile);
+            e += __popc(done);
+            if (done != 0xffffffffu) break;
+        }
+        if (e >= E) return false;
+        const int t0 = e ? tile_end[e - 1] : 0, a = first[e], count = first[E + 1 + e], blocks = (count + kTok - 1) / kTok, local = tile - t0;
+        const int b = local % blocks;
+        rp = local / blocks;
+        width = ((count + blocks - 1) / blocks + 15) & ~15;   // as even as multiples of 16 allow
+        row0 = a + b * width;
+        live = min(width, count - b * width);
+        width = (live + 15) & ~15;
+        return true;
+    }
+};
+
+// y of 16 y rows for one matrix row a lane: y points at the matrix row's element of the first y row
+template <int MODE>
+__device__ __forceinline__ void store16(const uint32_t (&v)[16], void* y, int64_t ldy, int live, bool have, bool pairs) {
+    if (MODE == kYf32) {
+        float* p = static_cast<float*>(y);
+#pragma unroll
+        for (int i = 0; i < 16; ++i, p += ldy)
+            if (i < live && have) *p = __uint_as_float(v[i]);
+        return;
+    }
+    const bool odd = threadIdx.x & 1;
+    if (pairs) {   // two lanes exchange a value so that each has two neighbouring matrix rows of one y row
+        uint16_t* p = static_cast<uint16_t*>(y) + (odd ? ldy - 1 : 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i, p += 2 * ldy) {
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? v[2 * i] : v[2 * i + 1], 1);
+            const float lo = __uint_as_float(odd ? got : v[2 * i]), hi = __uint_as_float(odd ? v[2 * i + 1] : got);
+            uint32_t w;
+            if (MODE == kYbf16) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+                w = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(lo, hi);
+                w = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            if (2 * i + int(odd) < live && have) *reinterpret_cast<uint32_t*>(p) = w;
+        }
+        return;
+    }
+    uint16_t* p = static_cast<uint16_t*>(y);
+#pragma unroll
+    for (int i = 0; i < 16; ++i, p += ldy)
+        if (i < live && have) {
+            if (MODE == kYbf16)
+                *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(__uint_as_float(v[i]));
+            else
+                *reinterpret_cast<__half*>(p) = __float2half_rn(__uint_as_float(v[i]));
+        }
+}
+
+// silu(g) * u of eight y rows for one hidden row a lane; the warp's 32 hidden rows are one block. codes: where this lane's word goes,
+// four bytes (eight hidden rows) of y row lane % 8; scale: that row's scale byte, of lane < 8.
+__device__ __forceinline__ void swiglu8(const uint32_t* g, const uint32_t* u, uint32_t& codes, uint32_t& scale) {
+    float h[8];
+    uint32_t bytes[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // exp and the reciprocal to about 2^-22, like the sums that they are taken of
+        const float a = __uint_as_float(g[i]);
+        const float v = __fdividef(a, 1.0f + __expf(-a)) * __uint_as_float(u[i]);
+        const uint32_t byte = mx_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
+        bytes[i / 4] |= byte << (8 * (i % 4));
+        h[i] = byte == 255u ? 0.0f : v * mx_inverse(byte);
+    }
+    // lane l has the codes of row l for eight y rows, one a nibble; wanted: y row l % 8 for the eight hidden rows of its lanes
+    const unsigned lane = threadIdx.x & 31u;
+    uint32_t w = mx_codes8(h), other = __shfl_xor_sync(0xffffffffu, w, 4);
+    w = __byte_perm(w, other, lane & 4u ? 0x3276 : 0x5410);
+    other = __shfl_xor_sync(0xffffffffu, w, 2);
+    w = __byte_perm(w, other, lane & 2u ? 0x3715 : 0x6240);
+    other = __shfl_xor_sync(0xffffffffu, w, 1);
+    codes = lane & 1u ? ((other >> 4) & 0x0f0f0f0fu) | (w & 0xf0f0f0f0u) : (w & 0x0f0f0f0fu) | ((other & 0x0f0f0f0fu) << 4);
+    scale = (bytes[(lane >> 2) & 1u] >> (8u * (lane & 3u))) & 255u;
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const uint32_t s0 = smem_u32(smem), stages0 = s0 + kSmemHead, bars = s0, abort = s0 + 240;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 240);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 244);
+    int* warp_sums = reinterpret_cast<int*>(smem + 256);   // 14 of them
+    const uint32_t n_stages = uint32_t(p.stages);
+    int* tile_end = reinterpret_cast<int*>(smem + kSmemHead + n_stages * kStageBytes);   // [E], then first rows [E + 1], then row counts [E]
+    int* first = tile_end + p.E;
+    const int units = p.n / kMxUnitK;
+    const int row_tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, row_pairs = MODE == kYswiglu ? row_tiles : (row_tiles + 1) / 2;
+    static_assert(kBars * 8 <= 240, "the barriers' block");
+
+    if (threadIdx.x == 0) {
+        uint64_t* b = reinterpret_cast<uint64_t*>(smem);
+        for (int i = 0; i < kMaxStages; ++i) {
+            mbar_init(b + kBarFull + i, 1 + kWarpsAct);
+            mbar_init(b + kBarFree + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(b + kBarDFull + i, 1);
+            mbar_init(b + kBarDFree + i, kWarpsEpi);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == kWarpMma) tmem_alloc(tmem_slot, 512);
     pdl_wait();
     pdl_trigger();
-    if (threadIdx.x == 0) {
-        int left = int(blockIdx.x), e = 0, a = 0, b = p.offsets ? 0 : p.S;
-        item[0] = -1;
-        for (; e < p.E; ++e) {
-            if (p.offsets) {
+    // tiles of every expert: a thread takes a few experts in a row
+    {
+        const int per = (p.E + kMxThreads - 1) / kMxThreads, e0 = min(p.E, int(threadIdx.x) * per), e1 = min(p.E, e0 + per);
+        int sum = 0;
+        for (int e = e0; e < e1; ++e) {
+            int a = 0, b = p.S;
+            if (p.offsets) {   // (what a plan says beyond the rows that there are is left out)
                 a = min(max(p.offsets[e], 0), p.S);
                 b = min(max(p.offsets[e + 1], a), p.S);
             }
-            const int items = (b - a + 7) / 8;
-            if (left < items) {
-                item[0] = e;
-                item[1] = a + left * 8;
-                item[2] = min(8, b - item[1]);
-                break;
+            first[e] = a;
+            first[p.E + 1 + e] = b - a;
+            sum += (b - a + kTok - 1) / kTok * row_pairs;
+            tile_end[e] = sum;
+        }
+        int inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += up;
+        }
+        if (lane == 31) warp_sums[warp] = inc;
+        __syncthreads();
+        int before = inc - sum;
+        for (int i = 0; i < warp; ++i) before += warp_sums[i];
+        for (int e = e0; e < e1; ++e) tile_end[e] += before;
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    MxWalk t;
+    t.begin(tile_end, first, p.E, row_pairs);
+
+    // "free" barriers are waited on with the parity of the phase before the one about to be used, which a fresh barrier reports as complete
+    if (warp == kWarpW) {
+        // ---------------- weights: one lane, a bulk copy per row tile and stage
+        uint32_t st = 0, phase = 1;
+        const size_t tile_bytes = size_t(units) * kMxUnitBytes;
+        while (t.next()) {
+            const uint8_t *w0, *w1;
+            bool second = true;
+            if (MODE == kYswiglu) {
+                const size_t at = (size_t(t.e) * row_tiles + t.rp) * tile_bytes;
+                w0 = p.w[0] + at;
+                w1 = p.w[1] + at;
+            } else {
+                w0 = p.w[0] + (size_t(t.e) * row_tiles + 2 * t.rp) * tile_bytes;
+                w1 = w0 + tile_bytes;
+                second = 2 * t.rp + 1 < row_tiles;
             }
-            left -= items;
+            for (int u = 0; u < units; ++u) {
+                const uint32_t full = bars + (kBarFull + st) * 8, dst = stages0 + st * kStageBytes;
+                mbar_spin(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns);
+                if (lane == 0) {
+                    mbar_expect_tx(full, second ? 2 * kMxUnitBytes : kMxUnitBytes);
+                    bulk_g2s(dst, w0, kMxUnitBytes, full);
+                    if (second) bulk_g2s(dst + kMxUnitBytes, w1, kMxUnitBytes, full);
+                }
+                __syncwarp();
+                w0 += kMxUnitBytes;
+                w1 += kMxUnitBytes;
+                if (++st == n_stages) st = 0, phase ^= 1u;
+            }
+        }
+    } else if (warp >= kWarpAct) {
+        // ---------------- activations: y rows in groups of eight, groups dealt to the warps; lane: row lane % 8, 16 bytes lane / 8 of its 64.
+        // Generic-proxy writes: each lane waits for its own copies and makes them visible to the tensor core before the arrival.
+        const int aw = warp - kWarpAct;
+        constexpr int kGroups = (kTok / 8 + kWarpsAct - 1) / kWarpsAct;
+        uint32_t st = 0, phase = 1, hand = 0, pending = 0;
+        const size_t row_codes = size_t(p.n / 2), row_scales = size_t(p.n / kMxBlock);
+        auto hand_on = [&]() {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + (kBarFull + hand) * 8);
+            if (++hand == n_stages) hand = 0;
+            --pending;
+        };
+        while (t.next()) {
+            const int groups = t.width >> 3;
+            int row[kGroups];   // of group aw + 4 i: the x row of y row lane % 8 (beyond the live ones the last again)
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                const int r = t.row0 + min((aw + i * kWarpsAct) * 8 + (lane & 7), t.live - 1);
+                int x = r;
+                if (p.slot_of) {
+                    const int slot = p.slot_of[r];
+                    x = slot < 0 ? 0 : slot / p.K;
+                }
+                row[i] = x < p.x_rows ? x : 0;
+            }
+            // scales: lane / 8 is the group, lane % 8 the row in it
+            int srow = row[0];
+#pragma unroll
+            for (int i = 1; i < kGroups; ++i)
+                if (lane >> 3 == i) srow = row[i];
+            const int stok = (aw + (lane >> 3) * kWarpsAct) * 8 + (lane & 7);
+            const bool s_on = (lane >> 3) < kGroups && stok < t.width;
+            const uint8_t* ssrc = p.scales + size_t(srow) * row_scales;
+            const uint32_t sdst = kStageW + kStageB + (stok & 31) * 16 + (stok >> 5) * 4;
+            const uint8_t* src[kGroups];
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) src[i] = p.codes + size_t(row[i]) * row_codes + (lane >> 3) * 16;
+            for (int u = 0; u < units; ++u) {
+                mbar_spin(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns);
+                const uint32_t dst = stages0 + st * kStageBytes;
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i) {
+                    const int grp = aw + i * kWarpsAct;
+                    if (grp < groups) cp_async16(dst + kStageW + (lane >> 3) * (kTok * 16) + (grp * 8 + (lane & 7)) * 16, src[i] + size_t(u) * 64);
+                }
+                if (s_on) cp_async4(dst + sdst, ssrc + u * 4);
+                cp_async_commit();
+                if (++st == n_stages) st = 0, phase ^= 1u;
+                ++pending;
+                cp_async_wait<kLag>();
+                if (pending > kLag) hand_on();
+            }
+        }
+        cp_async_wait<0>();
+        while (pending) hand_on();
+    } else if (warp == kWarpMma) {
+        // ---------------- MMA: one elected lane issues, the warp stays together
+        uint32_t st = 0, phase = 0, set = 0, sc = 0, dphase = 1;
+        while (t.next()) {
+            const uint32_t id0 = mx_idesc(t.width, 0), id1 = mx_idesc(t.width, 1);
+            const bool second = MODE == kYswiglu || 2 * t.rp + 1 < row_tiles;
+            mbar_spin(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns);
+            const uint32_t acc = tmem + set * kColsAcc;
+            for (int u = 0; u < units; ++u) {
+                mbar_spin(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns);
+                tc_fence_after_sync();
+                if (elect_one()) {
+                    const uint32_t base = stages0 + st * kStageBytes, sf = tmem + kColScale + sc * kColsScale;
+                    tmem_copy_scales(sf, umma_desc(base + kMxUnitCode, 128, 128));
+                    if (second) tmem_copy_scales(sf + 4, umma_desc(base + kMxUnitBytes + kMxUnitCode, 128, 128));
+                    tmem_copy_scales(sf + 8, umma_desc(base + kStageW + kStageB, 128, 128));
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const uint64_t db = umma_desc(base + kStageW + s * 2 * kTok * 16, kTok * 16, 128);
+                        const uint32_t on = u > 0 || s > 0;
+                        umma_mxf4(acc, umma_desc(base + s * 4096, 2048, 128), db, s ? id1 : id0, sf, sf + 8, on);
+                        if (second) umma_mxf4(acc + kTok, umma_desc(base + kMxUnitBytes + s * 4096, 2048, 128), db, s ? id1 : id0, sf + 4, sf + 8, on);
+                    }
+                    umma_commit(bars + (kBarFree + st) * 8);
+                    if (u == units - 1) umma_commit(bars + (kBarDFull + set) * 8);
+                }
+                __syncwarp();
+                if (++st == n_stages) st = 0, phase ^= 1u;
+                if (++sc == kScaleSets) sc = 0;
+            }
+            set ^= 1u;
+            if (set == 0) dphase ^= 1u;
+        }
+    } else {
+        // ---------------- epilogue: a warp has a quarter of the lanes and every other 16 y rows
+        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
+        uint32_t set = 0, phase = 0;
+        const bool pairs = MODE != kYf32 && p.rows % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
+        while (t.next()) {
+            mbar_spin(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);
+            tc_fence_after_sync();
+            const bool lost = lds32(abort) != 0;   // a wait ran out: NaN, not a wrong number
+            const uint32_t acc = tmem + (uint32_t(quarter * 32) << 16) + set * kColsAcc;
+            const int chunks = t.width >> 4;
+            for (int c = half; c < chunks; c += 2) {
+                uint32_t v[2][16];
+                tmem_ld16x2(acc + c * 16, acc + kTok + c * 16, v[0], v[1]);
+                if (lost)
+                    for (int i = 0; i < 16; ++i) v[0][i] = v[1][i] = 0x7fffffffu;
+                if (c + 2 >= chunks) {   // the sums are all in registers: the accumulators go back
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bars + (kBarDFree + set) * 8);
+                }
+                const int live = t.live - c * 16;
+                const int64_t y0 = t.row0 + c * 16;
+                if (MODE == kYswiglu) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t codes, scale;
+                        swiglu8(&v[0][8 * i], &v[1][8 * i], codes, scale);
+                        const size_t y = size_t(y0) + 8 * i + (lane & 7);
+                        const uint32_t at = uint32_t(t.rp) * kMxTileRows + quarter * 32;   // the block's first hidden row
+                        if (8 * i + (lane & 7) < live) {
+                            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + y * (p.rows / 2) + at / 2 + (lane >> 3) * 4) = codes;
+                            if (lane < 8) p.y_scales[y * (p.rows / kMxBlock) + at / kMxBlock] = uint8_t(scale);
+                        }
+                    }
+                } else {
+                    constexpr int size = MODE == kYf32 ? 4 : 2;
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        const int row = (2 * t.rp + m) * kMxTileRows + r;
+                        store16<MODE>(v[m], static_cast<uint8_t*>(p.y) + (y0 * p.ldy + row) * size, p.ldy, live, row < p.rows, pairs);
+                    }
+                }
+            }
+            if (half >= chunks) {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bars + (kBarDFree + set) * 8);
+            }
+            set ^= 1u;
+            if (set == 0) phase ^= 1u;
         }
     }
+    tc_fence_before_sync();
     __syncthreads();
-    if (item[0] < 0) return;
-    const int units = p.n / kMxUnitK, tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, r = threadIdx.x, row = blockIdx.y * kMxTileRows + r;
-    const uint8_t* w = p.w + (size_t(item[0]) * tiles + blockIdx.y) * units * kMxUnitBytes;
-    float acc[8] = {};
-    for (int u = 0; u < units; ++u, w += kMxUnitBytes)
-        for (int c = 0; c < 4; ++c) {   // a block of 32
-            const uint32_t ws = w[kMxUnitCode + (r % 32) * 16 + (r / 32) * 4 + c];
-            const uint4 wc = reinterpret_cast<const uint4*>(w)[c * kMxTileRows + r];
-            const uint32_t ww[4] = {wc.x, wc.y, wc.z, wc.w};
-            for (int j = 0; j < item[2]; ++j) {
-                const int slot = p.slot_of ? p.slot_of[item[1] + j] : (item[1] + j) * p.K;
-                const int t = slot / p.K;
-                if (slot < 0 || t >= p.x_rows) continue;
-                const size_t at = size_t(t) * (p.n / kMxBlock) + u * 4 + c;
-                float sum = 0.0f;
-                for (int q = 0; q < 4; ++q) {
-                    float a[8], b[8];
-                    mx_values8(ww[q], a);
-                    mx_values8(reinterpret_cast<const uint32_t*>(p.codes)[at * 4 + q], b);
-                    for (int i = 0; i < 8; ++i) sum = fmaf(a[i], b[i], sum);
-                }
-                acc[j] = fmaf(sum * mx_scale(ws), mx_scale(p.scales[at]), acc[j]);
-            }
+    if (*abort_flag) {
+        // A wait ran out: copies and MMAs may still be in flight. Give them time to land before tensor memory and the block's
+        // shared memory are released.
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 2000000ull) {
         }
-    if (row < p.rows)
-        for (int j = 0; j < item[2]; ++j) store_y(p, item[1] + j, row, acc[j]);
+        __syncthreads();
+        if (threadIdx.x == 0 && p.status) p.status[0] = kDevWaitTimeout;
+    }
+    if (warp == kWarpMma) tmem_free(tmem, 512);
 }
 
-int launch_product(const MxProduct& p, cudaStream_t stream, int cls) {
-    const int tiles = (p.rows + kMxTileRows - 1) / kMxTileRows;
-    const dim3 grid(unsigned((int64_t(p.S) + 7) / 8 + (p.offsets ? p.E : 0)), unsigned(tiles));
-    FRX_LAUNCH(cls, stream, launch_pdl(k_mx_product, grid, dim3(kMxTileRows), 0, stream, p));
+template <int MODE>
+int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
+    const size_t tables = (size_t(p.E) * 3 + 1) * 4;
+    const int64_t row_tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, pairs = MODE == kYswiglu ? row_tiles : (row_tiles + 1) / 2;
+    if ((int64_t(p.S) / kTok + p.E) * pairs > 0x7fff0000) return fail(FRX_ERR_SHAPE, "MXFP4 product: %d rows by %d is more than 2^31 tiles", p.S, p.rows);
+    constexpr size_t kSmem = 227 * 1024;
+    static std::mutex mu;
+    static bool done[64] = {};
+    {
+        int dev = 0;
+        FRX_CUDA(cudaGetDevice(&dev));
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev < 0 || dev >= 64 || !done[dev]) FRX_CUDA(cudaFuncSetAttribute(k_mx_product<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
+        if (dev >= 0 && dev < 64) done[dev] = true;
+    }
+    p.stages = int(std::min<size_t>(kMaxStages, (kSmem - kSmemHead - tables) / kStageBytes));
+    static_assert((kSmem - kSmemHead - (4096 * 3 + 1) * 4) / kStageBytes > kLag, "a stage must be handed on before it is needed again");
+    p.wait_ns = wait_limit_ns();
+    const int64_t most = (int64_t(p.S) / kTok + std::min(p.E, p.S)) * pairs;   // tiles at most (every expert's last block may be a part of one)
+    const unsigned grid = unsigned(std::min<int64_t>(sm_count(), std::max<int64_t>(1, most)));
+    FRX_LAUNCH(cls, stream, launch_pdl(k_mx_product<MODE>, dim3(grid), dim3(kMxThreads), kSmemHead + size_t(p.stages) * kStageBytes + tables, stream, p));
     FRX_CUDA(cudaGetLastError());
     return FRX_OK;
 }
-
-// h = silu(g) * u of the rows that experts have, to MXFP4: a warp per block of 32
-__global__ void __launch_bounds__(256) k_mx_swiglu(const float* __restrict__ g, const float* __restrict__ u, const int32_t* __restrict__ n_rows, int ff, uint32_t* __restrict__ codes,
-                                                   uint8_t* __restrict__ scales) {
-    pdl_wait();
-    pdl_trigger();
-    const size_t b = size_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const uint32_t lane = threadIdx.x & 31u;
-    if (b >= size_t(*n_rows) * (ff / kMxBlock)) return;
-    const float a = g[b * kMxBlock + lane], v = a / (1.0f + expf(-a)) * u[b * kMxBlock + lane];
-    const uint32_t byte = mx_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-    const float mine = v * mx_inverse(min(byte, 253u));
-    float f[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = __shfl_sync(0xffffffffu, mine, (lane & ~7u) + j);
-    const uint32_t w = byte == 255u ? 0u : mx_codes8(f);
-    if ((lane & 7u) == 0) codes[b * 4 + lane / 8] = w;
-    if (lane == 0) scales[b] = uint8_t(byte);
+int launch_product(MxProduct& p, int mode, cudaStream_t stream, int cls) {
+    switch (mode) {
+        case kYf32: return launch_mode<kYf32>(p, stream, cls);
+        case kYbf16: return launch_mode<kYbf16>(p, stream, cls);
+        case kYf16: return launch_mode<kYf16>(p, stream, cls);
+        default: return launch_mode<kYswiglu>(p, stream, cls);
+    }
 }
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 // where the layer keeps what it forms, in its workspace
 struct LayerBuffers {
-    size_t offsets, slot_of, row_of, sort, xq, xs, hq, hs, g, u, y, total;
+    size_t offsets, slot_of, row_of, sort, xq, xs, hq, hs, y, total;
 };
 LayerBuffers layer_buffers(int T, int K, int n, int ff, int E) {
     LayerBuffers b{};
@@ -228,8 +588,6 @@ LayerBuffers layer_buffers(int T, int K, int n, int ff, int E) {
     take(b.xs, size_t(T) * n / kMxBlock);
     take(b.hq, S * ff / 2);
     take(b.hs, S * ff / kMxBlock);
-    take(b.g, S * ff * 4);
-    take(b.u, S * ff * 4);
     take(b.y, S * n * 4);
     b.total = at;
     return b;
@@ -343,7 +701,7 @@ int frx_mxfp4_matmul(frx_stream_t stream, const void* codes, const void* scales,
     const int rc = product_args(who, codes, scales, packed, T, n, 1, rows, y, ldy, dtype);
     if (rc != FRX_OK) return rc;
     MxProduct p{};
-    p.w = static_cast<const uint8_t*>(packed);
+    p.w[0] = static_cast<const uint8_t*>(packed);
     p.codes = static_cast<const uint8_t*>(codes);
     p.scales = static_cast<const uint8_t*>(scales);
     p.y = y;
@@ -354,8 +712,7 @@ int frx_mxfp4_matmul(frx_stream_t stream, const void* codes, const void* scales,
     p.K = 1;
     p.x_rows = T;
     p.S = T;
-    p.y_type = dtype;
-    return launch_product(p, stream, kKGateUp);
+    return launch_product(p, dtype, stream, kKGateUp);
 }
 
 int frx_mxfp4_moe_matmul(frx_stream_t stream, const void* codes, const void* scales, int T, int n, const void* packed, int E, int rows, const int32_t* offsets,
@@ -363,12 +720,12 @@ int frx_mxfp4_moe_matmul(frx_stream_t stream, const void* codes, const void* sca
     const char* who = "frx_mxfp4_moe_matmul";
     if (S < 0 || T < 0 || K < 1) return fail(FRX_ERR_ARG, "%s: S %d, T %d, K %d", who, S, T, K);
     if (!slot_of && (K != 1 || T < S)) return fail(FRX_ERR_ARG, "%s: %d rows of x for %d sorted rows (without slot_of row r of y is of row r of x, K 1)", who, T, S);
-    if (S == 0 && n > 0 && n % kMxUnitK == 0 && rows > 0 && dtype_size(dtype)) return FRX_OK;
+    if ((S == 0 || T == 0) && n > 0 && n % kMxUnitK == 0 && rows > 0 && dtype_size(dtype)) return FRX_OK;
     const int rc = product_args(who, codes, scales, packed, T, n, E, rows, y, ldy, dtype);
     if (rc != FRX_OK) return rc;
     if (!offsets) return fail(FRX_ERR_ARG, "%s: null pointer (offsets)", who);
     MxProduct p{};
-    p.w = static_cast<const uint8_t*>(packed);
+    p.w[0] = static_cast<const uint8_t*>(packed);
     p.codes = static_cast<const uint8_t*>(codes);
     p.scales = static_cast<const uint8_t*>(scales);
     p.offsets = offsets;
@@ -381,8 +738,7 @@ int frx_mxfp4_moe_matmul(frx_stream_t stream, const void* codes, const void* sca
     p.K = K;
     p.x_rows = T;
     p.S = S;
-    p.y_type = dtype;
-    return launch_product(p, stream, kKGateUp);
+    return launch_product(p, dtype, stream, kKGateUp);
 }
 
 size_t frx_mxfp4_moe_layer_workspace_bytes(int T, int K, int n, int ff, int E) {
@@ -422,18 +778,15 @@ int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_u
     p.K = K;
     p.x_rows = T;
     p.S = S;
-    p.y_type = FRX_F32;
-    p.ldy = ff;
-    for (int i = 0; i < 2; ++i) {
-        p.w = static_cast<const uint8_t*>(i ? w_up : w_gate);
-        p.y = base + (i ? b.u : b.g);
-        if ((rc = launch_product(p, stream, kKGateUp)) != FRX_OK) return rc;
-    }
-    FRX_LAUNCH(kKQuant, stream, launch_pdl(k_mx_swiglu, dim3(unsigned((size_t(S) * (ff / 32) + 7) / 8)), dim3(256), 0, stream, reinterpret_cast<const float*>(base + b.g),
-                                           reinterpret_cast<const float*>(base + b.u), (const int32_t*)(offsets + E), ff, reinterpret_cast<uint32_t*>(base + b.hq), base + b.hs));
+    p.w[0] = static_cast<const uint8_t*>(w_gate);
+    p.w[1] = static_cast<const uint8_t*>(w_up);
+    p.y = base + b.hq;
+    p.y_scales = base + b.hs;
+    p.status = reinterpret_cast<int*>(base);
+    if ((rc = launch_product(p, kYswiglu, stream, kKGateUp)) != FRX_OK) return rc;
     // an expert's rows are kept in bfloat16 on their way to a bfloat16 sum: that rounding is half of what such a sum is rounded to anyway,
     // and the rows are the largest thing that the layer writes and reads
-    p.w = static_cast<const uint8_t*>(w_down);
+    p.w[0] = static_cast<const uint8_t*>(w_down);
     p.codes = base + b.hq;
     p.scales = base + b.hs;
     p.slot_of = nullptr;
@@ -443,9 +796,9 @@ int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_u
     p.x_rows = S;
     p.y = base + b.y;
     p.ldy = n;
-    p.y_type = out_dtype == FRX_BF16 ? FRX_BF16 : FRX_F32;
-    if ((rc = launch_product(p, stream, kKDown)) != FRX_OK) return rc;
-    return rows_back(base + b.y, n, p.y_type, wts, row_of, S, T, K, n, out, ldo, out_dtype, stream);
+    const int y_type = out_dtype == FRX_BF16 ? FRX_BF16 : FRX_F32;
+    if ((rc = launch_product(p, y_type, stream, kKDown)) != FRX_OK) return rc;
+    return rows_back(base + b.y, n, y_type, wts, row_of, S, T, K, n, out, ldo, out_dtype, stream);
 }
 
 }  // extern "C"
