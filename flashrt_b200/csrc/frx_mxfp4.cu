@@ -117,16 +117,20 @@ __global__ void __launch_bounds__(kMxTileRows) k_mx_pack(uint4* __restrict__ cod
 // epilogue runs beside the next tile's products, and four sets of scales (16 columns each).
 constexpr int kTok = 112;                 // y rows of a tile at most
 constexpr int kRowTiles = 2;              // row tiles of a tile
-constexpr int kStageW = kRowTiles * kMxUnitBytes, kStageB = 4 * kTok * 16, kStageBytes = kStageW + kStageB + 512;
-constexpr int kMaxStages = 8, kLag = 4;   // stages; a stage's gathered rows are handed on kLag stages after their copies were issued
-constexpr int kWarpsEpi = 8, kWarpW = 8, kWarpMma = 9, kWarpAct = 10, kWarpsAct = 4;
+constexpr int kStageUnits = 2;            // units of a stage
+constexpr int kPlaneB = kTok * 16 + 64, kUnitB = 4 * kPlaneB + 512;   // the y rows' codes of 32 columns (64 bytes keep planes off each other's banks); codes and scales of a unit
+constexpr int kTileW = kStageUnits * kMxUnitBytes, kStageW = kRowTiles * kTileW, kStageBytes = kStageW + kStageUnits * kUnitB;
+constexpr int kMaxStages = 4;
+constexpr int kWarpsEpi = 16, kWarpW = 16, kWarpMma = 17, kWarpAct = 18, kWarpsAct = 8;
 constexpr int kMxThreads = 32 * (kWarpAct + kWarpsAct);
 constexpr int kColsAcc = kRowTiles * kTok, kColScale = 2 * kColsAcc, kScaleSets = 4, kColsScale = 16;
 static_assert(kColScale + kScaleSets * kColsScale <= 512, "tensor memory has 512 columns");
+static_assert((kTok / 4 + kWarpsAct - 1) / kWarpsAct <= 8, "a lane for each row of a warp's scales");
+static_assert(kStageUnits == 2, "the scale words are taken from their four by stage");
 static_assert(kTok % 16 == 0 && kTok <= 128, "the tokens' scales of a unit are one block of 512 bytes");
 // barriers, 8 bytes each, then the abort flag, the address of the tensor memory and the scan's sums
 constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBars = kBarDFree + 2;
-constexpr int kSmemHead = 256 + 64;
+constexpr int kSmemHead = 256 + 128;   // (one word a warp)
 
 enum { kYf32 = FRX_F32, kYbf16 = FRX_BF16, kYf16 = FRX_F16, kYswiglu = 3 };
 
@@ -146,10 +150,8 @@ struct MxProduct {
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// an arrival at the barrier when all copies that this thread has issued so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 
 // Instruction descriptor of kind::mxf4 with scales of 32: A and B E2M1 (1), scales UE8M0, both K-major, D fp32 128 x n; the byte pair of
 // the scale words that belongs to these 64 columns is part of it.
@@ -168,15 +170,14 @@ __device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint
 __device__ __forceinline__ void tmem_copy_scales(uint32_t tmem, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
-// 16 columns of this warp's lanes from two places, complete on return
-__device__ __forceinline__ void tmem_ld16x2(uint32_t a0, uint32_t a1, uint32_t (&v)[16], uint32_t (&w)[16]) {
+// 8 columns of this warp's lanes from two places, complete on return
+__device__ __forceinline__ void tmem_ld8x2(uint32_t a0, uint32_t a1, uint32_t (&v)[8], uint32_t (&w)[8]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
-          "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]), "=r"(w[8]), "=r"(w[9]),
-          "=r"(w[10]), "=r"(w[11]), "=r"(w[12]), "=r"(w[13]), "=r"(w[14]), "=r"(w[15])
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]),
+          "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
         : "r"(a0), "r"(a1)
         : "memory");
 }
@@ -215,13 +216,26 @@ struct MxWalk {
     }
 };
 
-// y of 16 y rows for one matrix row a lane: y points at the matrix row's element of the first y row
+// The scale words of units u .. u + 3 of a row (as far as there are so many)
+__device__ __forceinline__ void load_words(uint32_t (&w)[4], const uint8_t* row, int u, int units, bool wide, bool on) {
+    if (!on || u >= units) return;
+    if (wide) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + u * 4));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (u + j < units) w[j] = __ldg(reinterpret_cast<const uint32_t*>(row + (u + j) * 4));
+    }
+}
+
+// y of eight y rows for one matrix row a lane: y points at the matrix row's element of the first y row
 template <int MODE>
-__device__ __forceinline__ void store16(const uint32_t (&v)[16], void* y, int64_t ldy, int live, bool have, bool pairs) {
+__device__ __forceinline__ void store8(const uint32_t (&v)[8], void* y, int64_t ldy, int live, bool have, bool pairs) {
     if (MODE == kYf32) {
         float* p = static_cast<float*>(y);
 #pragma unroll
-        for (int i = 0; i < 16; ++i, p += ldy)
+        for (int i = 0; i < 8; ++i, p += ldy)
             if (i < live && have) *p = __uint_as_float(v[i]);
         return;
     }
@@ -229,7 +243,7 @@ __device__ __forceinline__ void store16(const uint32_t (&v)[16], void* y, int64_
     if (pairs) {   // two lanes exchange a value so that each has two neighbouring matrix rows of one y row
         uint16_t* p = static_cast<uint16_t*>(y) + (odd ? ldy - 1 : 0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i, p += 2 * ldy) {
+        for (int i = 0; i < 4; ++i, p += 2 * ldy) {
             const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? v[2 * i] : v[2 * i + 1], 1);
             const float lo = __uint_as_float(odd ? got : v[2 * i]), hi = __uint_as_float(odd ? v[2 * i + 1] : got);
             uint32_t w;
@@ -246,7 +260,7 @@ __device__ __forceinline__ void store16(const uint32_t (&v)[16], void* y, int64_
     }
     uint16_t* p = static_cast<uint16_t*>(y);
 #pragma unroll
-    for (int i = 0; i < 16; ++i, p += ldy)
+    for (int i = 0; i < 8; ++i, p += ldy)
         if (i < live && have) {
             if (MODE == kYbf16)
                 *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(__uint_as_float(v[i]));
@@ -257,27 +271,39 @@ __device__ __forceinline__ void store16(const uint32_t (&v)[16], void* y, int64_
 
 // silu(g) * u of eight y rows for one hidden row a lane; the warp's 32 hidden rows are one block. codes: where this lane's word goes,
 // four bytes (eight hidden rows) of y row lane % 8; scale: that row's scale byte, of lane < 8.
-__device__ __forceinline__ void swiglu8(const uint32_t* g, const uint32_t* u, uint32_t& codes, uint32_t& scale) {
+__device__ __forceinline__ void swiglu8(const uint32_t (&g)[8], const uint32_t (&u)[8], uint32_t& codes, uint32_t& scale) {
+    const unsigned lane = threadIdx.x & 31u;
     float h[8];
-    uint32_t bytes[2] = {0u, 0u};
+    uint32_t top[8], mine = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         // exp and the reciprocal to about 2^-22, like the sums that they are taken of
         const float a = __uint_as_float(g[i]);
-        const float v = __fdividef(a, 1.0f + __expf(-a)) * __uint_as_float(u[i]);
-        const uint32_t byte = mx_scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-        bytes[i / 4] |= byte << (8 * (i % 4));
-        h[i] = byte == 255u ? 0.0f : v * mx_inverse(byte);
+        float e, r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * -1.44269504f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+        h[i] = a * r * __uint_as_float(u[i]);
+        top[i] = __reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7fffffffu);
+        mine = (lane & 7u) == unsigned(i) ? top[i] : mine;
+    }
+    scale = mx_scale_byte(mine);
+    if (__any_sync(0xffffffffu, mine - (3u << 23) >= (252u << 23))) {   // a block whose scale is at its lowest, or with a NaN or an infinity
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t byte = mx_scale_byte(top[i]);
+            h[i] = byte == 255u ? 0.0f : h[i] * mx_inverse(byte);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] *= __uint_as_float((256u << 23) - (top[i] & 0x7f800000u));   // mx_inverse of the byte e - 2
     }
     // lane l has the codes of row l for eight y rows, one a nibble; wanted: y row l % 8 for the eight hidden rows of its lanes
-    const unsigned lane = threadIdx.x & 31u;
     uint32_t w = mx_codes8(h), other = __shfl_xor_sync(0xffffffffu, w, 4);
     w = __byte_perm(w, other, lane & 4u ? 0x3276 : 0x5410);
     other = __shfl_xor_sync(0xffffffffu, w, 2);
     w = __byte_perm(w, other, lane & 2u ? 0x3715 : 0x6240);
     other = __shfl_xor_sync(0xffffffffu, w, 1);
     codes = lane & 1u ? ((other >> 4) & 0x0f0f0f0fu) | (w & 0xf0f0f0f0u) : (w & 0x0f0f0f0fu) | ((other & 0x0f0f0f0fu) << 4);
-    scale = (bytes[(lane >> 2) & 1u] >> (8u * (lane & 3u))) & 255u;
 }
 
 template <int MODE>
@@ -287,7 +313,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
     const uint32_t s0 = smem_u32(smem), stages0 = s0 + kSmemHead, bars = s0, abort = s0 + 240;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 240);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 244);
-    int* warp_sums = reinterpret_cast<int*>(smem + 256);   // 14 of them
+    int* warp_sums = reinterpret_cast<int*>(smem + 256);   // one a warp
     const uint32_t n_stages = uint32_t(p.stages);
     int* tile_end = reinterpret_cast<int*>(smem + kSmemHead + n_stages * kStageBytes);   // [E], then first rows [E + 1], then row counts [E]
     int* first = tile_end + p.E;
@@ -298,7 +324,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
     if (threadIdx.x == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(smem);
         for (int i = 0; i < kMaxStages; ++i) {
-            mbar_init(b + kBarFull + i, 1 + kWarpsAct);
+            mbar_init(b + kBarFull + i, 1 + kWarpsAct + 32 * kWarpsAct);   // the weights, a warp's scale words, a thread's copies
             mbar_init(b + kBarFree + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -362,77 +388,106 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
                 w1 = w0 + tile_bytes;
                 second = 2 * t.rp + 1 < row_tiles;
             }
-            for (int u = 0; u < units; ++u) {
-                const uint32_t full = bars + (kBarFull + st) * 8, dst = stages0 + st * kStageBytes;
+            for (int u = 0; u < units; u += kStageUnits) {
+                const uint32_t full = bars + (kBarFull + st) * 8, dst = stages0 + st * kStageBytes, bytes = uint32_t(min(kStageUnits, units - u)) * kMxUnitBytes;
                 mbar_spin(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns);
                 if (lane == 0) {
-                    mbar_expect_tx(full, second ? 2 * kMxUnitBytes : kMxUnitBytes);
-                    bulk_g2s(dst, w0, kMxUnitBytes, full);
-                    if (second) bulk_g2s(dst + kMxUnitBytes, w1, kMxUnitBytes, full);
+                    mbar_expect_tx(full, second ? 2 * bytes : bytes);
+                    bulk_g2s(dst, w0, bytes, full);
+                    if (second) bulk_g2s(dst + kTileW, w1, bytes, full);
                 }
                 __syncwarp();
-                w0 += kMxUnitBytes;
-                w1 += kMxUnitBytes;
+                w0 += kTileW;
+                w1 += kTileW;
                 if (++st == n_stages) st = 0, phase ^= 1u;
             }
         }
     } else if (warp >= kWarpAct) {
-        // ---------------- activations: y rows in groups of eight, groups dealt to the warps; lane: row lane % 8, 16 bytes lane / 8 of its 64.
-        // Generic-proxy writes: each lane waits for its own copies and makes them visible to the tensor core before the arrival.
+        // ---------------- activations: y rows in fours, dealt to the warps; a lane copies 16 of the 128 bytes that a row has in a stage.
+        // Copies report to the stage's barrier when they land; they and the scale words are generic-proxy writes: the words' writers make theirs
+        // visible to the tensor core before their arrival, for the copies the MMA thread does so behind its wait. (Warps that wait for their
+        // copies themselves hand a stage on late, which halves the ring.) A tile begins with two dependent loads, slots and then scale words;
+        // they are made during the tile in front, or the ring would run empty at every tile.
         const int aw = warp - kWarpAct;
-        constexpr int kGroups = (kTok / 8 + kWarpsAct - 1) / kWarpsAct;
-        uint32_t st = 0, phase = 1, hand = 0, pending = 0;
+        constexpr int kFours = (kTok / 4 + kWarpsAct - 1) / kWarpsAct;
         const size_t row_codes = size_t(p.n / 2), row_scales = size_t(p.n / kMxBlock);
-        auto hand_on = [&]() {
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bars + (kBarFull + hand) * 8);
-            if (++hand == n_stages) hand = 0;
-            --pending;
+        const bool s_wide = units % 4 == 0 && reinterpret_cast<uintptr_t>(p.scales) % 16 == 0;
+        const int four = lane >> 3, chunk = lane & 7;   // row of the four, 16 bytes of its 128
+        const uint32_t cdst = (chunk >> 2) * kUnitB + (chunk & 3) * kPlaneB + (aw * 4 + four) * 16;   // of the first four's copies in a stage
+        const int stok = (aw + (lane >> 2) * kWarpsAct) * 4 + (lane & 3);   // scale words: a lane has one of the warp's rows
+        const uint32_t sdst = 4 * kPlaneB + (stok & 31) * 16 + (stok >> 5) * 4;
+        uint32_t st = 0, phase = 1;
+        int slot[kFours], sslot = 0;   // of the rows (beyond the live ones the last again): their slots, or themselves
+        const uint8_t *src[kFours], *ssrc = nullptr;
+        uint32_t words[2][4];
+        auto look_up = [&]() {
+#pragma unroll
+            for (int i = 0; i < kFours; ++i) {
+                const int r = t.row0 + min((aw + i * kWarpsAct) * 4 + four, t.live - 1);
+                slot[i] = p.slot_of ? __ldg(p.slot_of + r) : r;
+            }
+            const int r = t.row0 + min(stok, t.live - 1);
+            sslot = p.slot_of ? __ldg(p.slot_of + r) : r;
         };
-        while (t.next()) {
-            const int groups = t.width >> 3;
-            int row[kGroups];   // of group aw + 4 i: the x row of y row lane % 8 (beyond the live ones the last again)
+        auto x_row = [&](int s) {
+            const int x = p.slot_of ? (s < 0 ? 0 : s / p.K) : s;
+            return size_t(x < p.x_rows ? x : 0);
+        };
+        auto rows_of_slots = [&](const uint8_t* (&to)[kFours], const uint8_t*& to_scale) {
 #pragma unroll
-            for (int i = 0; i < kGroups; ++i) {
-                const int r = t.row0 + min((aw + i * kWarpsAct) * 8 + (lane & 7), t.live - 1);
-                int x = r;
-                if (p.slot_of) {
-                    const int slot = p.slot_of[r];
-                    x = slot < 0 ? 0 : slot / p.K;
-                }
-                row[i] = x < p.x_rows ? x : 0;
-            }
-            // scales: lane / 8 is the group, lane % 8 the row in it
-            int srow = row[0];
-#pragma unroll
-            for (int i = 1; i < kGroups; ++i)
-                if (lane >> 3 == i) srow = row[i];
-            const int stok = (aw + (lane >> 3) * kWarpsAct) * 8 + (lane & 7);
-            const bool s_on = (lane >> 3) < kGroups && stok < t.width;
-            const uint8_t* ssrc = p.scales + size_t(srow) * row_scales;
-            const uint32_t sdst = kStageW + kStageB + (stok & 31) * 16 + (stok >> 5) * 4;
-            const uint8_t* src[kGroups];
-#pragma unroll
-            for (int i = 0; i < kGroups; ++i) src[i] = p.codes + size_t(row[i]) * row_codes + (lane >> 3) * 16;
-            for (int u = 0; u < units; ++u) {
-                mbar_spin(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns);
-                const uint32_t dst = stages0 + st * kStageBytes;
-#pragma unroll
-                for (int i = 0; i < kGroups; ++i) {
-                    const int grp = aw + i * kWarpsAct;
-                    if (grp < groups) cp_async16(dst + kStageW + (lane >> 3) * (kTok * 16) + (grp * 8 + (lane & 7)) * 16, src[i] + size_t(u) * 64);
-                }
-                if (s_on) cp_async4(dst + sdst, ssrc + u * 4);
-                cp_async_commit();
-                if (++st == n_stages) st = 0, phase ^= 1u;
-                ++pending;
-                cp_async_wait<kLag>();
-                if (pending > kLag) hand_on();
-            }
+            for (int i = 0; i < kFours; ++i) to[i] = p.codes + x_row(slot[i]) * row_codes + chunk * 16;
+            to_scale = p.scales + x_row(sslot) * row_scales;
+        };
+        bool more = t.next();
+        if (more) {
+            look_up();
+            rows_of_slots(src, ssrc);
+            // (a scale word of scattered rows costs an access a row, whatever its width: four units' words are loaded at a time
+            // where rows allow it)
+            load_words(words[0], ssrc, 0, units, s_wide, stok < t.width);
         }
-        cp_async_wait<0>();
-        while (pending) hand_on();
+        while (more) {
+            const int width = t.width;
+            more = t.next();
+            if (more) look_up();
+            const bool s_on = stok < width && lane < 4 * kFours;
+            const int ahead = min(2 * kStageUnits, (units - 1) / kStageUnits * kStageUnits);   // the stage behind which the next tile's rows are taken up
+            const uint8_t *next_src[kFours], *next_ssrc = nullptr;
+            uint32_t next_words[4];
+            for (int u = 0; u < units; u += kStageUnits) {
+                if ((u & 3) == 0) {
+                    if (u) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) words[0][j] = words[1][j];
+                    }
+                    load_words(words[1], ssrc, u + 4, units, s_wide, s_on);
+                }
+                mbar_spin(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns);
+                const uint32_t dst = stages0 + st * kStageBytes + kStageW, full = bars + (kBarFull + st) * 8;
+                const bool c_on = u + (chunk >> 2) < units;
+#pragma unroll
+                for (int i = 0; i < kFours; ++i)
+                    if ((aw + i * kWarpsAct) * 4 < width && c_on) cp_async16(dst + cdst + i * kWarpsAct * 64, src[i] + size_t(u) * 64);
+#pragma unroll
+                for (int k = 0; k < kStageUnits; ++k)
+                    if (s_on && u + k < units) sts32(dst + k * kUnitB + sdst, u & 2 ? words[0][2 + k] : words[0][k]);
+                cp_async_arrive(full);
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full);
+                if (++st == n_stages) st = 0, phase ^= 1u;
+                if (u == ahead && more) {
+                    rows_of_slots(next_src, next_ssrc);
+                    load_words(next_words, next_ssrc, 0, units, s_wide, stok < t.width);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kFours; ++i) src[i] = next_src[i];
+            ssrc = next_ssrc;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) words[0][j] = next_words[j];
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == kWarpMma) {
         // ---------------- MMA: one elected lane issues, the warp stays together
         uint32_t st = 0, phase = 0, set = 0, sc = 0, dphase = 1;
@@ -441,34 +496,51 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
             const bool second = MODE == kYswiglu || 2 * t.rp + 1 < row_tiles;
             mbar_spin(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns);
             const uint32_t acc = tmem + set * kColsAcc;
-            for (int u = 0; u < units; ++u) {
-                mbar_spin(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns);
-                tc_fence_after_sync();
-                if (elect_one()) {
-                    const uint32_t base = stages0 + st * kStageBytes, sf = tmem + kColScale + sc * kColsScale;
-                    tmem_copy_scales(sf, umma_desc(base + kMxUnitCode, 128, 128));
-                    if (second) tmem_copy_scales(sf + 4, umma_desc(base + kMxUnitBytes + kMxUnitCode, 128, 128));
-                    tmem_copy_scales(sf + 8, umma_desc(base + kStageW + kStageB, 128, 128));
+            if (elect_one()) {
+                uint32_t st_ = st, phase_ = phase, sc_ = sc;
+                for (int u = 0; u < units; u += kStageUnits) {
+                    mbar_spin(bars + (kBarFull + st_) * 8, phase_, abort, p.wait_ns);
+                    fence_async_smem();   // the gathered rows, which landed as generic-proxy writes
+                    tc_fence_after_sync();
+                    const uint32_t base = stages0 + st_ * kStageBytes;
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const uint64_t db = umma_desc(base + kStageW + s * 2 * kTok * 16, kTok * 16, 128);
-                        const uint32_t on = u > 0 || s > 0;
-                        umma_mxf4(acc, umma_desc(base + s * 4096, 2048, 128), db, s ? id1 : id0, sf, sf + 8, on);
-                        if (second) umma_mxf4(acc + kTok, umma_desc(base + kMxUnitBytes + s * 4096, 2048, 128), db, s ? id1 : id0, sf + 4, sf + 8, on);
+                    for (int k = 0; k < kStageUnits; ++k) {
+                        if (u + k >= units) break;
+                        const uint32_t wa = base + k * kMxUnitBytes + kMxUnitCode, sf = tmem + kColScale + ((sc_ + k) % kScaleSets) * kColsScale;
+                        tmem_copy_scales(sf, umma_desc(wa, 128, 128));
+                        if (second) tmem_copy_scales(sf + 4, umma_desc(wa + kTileW, 128, 128));
+                        tmem_copy_scales(sf + 8, umma_desc(base + kStageW + k * kUnitB + 4 * kPlaneB, 128, 128));
                     }
-                    umma_commit(bars + (kBarFree + st) * 8);
-                    if (u == units - 1) umma_commit(bars + (kBarDFull + set) * 8);
+#pragma unroll
+                    for (int k = 0; k < kStageUnits; ++k) {
+                        if (u + k >= units) break;
+                        const uint32_t wa = base + k * kMxUnitBytes, sf = tmem + kColScale + ((sc_ + k) % kScaleSets) * kColsScale;
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            const uint64_t db = umma_desc(base + kStageW + k * kUnitB + s * 2 * kPlaneB, kPlaneB, 128);
+                            const uint32_t on = u + k + s > 0;
+                            umma_mxf4(acc, umma_desc(wa + s * 4096, 2048, 128), db, s ? id1 : id0, sf, sf + 8, on);
+                            if (second) umma_mxf4(acc + kTok, umma_desc(wa + kTileW + s * 4096, 2048, 128), db, s ? id1 : id0, sf + 4, sf + 8, on);
+                        }
+                    }
+                    sc_ = (sc_ + kStageUnits) % kScaleSets;
+                    umma_commit(bars + (kBarFree + st_) * 8);
+                    if (++st_ == n_stages) st_ = 0, phase_ ^= 1u;
                 }
-                __syncwarp();
-                if (++st == n_stages) st = 0, phase ^= 1u;
-                if (++sc == kScaleSets) sc = 0;
+                umma_commit(bars + (kBarDFull + set) * 8);
             }
+            __syncwarp();
+            for (int u = 0; u < units; u += kStageUnits)
+                if (++st == n_stages) st = 0, phase ^= 1u;
+            sc = (sc + (units + kStageUnits - 1) / kStageUnits * kStageUnits) % kScaleSets;
             set ^= 1u;
             if (set == 0) dphase ^= 1u;
         }
     } else {
-        // ---------------- epilogue: a warp has a quarter of the lanes and every other 16 y rows
-        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
+        // ---------------- epilogue: a warp has a quarter of the lanes (32 matrix rows of either row tile) and every fourth eight of the y rows.
+        // Chains of dependent steps (load, SwiGLU, maximum over the warp, codes, exchange, store): it takes four warps a scheduler to hide them.
+        const int quarter = warp & 3, part = warp >> 2, r = quarter * 32 + lane;
+        constexpr int kParts = kWarpsEpi / 4;
         uint32_t set = 0, phase = 0;
         const bool pairs = MODE != kYf32 && p.rows % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
         while (t.next()) {
@@ -476,41 +548,38 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
             tc_fence_after_sync();
             const bool lost = lds32(abort) != 0;   // a wait ran out: NaN, not a wrong number
             const uint32_t acc = tmem + (uint32_t(quarter * 32) << 16) + set * kColsAcc;
-            const int chunks = t.width >> 4;
-            for (int c = half; c < chunks; c += 2) {
-                uint32_t v[2][16];
-                tmem_ld16x2(acc + c * 16, acc + kTok + c * 16, v[0], v[1]);
+            const int eights = t.width >> 3;
+            for (int c = part; c < eights; c += kParts) {
+                uint32_t v[2][8];
+                tmem_ld8x2(acc + c * 8, acc + kTok + c * 8, v[0], v[1]);
                 if (lost)
-                    for (int i = 0; i < 16; ++i) v[0][i] = v[1][i] = 0x7fffffffu;
-                if (c + 2 >= chunks) {   // the sums are all in registers: the accumulators go back
+                    for (int i = 0; i < 8; ++i) v[0][i] = v[1][i] = 0x7fffffffu;
+                if (c + kParts >= eights) {   // the sums are all in registers: the accumulators go back
                     tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bars + (kBarDFree + set) * 8);
                 }
-                const int live = t.live - c * 16;
-                const int64_t y0 = t.row0 + c * 16;
+                const int live = t.live - c * 8;
+                const int64_t y0 = t.row0 + c * 8;
                 if (MODE == kYswiglu) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        uint32_t codes, scale;
-                        swiglu8(&v[0][8 * i], &v[1][8 * i], codes, scale);
-                        const size_t y = size_t(y0) + 8 * i + (lane & 7);
-                        const uint32_t at = uint32_t(t.rp) * kMxTileRows + quarter * 32;   // the block's first hidden row
-                        if (8 * i + (lane & 7) < live) {
-                            *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + y * (p.rows / 2) + at / 2 + (lane >> 3) * 4) = codes;
-                            if (lane < 8) p.y_scales[y * (p.rows / kMxBlock) + at / kMxBlock] = uint8_t(scale);
-                        }
+                    uint32_t codes, scale;
+                    swiglu8(v[0], v[1], codes, scale);
+                    const size_t y = size_t(y0) + (lane & 7);
+                    const uint32_t at = uint32_t(t.rp) * kMxTileRows + quarter * 32;   // the block's first hidden row
+                    if (int(lane & 7) < live) {
+                        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.y) + y * (p.rows / 2) + at / 2 + (lane >> 3) * 4) = codes;
+                        if (lane < 8) p.y_scales[y * (p.rows / kMxBlock) + at / kMxBlock] = uint8_t(scale);
                     }
                 } else {
                     constexpr int size = MODE == kYf32 ? 4 : 2;
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
                         const int row = (2 * t.rp + m) * kMxTileRows + r;
-                        store16<MODE>(v[m], static_cast<uint8_t*>(p.y) + (y0 * p.ldy + row) * size, p.ldy, live, row < p.rows, pairs);
+                        store8<MODE>(v[m], static_cast<uint8_t*>(p.y) + (y0 * p.ldy + row) * size, p.ldy, live, row < p.rows, pairs);
                     }
                 }
             }
-            if (half >= chunks) {
+            if (part >= eights) {
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bars + (kBarDFree + set) * 8);
@@ -549,7 +618,7 @@ int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
         if (dev >= 0 && dev < 64) done[dev] = true;
     }
     p.stages = int(std::min<size_t>(kMaxStages, (kSmem - kSmemHead - tables) / kStageBytes));
-    static_assert((kSmem - kSmemHead - (4096 * 3 + 1) * 4) / kStageBytes > kLag, "a stage must be handed on before it is needed again");
+    static_assert((kSmem - kSmemHead - (4096 * 3 + 1) * 4) / kStageBytes >= 2, "stages beside the tables of 4096 experts");
     p.wait_ns = wait_limit_ns();
     const int64_t most = (int64_t(p.S) / kTok + std::min(p.E, p.S)) * pairs;   // tiles at most (every expert's last block may be a part of one)
     const unsigned grid = unsigned(std::min<int64_t>(sm_count(), std::max<int64_t>(1, most)));

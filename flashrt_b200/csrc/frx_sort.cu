@@ -150,10 +150,22 @@ inline size_t sort_place_smem(int E) { return size_t(kChunkSlots) * 4 + size_t(E
 // ---- rows out and back. A block per token; the token's K rows are looked up once, in shared memory.
 constexpr int kMaxK = 32;
 
-__device__ __forceinline__ void load_rows(int (&row)[kMaxK], const int32_t* __restrict__ row_of, size_t t, int K, int64_t rows) {
-    if (threadIdx.x < K) {
-        const int r = row_of[t * K + threadIdx.x];
-        row[threadIdx.x] = r < rows ? r : -1;   // a row that the buffer does not have is left alone
+// The rows that the token has in a buffer of `rows`, in k order, by the first warp: row[i] of the slot slot[i], and how many; a row that the
+// buffer does not have is none. (Lists without gaps: what loops over them loads without asking, so that the loads are in flight together.)
+struct TokenRows {
+    int row[kMaxK], slot[kMaxK], count;
+};
+__device__ __forceinline__ void load_rows(TokenRows& list, const int32_t* __restrict__ row_of, size_t t, int K, int64_t rows) {
+    if (threadIdx.x < 32) {
+        const int r = int(threadIdx.x) < K ? row_of[t * K + threadIdx.x] : -1;
+        const bool have = r >= 0 && r < rows;
+        const unsigned all = __ballot_sync(0xffffffffu, have);
+        const int at = __popc(all & ((1u << threadIdx.x) - 1u));
+        if (have) {
+            list.row[at] = r;
+            list.slot[at] = threadIdx.x;
+        }
+        if (threadIdx.x == 0) list.count = __popc(all);
     }
     __syncthreads();
 }
@@ -162,43 +174,49 @@ __device__ __forceinline__ void load_rows(int (&row)[kMaxK], const int32_t* __re
 template <class V>
 __global__ void __launch_bounds__(256) k_rows_out(const V* __restrict__ x, int64_t ldx, const int32_t* __restrict__ row_of, int K, int nv, V* __restrict__ xs,
                                                   int64_t lds, int64_t rows) {
-    __shared__ int row[kMaxK];
+    __shared__ TokenRows list;
     pdl_wait();
     pdl_trigger();
     const size_t t = blockIdx.x;
-    load_rows(row, row_of, t, K, rows);
-    for (int i = threadIdx.x; i < nv; i += blockDim.x) {
-        const V v = x[t * ldx + i];
-        for (int k = 0; k < K; ++k)
-            if (row[k] >= 0) xs[size_t(row[k]) * lds + i] = v;
+    const int first = threadIdx.x;
+    V v{};
+    if (first < nv) v = x[t * ldx + first];
+    load_rows(list, row_of, t, K, rows);
+    for (int i = first; i < nv; i += blockDim.x) {
+        if (i != first) v = x[t * ldx + i];
+        for (int k = 0; k < list.count; ++k) xs[size_t(list.row[k]) * lds + i] = v;
     }
 }
 
-// out[t] = sum_k w * ys[row]: eight rows in flight
+// out[t] = sum_k w * ys[row], kFlight rows in flight
 template <class T, class O, int N>
 __global__ void __launch_bounds__(256) k_rows_back(const T* __restrict__ ys, int64_t ldy, const float* __restrict__ wts, const int32_t* __restrict__ row_of, int K, int n,
                                                    O* __restrict__ out, int64_t ldo, int64_t rows) {
-    __shared__ int row[kMaxK];
-    __shared__ float w[kMaxK];
+    constexpr int kFlight = 8;
+    __shared__ TokenRows list;
     pdl_wait();
     pdl_trigger();
     const size_t t = blockIdx.x;
-    if (threadIdx.x < K) w[threadIdx.x] = wts ? wts[t * K + threadIdx.x] : 1.0f;
-    load_rows(row, row_of, t, K, rows);
+    load_rows(list, row_of, t, K, rows);
+    const int count = list.count;
     for (int i = threadIdx.x * N; i < n; i += blockDim.x * N) {
         float acc[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] = 0.0f;
-        for (int k0 = 0; k0 < K; k0 += 8) {
-            Vec<T, N> v[8];
+        for (int k0 = 0; k0 < count; k0 += kFlight) {
+            Vec<T, N> v[kFlight];
+            float w[kFlight];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k0 + k < K && row[k0 + k] >= 0) v[k] = *reinterpret_cast<const Vec<T, N>*>(ys + size_t(row[k0 + k]) * ldy + i);
+            for (int k = 0; k < kFlight; ++k) {   // (behind the last row the last again, with weight 0 and not added)
+                const int at = min(k0 + k, count - 1);
+                v[k] = *reinterpret_cast<const Vec<T, N>*>(ys + size_t(list.row[at]) * ldy + i);
+                w[k] = wts ? __ldg(wts + t * K + list.slot[at]) : 1.0f;
+            }
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k0 + k < K && row[k0 + k] >= 0)
+            for (int k = 0; k < kFlight; ++k)
+                if (k0 + k < count)
 #pragma unroll
-                    for (int j = 0; j < N; ++j) acc[j] = fmaf(w[k0 + k], to_float(v[k].v[j]), acc[j]);
+                    for (int j = 0; j < N; ++j) acc[j] = fmaf(w[k], to_float(v[k].v[j]), acc[j]);
         }
         Vec<O, N> o;
 #pragma unroll
@@ -212,50 +230,58 @@ template <class T, int N>
 __global__ void __launch_bounds__(256) k_rows_back_grad(const T* __restrict__ gout, int64_t ldg, const T* __restrict__ ys, int64_t ldy, const float* __restrict__ wts,
                                                         const int32_t* __restrict__ row_of, int K, int n, T* __restrict__ gys, int64_t ldgy, float* __restrict__ gw,
                                                         int64_t rows) {
-    constexpr int kB = 4;   // slots in flight
-    __shared__ int row[kMaxK];
-    __shared__ float w[kMaxK], part[8][kMaxK];
+    constexpr int kFlight = 4;   // rows in flight
+    __shared__ TokenRows list;
+    __shared__ float part[8][kMaxK];
     pdl_wait();
     pdl_trigger();
     const size_t t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
-    if (threadIdx.x < K) w[threadIdx.x] = wts[t * K + threadIdx.x];
-    load_rows(row, row_of, t, K, rows);
-    for (int k0 = 0; k0 < K; k0 += kB) {
-        float dot[kB];
+    load_rows(list, row_of, t, K, rows);
+    const int count = list.count;
+    for (int k0 = 0; k0 < count; k0 += kFlight) {
+        float dot[kFlight], w[kFlight];
+        size_t at[kFlight];
 #pragma unroll
-        for (int k = 0; k < kB; ++k) dot[k] = 0.0f;
+        for (int k = 0; k < kFlight; ++k) {
+            const int l = min(k0 + k, count - 1);
+            dot[k] = 0.0f;
+            at[k] = size_t(list.row[l]);
+            w[k] = __ldg(wts + t * K + list.slot[l]);
+        }
         for (int i = threadIdx.x * N; i < n; i += blockDim.x * N) {
-            Vec<T, N> v[kB];
+            Vec<T, N> v[kFlight];
             const Vec<T, N> g = *reinterpret_cast<const Vec<T, N>*>(gout + t * ldg + i);
 #pragma unroll
-            for (int k = 0; k < kB; ++k)
-                if (k0 + k < K && row[k0 + k] >= 0) v[k] = *reinterpret_cast<const Vec<T, N>*>(ys + size_t(row[k0 + k]) * ldy + i);
+            for (int k = 0; k < kFlight; ++k) v[k] = *reinterpret_cast<const Vec<T, N>*>(ys + at[k] * ldy + i);
 #pragma unroll
-            for (int k = 0; k < kB; ++k)
-                if (k0 + k < K && row[k0 + k] >= 0) {
+            for (int k = 0; k < kFlight; ++k)
+                if (k0 + k < count) {
                     Vec<T, N> o;
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
                         const float gj = to_float(g.v[j]);
                         dot[k] = fmaf(gj, to_float(v[k].v[j]), dot[k]);
-                        o.v[j] = from_float<T>(w[k0 + k] * gj);
+                        o.v[j] = from_float<T>(w[k] * gj);
                     }
-                    *reinterpret_cast<Vec<T, N>*>(gys + size_t(row[k0 + k]) * ldgy + i) = o;
+                    *reinterpret_cast<Vec<T, N>*>(gys + at[k] * ldgy + i) = o;
                 }
         }
 #pragma unroll
-        for (int k = 0; k < kB; ++k) {
+        for (int k = 0; k < kFlight; ++k) {
 #pragma unroll
             for (int d = 16; d; d >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], d);
-            if (lane == 0 && k0 + k < K) part[warp][k0 + k] = dot[k];
+            if (lane == 0 && k0 + k < count) part[warp][list.slot[k0 + k]] = dot[k];
         }
     }
     __syncthreads();
-    if (threadIdx.x < K) {
+    if (int(threadIdx.x) < K) {
         float sum = 0.0f;
-        for (int p = 0; p < warps; ++p) sum += part[p][threadIdx.x];
-        gw[t * K + threadIdx.x] = sum;   // of a slot without a row: no term was added, so 0
+        bool have = false;
+        for (int i = 0; i < count; ++i) have = have || list.slot[i] == int(threadIdx.x);
+        if (have)
+            for (int p = 0; p < warps; ++p) sum += part[p][threadIdx.x];
+        gw[t * K + threadIdx.x] = sum;   // 0 for a slot without a row
     }
 }
 
