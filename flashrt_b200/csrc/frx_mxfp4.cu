@@ -1,6 +1,9 @@
 // MXFP4: the quantizer, the way back, the layout that the product reads, the product (dense, and grouped by expert), and
 // the expert layer made of them.
+#include <cuda.h>
+
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -111,26 +114,29 @@ __global__ void __launch_bounds__(kMxTileRows) k_mx_pack(uint4* __restrict__ cod
 //
 // A tile is 256 matrix rows (two row tiles of 128: the M of the instruction, or the gate and the up tile of 128 hidden rows) by
 // up to 112 y rows of one expert (its N), so weights are read once per 112 rows and an expert with few rows costs what its weights
-// cost. kind::mxf4 multiplies 64 columns per instruction with the block scales in tensor memory. A stage of the ring is 128 columns:
-// per row tile one 8,704-byte unit of the packed layout, brought by one bulk copy, and the y rows' codes (64 bytes each) and scale
-// words, gathered by cp.async through slot_of. Tensor memory: two sets of accumulators (2 x 2 x 112 columns), so that a tile's
-// epilogue runs beside the next tile's products, and four sets of scales (16 columns each).
+// cost. kind::mxf4 multiplies 64 columns per instruction with the block scales in tensor memory. A stage of the ring is 256 columns:
+// per row tile two 8,704-byte units of the packed layout, brought by one bulk copy, and 128 bytes of codes of each y row, gathered by
+// TMA four rows at a time into the 128-byte swizzle. The y rows' scale words, 4 bytes a row and unit, come in segments of 16 units
+// through registers. Tensor memory: two sets of accumulators (2 x 2 x 112 columns), so that a tile's epilogue runs beside the next
+// tile's products, and four sets of scales (16 columns each).
 constexpr int kTok = 112;                 // y rows of a tile at most
 constexpr int kRowTiles = 2;              // row tiles of a tile
 constexpr int kStageUnits = 2;            // units of a stage
-constexpr int kPlaneB = kTok * 16 + 64, kUnitB = 4 * kPlaneB + 512;   // the y rows' codes of 32 columns (64 bytes keep planes off each other's banks); codes and scales of a unit
-constexpr int kTileW = kStageUnits * kMxUnitBytes, kStageW = kRowTiles * kTileW, kStageBytes = kStageW + kStageUnits * kUnitB;
+constexpr int kTileW = kStageUnits * kMxUnitBytes, kStageW = kRowTiles * kTileW, kRowB = kStageUnits * kMxUnitK / 2, kStageBytes = kStageW + kTok * kRowB;
+constexpr int kSegUnits = 16, kSegBytes = kSegUnits * 512, kSegs = 2;   // scale words of y rows: units of a segment, and segments
 constexpr int kMaxStages = 4;
 constexpr int kWarpsEpi = 16, kWarpW = 16, kWarpMma = 17, kWarpAct = 18, kWarpsAct = 8;
 constexpr int kMxThreads = 32 * (kWarpAct + kWarpsAct);
 constexpr int kColsAcc = kRowTiles * kTok, kColScale = 2 * kColsAcc, kScaleSets = 4, kColsScale = 16;
 static_assert(kColScale + kScaleSets * kColsScale <= 512, "tensor memory has 512 columns");
-static_assert((kTok / 4 + kWarpsAct - 1) / kWarpsAct <= 8, "a lane for each row of a warp's scales");
-static_assert(kStageUnits == 2, "the scale words are taken from their four by stage");
 static_assert(kTok % 16 == 0 && kTok <= 128, "the tokens' scales of a unit are one block of 512 bytes");
+static_assert(kRowB == 128 && kStageW % 1024 == 0 && kStageBytes % 1024 == 0, "rows of the 128-byte swizzle, in groups of eight");
+static_assert(kSegUnits % kStageUnits == 0, "a stage has its scales in one segment");
+static_assert(kTok <= 16 * kWarpsAct, "sixteen rows a warp");
 // barriers, 8 bytes each, then the abort flag, the address of the tensor memory and the scan's sums
-constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBars = kBarDFree + 2;
-constexpr int kSmemHead = 256 + 128;   // (one word a warp)
+constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBarSFull = kBarDFree + 2, kBarSFree = kBarSFull + kSegs,
+              kBars = kBarSFree + kSegs;
+constexpr int kSmemSegs = 1024, kSmemHead = kSmemSegs + kSegs * kSegBytes;   // the scale segments, then the stages
 
 enum { kYf32 = FRX_F32, kYbf16 = FRX_BF16, kYf16 = FRX_F16, kYswiglu = 3 };
 
@@ -149,9 +155,15 @@ struct MxProduct {
     int stages;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
-// an arrival at the barrier when all copies that this thread has issued so far have landed
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+// Four rows of the map's box width from column x (bytes here) on, one below the other in shared memory; completion counted on an mbarrier.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, const int (&row)[4], uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+                 : "memory");
+}
+// umma_desc for rows of 128 bytes in the 128-byte swizzle (the 16-byte pieces of row r in the order piece ^ (r % 8)), groups of eight rows 1024 bytes
+// apart; a column offset is added to the address
+__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) { return umma_desc(smem_addr, 16, 1024) | (uint64_t(2) << 61); }
 
 // Instruction descriptor of kind::mxf4 with scales of 32: A and B E2M1 (1), scales UE8M0, both K-major, D fp32 128 x n; the byte pair of
 // the scale words that belongs to these 64 columns is part of it.
@@ -183,16 +195,17 @@ __device__ __forceinline__ void tmem_ld8x2(uint32_t a0, uint32_t a1, uint32_t (&
 }
 
 // The tiles of a block, one after the other: expert after expert, within one row pair after row pair, within these the blocks of y rows
-// (so that blocks that share weights run at the same time). tile_end[e]: tiles of the experts up to e; first[e]: the expert's first row.
+// (so that blocks that share weights run at the same time).
+struct MxTables {
+    int *tile_end, *first, *count, *blocks;   // per expert: tiles up to it, its first row, its rows, blocks of y rows | width << 24
+};
 struct MxWalk {
-    const int *tile_end, *first;
-    int E, pairs, tile, e;
+    MxTables tab;
+    int E, tile, e;
     int rp, row0, live, width;   // row pair, first y row, y rows, their number rounded up to 16
-    __device__ __forceinline__ void begin(const int* ends, const int* rows, int experts, int row_pairs) {
-        tile_end = ends;
-        first = rows;
+    __device__ __forceinline__ void begin(const MxTables& tables, int experts) {
+        tab = tables;
         E = experts;
-        pairs = row_pairs;
         tile = int(blockIdx.x) - int(gridDim.x);
         e = 0;
     }
@@ -200,31 +213,36 @@ struct MxWalk {
         tile += int(gridDim.x);
         const int lane = threadIdx.x & 31;
         while (e < E) {   // 32 experts at a time: those that end at or before the tile
-            const unsigned done = __ballot_sync(0xffffffffu, e + lane < E && tile_end[e + lane] <= tile);
+            const unsigned done = __ballot_sync(0xffffffffu, e + lane < E && tab.tile_end[e + lane] <= tile);
             e += __popc(done);
             if (done != 0xffffffffu) break;
         }
         if (e >= E) return false;
-        const int t0 = e ? tile_end[e - 1] : 0, a = first[e], count = first[E + 1 + e], blocks = (count + kTok - 1) / kTok, local = tile - t0;
-        const int b = local % blocks;
-        rp = local / blocks;
-        width = ((count + blocks - 1) / blocks + 15) & ~15;   // as even as multiples of 16 allow
-        row0 = a + b * width;
-        live = min(width, count - b * width);
+        const int local = tile - (e ? tab.tile_end[e - 1] : 0), bw = tab.blocks[e], w = int(unsigned(bw) >> 24), blocks = bw & 0xffffff;
+        rp = blocks == 1 ? local : int(unsigned(local) / unsigned(blocks));
+        const int b = local - rp * blocks;
+        row0 = tab.first[e] + b * w;
+        live = min(w, tab.count[e] - b * w);
         width = (live + 15) & ~15;
+        // (the shuffles tell the compiler that the values are the same in all lanes)
+        width = __shfl_sync(0xffffffffu, width, 0);
         return true;
     }
 };
 
-// The scale words of units u .. u + 3 of a row (as far as there are so many)
-__device__ __forceinline__ void load_words(uint32_t (&w)[4], const uint8_t* row, int u, int units, bool wide, bool on) {
-    if (!on || u >= units) return;
+// The scale words of units u .. u + 7 of a row (as far as there are so many). Of scattered rows every access costs one a row, whatever its width.
+__device__ __forceinline__ void load_words(uint32_t (&w)[8], const uint8_t* row, int u, int units, bool wide, bool on) {
+    if (!on) return;
     if (wide) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + u * 4));
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (u + 4 * i < units) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + (u + 4 * i) * 4));
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 8; ++j)
             if (u + j < units) w[j] = __ldg(reinterpret_cast<const uint32_t*>(row + (u + j) * 4));
     }
 }
@@ -307,7 +325,7 @@ __device__ __forceinline__ void swiglu8(const uint32_t (&g)[8], const uint32_t (
 }
 
 template <int MODE>
-__global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p) {
+__global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p, const __grid_constant__ CUtensorMap codes_map) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t s0 = smem_u32(smem), stages0 = s0 + kSmemHead, bars = s0, abort = s0 + 240;
@@ -315,8 +333,11 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 244);
     int* warp_sums = reinterpret_cast<int*>(smem + 256);   // one a warp
     const uint32_t n_stages = uint32_t(p.stages);
-    int* tile_end = reinterpret_cast<int*>(smem + kSmemHead + n_stages * kStageBytes);   // [E], then first rows [E + 1], then row counts [E]
-    int* first = tile_end + p.E;
+    MxTables tab;
+    tab.tile_end = reinterpret_cast<int*>(smem + kSmemHead + n_stages * kStageBytes);
+    tab.first = tab.tile_end + p.E;
+    tab.count = tab.first + p.E;
+    tab.blocks = tab.count + p.E;
     const int units = p.n / kMxUnitK;
     const int row_tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, row_pairs = MODE == kYswiglu ? row_tiles : (row_tiles + 1) / 2;
     static_assert(kBars * 8 <= 240, "the barriers' block");
@@ -324,13 +345,18 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
     if (threadIdx.x == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(smem);
         for (int i = 0; i < kMaxStages; ++i) {
-            mbar_init(b + kBarFull + i, 1 + kWarpsAct + 32 * kWarpsAct);   // the weights, a warp's scale words, a thread's copies
+            mbar_init(b + kBarFull + i, 1);
             mbar_init(b + kBarFree + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(b + kBarDFull + i, 1);
             mbar_init(b + kBarDFree + i, kWarpsEpi);
         }
+        for (int i = 0; i < kSegs; ++i) {
+            mbar_init(b + kBarSFull + i, kWarpsAct);
+            mbar_init(b + kBarSFree + i, 1);
+        }
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&codes_map) : "memory");
         *abort_flag = 0;
         mbar_fence_init();
     }
@@ -347,10 +373,13 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
                 a = min(max(p.offsets[e], 0), p.S);
                 b = min(max(p.offsets[e + 1], a), p.S);
             }
-            first[e] = a;
-            first[p.E + 1 + e] = b - a;
-            sum += (b - a + kTok - 1) / kTok * row_pairs;
-            tile_end[e] = sum;
+            const int count = b - a, blocks = (count + kTok - 1) / kTok;
+            const int width = blocks ? ((count + blocks - 1) / blocks + 15) & ~15 : 0;   // as even as multiples of 16 allow
+            tab.first[e] = a;
+            tab.count[e] = count;
+            tab.blocks[e] = blocks | width << 24;
+            sum += blocks * row_pairs;
+            tab.tile_end[e] = sum;
         }
         int inc = sum;
 #pragma unroll
@@ -362,14 +391,14 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
         __syncthreads();
         int before = inc - sum;
         for (int i = 0; i < warp; ++i) before += warp_sums[i];
-        for (int e = e0; e < e1; ++e) tile_end[e] += before;
+        for (int e = e0; e < e1; ++e) tab.tile_end[e] += before;
     }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     MxWalk t;
-    t.begin(tile_end, first, p.E, row_pairs);
+    t.begin(tab, p.E);
 
     // "free" barriers are waited on with the parity of the phase before the one about to be used, which a fresh barrier reports as complete
     if (warp == kWarpW) {
@@ -392,7 +421,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
                 const uint32_t full = bars + (kBarFull + st) * 8, dst = stages0 + st * kStageBytes, bytes = uint32_t(min(kStageUnits, units - u)) * kMxUnitBytes;
                 mbar_spin(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns);
                 if (lane == 0) {
-                    mbar_expect_tx(full, second ? 2 * bytes : bytes);
+                    mbar_expect_tx(full, (second ? 2 * bytes : bytes) + uint32_t(t.width) * kRowB);   // the gathered rows' bytes too
                     bulk_g2s(dst, w0, bytes, full);
                     if (second) bulk_g2s(dst + kTileW, w1, bytes, full);
                 }
@@ -403,136 +432,123 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
             }
         }
     } else if (warp >= kWarpAct) {
-        // ---------------- activations: y rows in fours, dealt to the warps; a lane copies 16 of the 128 bytes that a row has in a stage.
-        // Copies report to the stage's barrier when they land; they and the scale words are generic-proxy writes: the words' writers make theirs
-        // visible to the tensor core before their arrival, for the copies the MMA thread does so behind its wait. (Warps that wait for their
-        // copies themselves hand a stage on late, which halves the ring.) A tile begins with two dependent loads, slots and then scale words;
-        // they are made during the tile in front, or the ring would run empty at every tile.
+        // ---------------- activations. Codes: lanes 0 to 3 of a warp gather four rows each. Scales: a lane has one of the warp's sixteen rows and half
+        // of a segment's units. A tile begins with dependent loads (slots, then scale words), which are made during the tile in front.
+        // (Gathered by cp.async instead, 512 bytes an instruction, the rows came at 11 bytes a clock: 217 us for 163,840 rows of
+        // 1,024 bytes, four times, with nothing else to do; arrivals and proxy fences of the copies were not what took it.)
         const int aw = warp - kWarpAct;
-        constexpr int kFours = (kTok / 4 + kWarpsAct - 1) / kWarpsAct;
-        const size_t row_codes = size_t(p.n / 2), row_scales = size_t(p.n / kMxBlock);
+        const size_t row_scales = size_t(p.n / kMxBlock);
         const bool s_wide = units % 4 == 0 && reinterpret_cast<uintptr_t>(p.scales) % 16 == 0;
-        const int four = lane >> 3, chunk = lane & 7;   // row of the four, 16 bytes of its 128
-        const uint32_t cdst = (chunk >> 2) * kUnitB + (chunk & 3) * kPlaneB + (aw * 4 + four) * 16;   // of the first four's copies in a stage
-        const int stok = (aw + (lane >> 2) * kWarpsAct) * 4 + (lane & 3);   // scale words: a lane has one of the warp's rows
-        const uint32_t sdst = 4 * kPlaneB + (stok & 31) * 16 + (stok >> 5) * 4;
-        uint32_t st = 0, phase = 1;
-        int slot[kFours], sslot = 0;   // of the rows (beyond the live ones the last again): their slots, or themselves
-        const uint8_t *src[kFours], *ssrc = nullptr;
-        uint32_t words[2][4];
+        const int four = aw + (lane & 3) * kWarpsAct;                    // the lane's four rows
+        const int stok = aw * 16 + (lane & 15), shalf = lane >> 4;       // the lane's row and half segment of scale words
+        const uint32_t sdst = s0 + kSmemSegs + shalf * (kSegBytes / 2) + (stok & 31) * 16 + (stok >> 5) * 4;
+        uint32_t st = 0, phase = 1, sg = 0, sphase = 1;
+        int slot[4], sslot = 0;   // of the rows (beyond the live ones the last again): their slots, or themselves
         auto look_up = [&]() {
 #pragma unroll
-            for (int i = 0; i < kFours; ++i) {
-                const int r = t.row0 + min((aw + i * kWarpsAct) * 4 + four, t.live - 1);
+            for (int i = 0; i < 4; ++i) {
+                const int r = t.row0 + min(four * 4 + i, t.live - 1);
                 slot[i] = p.slot_of ? __ldg(p.slot_of + r) : r;
             }
             const int r = t.row0 + min(stok, t.live - 1);
             sslot = p.slot_of ? __ldg(p.slot_of + r) : r;
         };
         auto x_row = [&](int s) {
-            const int x = p.slot_of ? (s < 0 ? 0 : s / p.K) : s;
-            return size_t(x < p.x_rows ? x : 0);
+            const int x = p.slot_of ? (s < 0 ? 0 : int(unsigned(s) / unsigned(p.K))) : s;
+            return x < p.x_rows ? x : 0;
         };
-        auto rows_of_slots = [&](const uint8_t* (&to)[kFours], const uint8_t*& to_scale) {
+        uint32_t words[8];   // the lane's half of the tile's first segment
+        int row[4];
+        const uint8_t* ssrc = nullptr;
+        auto take_up = [&]() {
 #pragma unroll
-            for (int i = 0; i < kFours; ++i) to[i] = p.codes + x_row(slot[i]) * row_codes + chunk * 16;
-            to_scale = p.scales + x_row(sslot) * row_scales;
+            for (int i = 0; i < 4; ++i) row[i] = x_row(slot[i]);
+            ssrc = p.scales + size_t(x_row(sslot)) * row_scales;
+            load_words(words, ssrc, shalf * (kSegUnits / 2), units, s_wide, stok < t.width);
         };
         bool more = t.next();
         if (more) {
             look_up();
-            rows_of_slots(src, ssrc);
-            // (a scale word of scattered rows costs an access a row, whatever its width: four units' words are loaded at a time
-            // where rows allow it)
-            load_words(words[0], ssrc, 0, units, s_wide, stok < t.width);
+            take_up();
         }
         while (more) {
             const int width = t.width;
+            int now[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) now[i] = row[i];
+            const uint8_t* snow = ssrc;
+            const bool s_on = stok < width;
             more = t.next();
             if (more) look_up();
-            const bool s_on = stok < width && lane < 4 * kFours;
-            const int ahead = min(2 * kStageUnits, (units - 1) / kStageUnits * kStageUnits);   // the stage behind which the next tile's rows are taken up
-            const uint8_t *next_src[kFours], *next_ssrc = nullptr;
-            uint32_t next_words[4];
+            const int last = (units - 1) / kStageUnits * kStageUnits, ahead = min(2 * kStageUnits, last);   // the stage behind which the next tile's rows are taken up
             for (int u = 0; u < units; u += kStageUnits) {
-                if ((u & 3) == 0) {
-                    if (u) {
+                if (u % kSegUnits == 0) {
+                    if (u) load_words(words, snow, u + shalf * (kSegUnits / 2), units, s_wide, s_on);
+                    mbar_spin(bars + (kBarSFree + sg) * 8, sphase, abort, p.wait_ns);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) words[0][j] = words[1][j];
-                    }
-                    load_words(words[1], ssrc, u + 4, units, s_wide, s_on);
+                    for (int j = 0; j < kSegUnits / 2; ++j)
+                        if (s_on && u + shalf * (kSegUnits / 2) + j < units) sts32(sdst + sg * kSegBytes + j * 512, words[j]);
+                    fence_async_smem();   // generic-proxy writes: visible to the tensor core before the arrival
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bars + (kBarSFull + sg) * 8);
+                    if (++sg == kSegs) sg = 0, sphase ^= 1u;
                 }
                 mbar_spin(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns);
-                const uint32_t dst = stages0 + st * kStageBytes + kStageW, full = bars + (kBarFull + st) * 8;
-                const bool c_on = u + (chunk >> 2) < units;
-#pragma unroll
-                for (int i = 0; i < kFours; ++i)
-                    if ((aw + i * kWarpsAct) * 4 < width && c_on) cp_async16(dst + cdst + i * kWarpsAct * 64, src[i] + size_t(u) * 64);
-#pragma unroll
-                for (int k = 0; k < kStageUnits; ++k)
-                    if (s_on && u + k < units) sts32(dst + k * kUnitB + sdst, u & 2 ? words[0][2 + k] : words[0][k]);
-                cp_async_arrive(full);
-                fence_async_smem();
+                if (lane < 4 && four * 4 < width) tma_gather4(stages0 + st * kStageBytes + kStageW + four * 4 * kRowB, &codes_map, u * (kMxUnitK / 2), now, bars + (kBarFull + st) * 8);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(full);
                 if (++st == n_stages) st = 0, phase ^= 1u;
-                if (u == ahead && more) {
-                    rows_of_slots(next_src, next_ssrc);
-                    load_words(next_words, next_ssrc, 0, units, s_wide, stok < t.width);
+                if (u == ahead && more) {   // (a tile of several segments has used its words by the last stage)
+                    if (last < kSegUnits) take_up();
                 }
             }
-#pragma unroll
-            for (int i = 0; i < kFours; ++i) src[i] = next_src[i];
-            ssrc = next_ssrc;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) words[0][j] = next_words[j];
+            if (more && last >= kSegUnits) take_up();
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == kWarpMma) {
-        // ---------------- MMA: one elected lane issues, the warp stays together
-        uint32_t st = 0, phase = 0, set = 0, sc = 0, dphase = 1;
+        // ---------------- MMA: one elected lane issues
+        uint32_t st = 0, phase = 0, set = 0, sc = 0, dphase = 1, sg = 0, sphase = 0;
         while (t.next()) {
             const uint32_t id0 = mx_idesc(t.width, 0), id1 = mx_idesc(t.width, 1);
             const bool second = MODE == kYswiglu || 2 * t.rp + 1 < row_tiles;
             mbar_spin(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns);
             const uint32_t acc = tmem + set * kColsAcc;
-            if (elect_one()) {
-                uint32_t st_ = st, phase_ = phase, sc_ = sc;
-                for (int u = 0; u < units; u += kStageUnits) {
-                    mbar_spin(bars + (kBarFull + st_) * 8, phase_, abort, p.wait_ns);
-                    fence_async_smem();   // the gathered rows, which landed as generic-proxy writes
-                    tc_fence_after_sync();
-                    const uint32_t base = stages0 + st_ * kStageBytes;
+            for (int u = 0; u < units; u += kStageUnits) {
+                if (u % kSegUnits == 0) mbar_spin(bars + (kBarSFull + sg) * 8, sphase, abort, p.wait_ns);
+                mbar_spin(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns);
+                tc_fence_after_sync();
+                const uint32_t base = stages0 + st * kStageBytes;
+                const uint64_t da0 = umma_desc(base, 2048, 128), db0 = umma_desc_sw128(base + kStageW);
+                const uint64_t dsa = umma_desc(base + kMxUnitCode, 128, 128), dsb = umma_desc(s0 + kSmemSegs + sg * kSegBytes + (u % kSegUnits) * 512, 128, 128);
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < kStageUnits; ++k) {
                         if (u + k >= units) break;
-                        const uint32_t wa = base + k * kMxUnitBytes + kMxUnitCode, sf = tmem + kColScale + ((sc_ + k) % kScaleSets) * kColsScale;
-                        tmem_copy_scales(sf, umma_desc(wa, 128, 128));
-                        if (second) tmem_copy_scales(sf + 4, umma_desc(wa + kTileW, 128, 128));
-                        tmem_copy_scales(sf + 8, umma_desc(base + kStageW + k * kUnitB + 4 * kPlaneB, 128, 128));
+                        const uint32_t sf = tmem + kColScale + (sc + k) * kColsScale;
+                        tmem_copy_scales(sf, dsa + uint64_t(k * kMxUnitBytes >> 4));
+                        if (second) tmem_copy_scales(sf + 4, dsa + uint64_t((kTileW + k * kMxUnitBytes) >> 4));
+                        tmem_copy_scales(sf + 8, dsb + uint64_t(k * 512 >> 4));
                     }
 #pragma unroll
                     for (int k = 0; k < kStageUnits; ++k) {
                         if (u + k >= units) break;
-                        const uint32_t wa = base + k * kMxUnitBytes, sf = tmem + kColScale + ((sc_ + k) % kScaleSets) * kColsScale;
+                        const uint32_t sf = tmem + kColScale + (sc + k) * kColsScale;
 #pragma unroll
                         for (int s = 0; s < 2; ++s) {
-                            const uint64_t db = umma_desc(base + kStageW + k * kUnitB + s * 2 * kPlaneB, kPlaneB, 128);
+                            const uint64_t db = db0 + uint64_t((k * 64 + s * 32) >> 4);
                             const uint32_t on = u + k + s > 0;
-                            umma_mxf4(acc, umma_desc(wa + s * 4096, 2048, 128), db, s ? id1 : id0, sf, sf + 8, on);
-                            if (second) umma_mxf4(acc + kTok, umma_desc(wa + kTileW + s * 4096, 2048, 128), db, s ? id1 : id0, sf + 4, sf + 8, on);
+                            umma_mxf4(acc, da0 + uint64_t((k * kMxUnitBytes + s * 4096) >> 4), db, s ? id1 : id0, sf, sf + 8, on);
+                            if (second) umma_mxf4(acc + kTok, da0 + uint64_t((kTileW + k * kMxUnitBytes + s * 4096) >> 4), db, s ? id1 : id0, sf + 4, sf + 8, on);
                         }
                     }
-                    sc_ = (sc_ + kStageUnits) % kScaleSets;
-                    umma_commit(bars + (kBarFree + st_) * 8);
-                    if (++st_ == n_stages) st_ = 0, phase_ ^= 1u;
+                    umma_commit(bars + (kBarFree + st) * 8);
+                    if (u + kStageUnits >= units || (u + kStageUnits) % kSegUnits == 0) umma_commit(bars + (kBarSFree + sg) * 8);
+                    if (u + kStageUnits >= units) umma_commit(bars + (kBarDFull + set) * 8);
                 }
-                umma_commit(bars + (kBarDFull + set) * 8);
-            }
-            __syncwarp();
-            for (int u = 0; u < units; u += kStageUnits)
+                __syncwarp();
                 if (++st == n_stages) st = 0, phase ^= 1u;
-            sc = (sc + (units + kStageUnits - 1) / kStageUnits * kStageUnits) % kScaleSets;
+                sc = (sc + kStageUnits) % kScaleSets;
+                if (u + kStageUnits >= units || (u + kStageUnits) % kSegUnits == 0)
+                    if (++sg == kSegs) sg = 0, sphase ^= 1u;
+            }
             set ^= 1u;
             if (set == 0) dphase ^= 1u;
         }
@@ -602,11 +618,30 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p)
     if (warp == kWarpMma) tmem_free(tmem, 512);
 }
 
+// The codes [rows][n / 2] as a tensor map whose box is 128 bytes of one row, in the 128-byte swizzle; bytes beyond a row are zeros.
+int codes_tensor_map(CUtensorMap& map, const void* codes, int rows, int n) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static std::atomic<void*> entry{nullptr};   // the driver's function: looked up once
+    void* fn = entry.load(std::memory_order_acquire);
+    if (!fn) {
+        cudaDriverEntryPointQueryResult found;
+        FRX_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+        if (found != cudaDriverEntryPointSuccess || !fn) return fail(FRX_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+        entry.store(fn, std::memory_order_release);
+    }
+    const cuuint64_t dims[2] = {cuuint64_t(n / 2), cuuint64_t(rows)}, strides[1] = {cuuint64_t(n / 2)};
+    const cuuint32_t box[2] = {cuuint32_t(kRowB), 1}, steps[2] = {1, 1};
+    const CUresult r = reinterpret_cast<Encode>(fn)(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FRX_OK : fail(FRX_ERR_CUDA, "cuTensorMapEncodeTiled: error %d (%d rows of %d bytes)", int(r), rows, n / 2);
+}
+
 template <int MODE>
 int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
-    const size_t tables = (size_t(p.E) * 3 + 1) * 4;
+    const size_t tables = size_t(p.E) * 4 * 4;
     const int64_t row_tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, pairs = MODE == kYswiglu ? row_tiles : (row_tiles + 1) / 2;
-    if ((int64_t(p.S) / kTok + p.E) * pairs > 0x7fff0000) return fail(FRX_ERR_SHAPE, "MXFP4 product: %d rows by %d is more than 2^31 tiles", p.S, p.rows);
+    if (int64_t(p.S) / kTok >= (1 << 24) || (int64_t(p.S) / kTok + p.E) * pairs > 0x7fff0000) return fail(FRX_ERR_SHAPE, "MXFP4 product: %d rows by %d is more than 2^31 tiles", p.S, p.rows);
     constexpr size_t kSmem = 227 * 1024;
     static std::mutex mu;
     static bool done[64] = {};
@@ -618,11 +653,14 @@ int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
         if (dev >= 0 && dev < 64) done[dev] = true;
     }
     p.stages = int(std::min<size_t>(kMaxStages, (kSmem - kSmemHead - tables) / kStageBytes));
-    static_assert((kSmem - kSmemHead - (4096 * 3 + 1) * 4) / kStageBytes >= 2, "stages beside the tables of 4096 experts");
+    static_assert((kSmem - kSmemHead - 4096 * 4 * 4) / kStageBytes >= 2, "stages beside the tables of 4096 experts");
     p.wait_ns = wait_limit_ns();
+    CUtensorMap map;
+    const int rc = codes_tensor_map(map, p.codes, p.x_rows, p.n);
+    if (rc != FRX_OK) return rc;
     const int64_t most = (int64_t(p.S) / kTok + std::min(p.E, p.S)) * pairs;   // tiles at most (every expert's last block may be a part of one)
     const unsigned grid = unsigned(std::min<int64_t>(sm_count(), std::max<int64_t>(1, most)));
-    FRX_LAUNCH(cls, stream, launch_pdl(k_mx_product<MODE>, dim3(grid), dim3(kMxThreads), kSmemHead + size_t(p.stages) * kStageBytes + tables, stream, p));
+    FRX_LAUNCH(cls, stream, launch_pdl(k_mx_product<MODE>, dim3(grid), dim3(kMxThreads), kSmemHead + size_t(p.stages) * kStageBytes + tables, stream, p, map));
     FRX_CUDA(cudaGetLastError());
     return FRX_OK;
 }
