@@ -161,6 +161,20 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map
                  "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
                  : "memory");
 }
+// sixteen consecutive rows
+__device__ __forceinline__ void tma_rows16(uint32_t dst, const CUtensorMap* map, int x, int row, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar) : "memory");
+}
+// A bounded wait of a whole warp: false, in all its lanes, when it, or another one of the block, ran out. The role then leaves its loop: what is
+// issued behind a wait that was given up could run the barriers' byte counts over.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t abort, uint64_t limit_ns) {
+    bool ok = mbar_try_wait(bar, parity);
+    if (!ok) {
+        mbar_spin_slow(bar, parity, abort, limit_ns);
+        ok = lds32(abort) == 0;
+    }
+    return __all_sync(0xffffffffu, ok);
+}
 // umma_desc for rows of 128 bytes in the 128-byte swizzle (the 16-byte pieces of row r in the order piece ^ (r % 8)), groups of eight rows 1024 bytes
 // apart; a column offset is added to the address
 __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) { return umma_desc(smem_addr, 16, 1024) | (uint64_t(2) << 61); }
@@ -212,10 +226,18 @@ struct MxWalk {
     __device__ __forceinline__ bool next() {
         tile += int(gridDim.x);
         const int lane = threadIdx.x & 31;
-        while (e < E) {   // 32 experts at a time: those that end at or before the tile
-            const unsigned done = __ballot_sync(0xffffffffu, e + lane < E && tab.tile_end[e + lane] <= tile);
-            e += __popc(done);
-            if (done != 0xffffffffu) break;
+        // 32 experts at a time, those that end at or before the tile: from the last one on, then, if all of these do, over the whole list
+        // in 32 steps
+        unsigned done = __ballot_sync(0xffffffffu, e + lane < E && tab.tile_end[e + lane] <= tile);
+        e += __popc(done);
+        if (done == 0xffffffffu) {
+            const int step = (E + 31) >> 5, at = min(E, (lane + 1) * step);
+            e = max(e, __popc(__ballot_sync(0xffffffffu, tab.tile_end[at - 1] <= tile)) * step);
+            while (e < E) {
+                done = __ballot_sync(0xffffffffu, e + lane < E && tab.tile_end[e + lane] <= tile);
+                e += __popc(done);
+                if (done != 0xffffffffu) break;
+            }
         }
         if (e >= E) return false;
         const int local = tile - (e ? tab.tile_end[e - 1] : 0), bw = tab.blocks[e], w = int(unsigned(bw) >> 24), blocks = bw & 0xffffff;
@@ -345,7 +367,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
     if (threadIdx.x == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(smem);
         for (int i = 0; i < kMaxStages; ++i) {
-            mbar_init(b + kBarFull + i, 1);
+            mbar_init(b + kBarFull + i, 1 + kWarpsAct);   // the weights' warp with the bytes of both, and every gathering warp
             mbar_init(b + kBarFree + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -405,7 +427,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         // ---------------- weights: one lane, a bulk copy per row tile and stage
         uint32_t st = 0, phase = 1;
         const size_t tile_bytes = size_t(units) * kMxUnitBytes;
-        while (t.next()) {
+        bool ok = true;
+        while (ok && t.next()) {
             const uint8_t *w0, *w1;
             bool second = true;
             if (MODE == kYswiglu) {
@@ -419,7 +442,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
             }
             for (int u = 0; u < units; u += kStageUnits) {
                 const uint32_t full = bars + (kBarFull + st) * 8, dst = stages0 + st * kStageBytes, bytes = uint32_t(min(kStageUnits, units - u)) * kMxUnitBytes;
-                mbar_spin(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns);
+                if (!(ok = warp_wait(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns))) break;
                 if (lane == 0) {
                     mbar_expect_tx(full, (second ? 2 * bytes : bytes) + uint32_t(t.width) * kRowB);   // the gathered rows' bytes too
                     bulk_g2s(dst, w0, bytes, full);
@@ -432,10 +455,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
             }
         }
     } else if (warp >= kWarpAct) {
-        // ---------------- activations. Codes: lanes 0 to 3 of a warp gather four rows each. Scales: a lane has one of the warp's sixteen rows and half
-        // of a segment's units. A tile begins with dependent loads (slots, then scale words), which are made during the tile in front.
-        // (Gathered by cp.async instead, 512 bytes an instruction, the rows came at 11 bytes a clock: 217 us for 163,840 rows of
-        // 1,024 bytes, four times, with nothing else to do; arrivals and proxy fences of the copies were not what took it.)
+        // ---------------- activations. Codes: rows that follow one another come sixteen at a time, others are gathered by lanes 0 to 3 of a warp, four
+        // rows each (36 clocks a four: 14 bytes a clock; by cp.async, 512 bytes an instruction, they came at 11). Scales: a lane has
+        // one of the warp's sixteen rows and half of a segment's units. A tile begins with dependent loads (slots, then scale words), which
+        // are made during the tile in front.
         const int aw = warp - kWarpAct;
         const size_t row_scales = size_t(p.n / kMxBlock);
         const bool s_wide = units % 4 == 0 && reinterpret_cast<uintptr_t>(p.scales) % 16 == 0;
@@ -466,25 +489,28 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
             ssrc = p.scales + size_t(x_row(sslot)) * row_scales;
             load_words(words, ssrc, shalf * (kSegUnits / 2), units, s_wide, stok < t.width);
         };
-        bool more = t.next();
+        bool more = t.next(), ok = true;
         if (more) {
             look_up();
             take_up();
         }
-        while (more) {
-            const int width = t.width;
+        while (more && ok) {
+            const int width = t.width, row0 = t.row0;
             int now[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) now[i] = row[i];
             const uint8_t* snow = ssrc;
             const bool s_on = stok < width;
+            // A warp without rows in the tile takes part in every stage all the same: whoever is more than a ring ahead of the MMAs or behind
+            // them can no longer tell the barriers' phases by their parity.
+            const bool mine = p.slot_of ? lane < 4 && four * 4 < width : lane == 0 && aw * 16 < width;
             more = t.next();
             if (more) look_up();
             const int last = (units - 1) / kStageUnits * kStageUnits, ahead = min(2 * kStageUnits, last);   // the stage behind which the next tile's rows are taken up
             for (int u = 0; u < units; u += kStageUnits) {
                 if (u % kSegUnits == 0) {
                     if (u) load_words(words, snow, u + shalf * (kSegUnits / 2), units, s_wide, s_on);
-                    mbar_spin(bars + (kBarSFree + sg) * 8, sphase, abort, p.wait_ns);
+                    if (!(ok = warp_wait(bars + (kBarSFree + sg) * 8, sphase, abort, p.wait_ns))) break;
 #pragma unroll
                     for (int j = 0; j < kSegUnits / 2; ++j)
                         if (s_on && u + shalf * (kSegUnits / 2) + j < units) sts32(sdst + sg * kSegBytes + j * 512, words[j]);
@@ -493,27 +519,33 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
                     if (lane == 0) mbar_arrive(bars + (kBarSFull + sg) * 8);
                     if (++sg == kSegs) sg = 0, sphase ^= 1u;
                 }
-                mbar_spin(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns);
-                if (lane < 4 && four * 4 < width) tma_gather4(stages0 + st * kStageBytes + kStageW + four * 4 * kRowB, &codes_map, u * (kMxUnitK / 2), now, bars + (kBarFull + st) * 8);
-                __syncwarp();
-                if (++st == n_stages) st = 0, phase ^= 1u;
-                if (u == ahead && more) {   // (a tile of several segments has used its words by the last stage)
-                    if (last < kSegUnits) take_up();
+                if (!(ok = warp_wait(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns))) break;
+                const uint32_t dst = stages0 + st * kStageBytes + kStageW, full = bars + (kBarFull + st) * 8;
+                if (mine) {
+                    if (p.slot_of)
+                        tma_gather4(dst + four * 4 * kRowB, &codes_map, u * (kMxUnitK / 2), now, full);
+                    else
+                        tma_rows16(dst + aw * 16 * kRowB, &codes_map, u * (kMxUnitK / 2), row0 + aw * 16, full);
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full);
+                if (++st == n_stages) st = 0, phase ^= 1u;
+                if (u == ahead && more && last < kSegUnits) take_up();   // (a tile of several segments has used its words by the last stage)
             }
-            if (more && last >= kSegUnits) take_up();
+            if (ok && more && last >= kSegUnits) take_up();
         }
     } else if (warp == kWarpMma) {
         // ---------------- MMA: one elected lane issues
         uint32_t st = 0, phase = 0, set = 0, sc = 0, dphase = 1, sg = 0, sphase = 0;
-        while (t.next()) {
+        bool ok = true;
+        while (ok && t.next()) {
             const uint32_t id0 = mx_idesc(t.width, 0), id1 = mx_idesc(t.width, 1);
             const bool second = MODE == kYswiglu || 2 * t.rp + 1 < row_tiles;
-            mbar_spin(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns);
+            if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
             const uint32_t acc = tmem + set * kColsAcc;
             for (int u = 0; u < units; u += kStageUnits) {
-                if (u % kSegUnits == 0) mbar_spin(bars + (kBarSFull + sg) * 8, sphase, abort, p.wait_ns);
-                mbar_spin(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns);
+                if (u % kSegUnits == 0 && !(ok = warp_wait(bars + (kBarSFull + sg) * 8, sphase, abort, p.wait_ns))) break;
+                if (!(ok = warp_wait(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns))) break;
                 tc_fence_after_sync();
                 const uint32_t base = stages0 + st * kStageBytes;
                 const uint64_t da0 = umma_desc(base, 2048, 128), db0 = umma_desc_sw128(base + kStageW);
@@ -560,17 +592,19 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         uint32_t set = 0, phase = 0;
         const bool pairs = MODE != kYf32 && p.rows % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
         while (t.next()) {
-            mbar_spin(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);
+            const bool lost = !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);   // a wait ran out: NaN, not a wrong number
             tc_fence_after_sync();
-            const bool lost = lds32(abort) != 0;   // a wait ran out: NaN, not a wrong number
             const uint32_t acc = tmem + (uint32_t(quarter * 32) << 16) + set * kColsAcc;
             const int eights = t.width >> 3;
             for (int c = part; c < eights; c += kParts) {
                 uint32_t v[2][8];
-                tmem_ld8x2(acc + c * 8, acc + kTok + c * 8, v[0], v[1]);
-                if (lost)
+                if (lost) {
+#pragma unroll
                     for (int i = 0; i < 8; ++i) v[0][i] = v[1][i] = 0x7fffffffu;
-                if (c + kParts >= eights) {   // the sums are all in registers: the accumulators go back
+                } else {
+                    tmem_ld8x2(acc + c * 8, acc + kTok + c * 8, v[0], v[1]);
+                }
+                if (c + kParts >= eights && !lost) {   // the sums are all in registers: the accumulators go back
                     tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bars + (kBarDFree + set) * 8);
@@ -595,7 +629,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
                     }
                 }
             }
-            if (part >= eights) {
+            if (part >= eights && !lost) {
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bars + (kBarDFree + set) * 8);
@@ -618,8 +652,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
     if (warp == kWarpMma) tmem_free(tmem, 512);
 }
 
-// The codes [rows][n / 2] as a tensor map whose box is 128 bytes of one row, in the 128-byte swizzle; bytes beyond a row are zeros.
-int codes_tensor_map(CUtensorMap& map, const void* codes, int rows, int n) {
+// The codes [rows][n / 2] as a tensor map whose box is 128 bytes of one row (gathered) or of sixteen, in the 128-byte swizzle; what lies beyond the rows is zeros.
+int codes_tensor_map(CUtensorMap& map, const void* codes, int rows, int n, bool gathered) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static std::atomic<void*> entry{nullptr};   // the driver's function: looked up once
@@ -631,7 +665,7 @@ int codes_tensor_map(CUtensorMap& map, const void* codes, int rows, int n) {
         entry.store(fn, std::memory_order_release);
     }
     const cuuint64_t dims[2] = {cuuint64_t(n / 2), cuuint64_t(rows)}, strides[1] = {cuuint64_t(n / 2)};
-    const cuuint32_t box[2] = {cuuint32_t(kRowB), 1}, steps[2] = {1, 1};
+    const cuuint32_t box[2] = {cuuint32_t(kRowB), gathered ? 1u : 16u}, steps[2] = {1, 1};
     const CUresult r = reinterpret_cast<Encode>(fn)(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FRX_OK : fail(FRX_ERR_CUDA, "cuTensorMapEncodeTiled: error %d (%d rows of %d bytes)", int(r), rows, n / 2);
@@ -656,7 +690,7 @@ int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
     static_assert((kSmem - kSmemHead - 4096 * 4 * 4) / kStageBytes >= 2, "stages beside the tables of 4096 experts");
     p.wait_ns = wait_limit_ns();
     CUtensorMap map;
-    const int rc = codes_tensor_map(map, p.codes, p.x_rows, p.n);
+    const int rc = codes_tensor_map(map, p.codes, p.x_rows, p.n, p.slot_of != nullptr);
     if (rc != FRX_OK) return rc;
     const int64_t most = (int64_t(p.S) / kTok + std::min(p.E, p.S)) * pairs;   // tiles at most (every expert's last block may be a part of one)
     const unsigned grid = unsigned(std::min<int64_t>(sm_count(), std::max<int64_t>(1, most)));
@@ -878,8 +912,8 @@ int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_u
     p.codes = base + b.xq;
     p.scales = base + b.xs;
     p.offsets = offsets;
-    p.slot_of = slot_of;
-    p.E = E;
+    p.slot_of = slot_of;   // (sorted copies of the rows instead, which the product reads 16 at a time: 16,384 tokens 219 instead of 248 us, but 24 more in
+    p.E = E;               // the quantizer; 4,096 tokens 113 instead of 103)
     p.rows = ff;
     p.n = n;
     p.K = K;

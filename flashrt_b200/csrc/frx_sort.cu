@@ -24,8 +24,10 @@ __device__ __forceinline__ int slot_expert(const int32_t* __restrict__ ids, int 
     if (s >= S) return -1;
     const int e = ids[s];
     if (e >= E) {
-        status[0] = kDevBadExpertId;
-        status[2] = s;
+        if (status) {
+            status[0] = kDevBadExpertId;
+            status[2] = s;
+        }
         return -1;
     }
     return e < 0 ? -1 : e;
@@ -83,7 +85,7 @@ __global__ void __launch_bounds__(kChunkSlots) k_sort_place(const int32_t* __res
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, c = blockIdx.x, s = c * kChunkSlots + tid, part = tid / kPartSlots, in = tid % kPartSlots;
-    if (chunks == 1 && tid == 0 && status[3] != kCookie) {
+    if (chunks == 1 && tid == 0 && status && status[3] != kCookie) {
         status[0] = kDevOk;
         status[2] = 0;
         status[3] = kCookie;
@@ -95,8 +97,9 @@ __global__ void __launch_bounds__(kChunkSlots) k_sort_place(const int32_t* __res
     __syncthreads();
     const int4* mine = reinterpret_cast<const int4*>(sort_smem + part * kPartSlots);
     int rank = 0, all = 0;
+    const int fours = min(kPartSlots, S - c * kChunkSlots - part * kPartSlots + 3) >> 2;   // of the part's slots (none behind the last)
 #pragma unroll 8
-    for (int j = 0; j < kPartSlots / 4; ++j) {
+    for (int j = 0; j < fours; ++j) {
         const int4 v = mine[j];
         const int d = in - 4 * j;
         all += int(v.x == e) + int(v.y == e) + int(v.z == e) + int(v.w == e);
@@ -395,10 +398,10 @@ int frx_moe_sort(frx_stream_t stream, const int32_t* ids, int T, int K, int E, i
     if (T < 0) return fail(FRX_ERR_ARG, "%s: T %d", who, T);
     const size_t need = frx_moe_sort_workspace_bytes(T, K, E);
     if (!need) return fail(FRX_ERR_SHAPE, "%s: unsupported shape T %d, K %d, E %d", who, T, K, E);
-    if (!offsets || !ws || (T > 0 && (!ids || !slot_of || !row_of))) return fail(FRX_ERR_ARG, "%s: null pointer", who);
+    if (!offsets || (!ws && (long long)T * K > kChunkSlots) || (T > 0 && (!ids || !slot_of || !row_of))) return fail(FRX_ERR_ARG, "%s: null pointer", who);
     if (uintptr_t(ws) % 16) return fail(FRX_ERR_ARG, "%s: misaligned workspace", who);
-    if (ws_bytes < need) return fail(FRX_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, need);
-    return sort_slots(ids, T * K, E, offsets, slot_of, row_of, static_cast<int*>(ws), reinterpret_cast<int*>(static_cast<uint8_t*>(ws) + kAlign), stream);
+    if (ws && ws_bytes < need) return fail(FRX_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, need);
+    return sort_slots(ids, T * K, E, offsets, slot_of, row_of, static_cast<int*>(ws), ws ? reinterpret_cast<int*>(static_cast<uint8_t*>(ws) + kAlign) : nullptr, stream);
 }
 
 int frx_moe_sort_rows(frx_stream_t stream, const void* x, int64_t ldx, int dtype, const int32_t* row_of, int T, int K, int n, void* xs, int64_t ldxs, int64_t rows) {

@@ -277,14 +277,15 @@ def moe_sort_workspace_bytes(T: int, K: int, E: int) -> int:
 
 def moe_sort(ids: torch.Tensor, E: int, ws: torch.Tensor | None = None, stream=None):
     """The plan that sorts the slots of ids int32 [T][K] by expert (frx_moe_sort): offsets int32 [E + 1], slot_of int32 [T * K],
-    row_of int32 [T][K]; -1 where a slot has no row (its id is negative) or a row no slot."""
+    row_of int32 [T][K]; -1 where a slot has no row (its id is negative) or a row no slot. An id of E or more has none either, and is reported by
+    workspace_status(ws) where a workspace is given."""
     _on_device(ids, ws)
     _ids("ids", ids)
     T, K = ids.shape
-    if ws is None:
+    if ws is None and T * K > 1024:
         ws = ids.new_empty(moe_sort_workspace_bytes(T, K, E) + 256, dtype=torch.uint8)
     offsets, slot_of, row_of = ids.new_empty(max(E, 0) + 1), ids.new_empty(T * K), torch.empty_like(ids)
-    wp, wb = _ws_span(ws)
+    wp, wb = (None, 0) if ws is None else _ws_span(ws)
     check(fast.moe_sort(_raw_stream(stream), ids.data_ptr(), T, K, E, offsets.data_ptr(), slot_of.data_ptr(), row_of.data_ptr(), wp, wb))
     return offsets, slot_of, row_of
 

@@ -202,7 +202,8 @@ int frx_route_topk_backward(frx_stream_t stream, const float* gwts, const float*
  * frx_moe_sort: ids [T][K] -> offsets [E + 1] (the rows of expert e are offsets[e] .. offsets[e + 1] - 1), row_of [T][K] (the row of a
  * slot) and slot_of [T * K] (the slot of a row). A slot with a negative id (a dropped or padded one, an expert that lives elsewhere)
  * has no row: row_of is -1 there, and slot_of is -1 for the rows behind offsets[E]. An id of E or more has no row either and is reported by
- * frx_workspace_status. The same ids give the same plan bit for bit. K <= 32, E <= 4096, T * K < 2^31; ws 16-byte aligned. */
+ * frx_workspace_status. The same ids give the same plan bit for bit. K <= 32, E <= 4096, T * K < 2^31; ws 16-byte aligned, or null where T * K <= 1024 (then such an id
+ * is left out without a report). */
 size_t frx_moe_sort_workspace_bytes(int T, int K, int E);
 int frx_moe_sort(frx_stream_t stream, const int32_t* ids, int T, int K, int E, int32_t* offsets, int32_t* slot_of, int32_t* row_of, void* ws,
                  size_t ws_bytes);

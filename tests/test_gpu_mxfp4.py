@@ -225,7 +225,8 @@ def routed(T, K, E, seed, drop=0.0, skew=False):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("T,K,E,n,rows,drop,skew", [(1, 1, 1, 128, 128, 0, False), (1, 4, 64, 256, 130, 0, False), (37, 4, 16, 384, 257, 0.3, False), (300, 2, 5, 256, 128, 0.1, True),
-                                                    (64, 8, 300, 128, 640, 0, False), (500, 3, 7, 640, 100, 0.5, True)])
+                                                    (64, 8, 300, 128, 640, 0, False), (500, 3, 7, 640, 100, 0.5, True), (350, 2, 500, 2048, 256, 0, False), (90, 2, 40, 4224, 128, 0.1, False),
+                                                    (256, 1, 2, 2176, 300, 0, True)])
 def test_moe_matmul(T, K, E, n, rows, drop, skew, dtype):
     ids, _ = routed(T, K, E, T + E, drop, skew)
     xq, wq = random_quantized((T, n), 3), random_quantized((E, rows, n), 4)

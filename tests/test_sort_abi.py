@@ -29,7 +29,7 @@ def test_sort_refusals(L):
     assert f(None, P, 4, 2, 8, P, P, P, P, 255) == L.ERR_WORKSPACE
     assert f(None, P, 4, 2, 8, P, P, P, C.c_void_p(4100), 4096) == L.ERR_ARG
     for i in (1, 5, 6, 7, 8):
-        args = [None, P, 4, 2, 8, P, P, P, P, 4096]
+        args = [None, P, 513, 2, 8, P, P, P, P, 4096]
         args[i] = None
         assert f(*args) == L.ERR_ARG
 
