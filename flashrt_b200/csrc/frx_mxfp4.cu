@@ -563,11 +563,11 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
             const uint32_t id0 = mx_idesc(t.width, 0), id1 = mx_idesc(t.width, 1);
             const bool second = MODE == kYswiglu || 2 * t.rp + 1 < row_tiles;
             if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
+            tc_fence_after_sync();   // behind the epilogue's loads of these accumulators
             const uint32_t acc = tmem + set * kColsAcc;
             for (int u = 0; u < units; u += kStageUnits) {
                 if (u % kSegUnits == 0 && !(ok = warp_wait(bars + (kBarSFull + sg) * 8, sphase, abort, p.wait_ns))) break;
                 if (!(ok = warp_wait(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns))) break;
-                tc_fence_after_sync();
                 const uint32_t base = stages0 + st * kStageBytes;
                 const uint64_t da0 = umma_desc(base, 2048, 128), db0 = umma_desc_sw128(base + kStageW);
                 const uint64_t dsa = umma_desc(base + kMxUnitCode, 128, 128), dsb = umma_desc(s0 + kSmemSegs + sg * kSegBytes + (u % kSegUnits) * 512, 128, 128);
