@@ -174,6 +174,7 @@ struct MxProduct {
     unsigned long long wait_ns;
     int E, rows, n, K, x_rows, S;   // rows: of a matrix; S: rows of y
     int stages;
+    int early;               // the plan was complete before the kernel in front began: it and the weights are read before the wait for that kernel
 };
 
 // Four rows of the map's box width from column x (bytes here) on, one below the other in shared memory; completion counted on an mbarrier.
@@ -280,13 +281,13 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[8], const uint8_t* row,
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             if (u + 4 * i < units) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + (u + 4 * i) * 4));
+                const uint4 v = __ldcg(reinterpret_cast<const uint4*>(row + (u + 4 * i) * 4));
                 w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
             }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (u + j < units) w[j] = __ldg(reinterpret_cast<const uint32_t*>(row + (u + j) * 4));
+            if (u + j < units) w[j] = __ldcg(reinterpret_cast<const uint32_t*>(row + (u + j) * 4));
     }
 }
 
@@ -404,8 +405,13 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         mbar_fence_init();
     }
     if (warp == kWarpMma) tmem_alloc(tmem_slot, 512);
-    pdl_wait();
-    pdl_trigger();
+    // With the plan known early only the warps that read activations or write y wait for the kernel in front, and let the next one in. (That kernel's blocks,
+    // which let this one in, had waited for the ones that made the plan, so these had completed.) One token: 2.1 us from the end of a kernel to
+    // the return of its dependents' wait, 1.4 for the tables and 2 to the first weights, now side by side.
+    if (!p.early) {
+        pdl_wait();
+        pdl_trigger();
+    }
     // tiles of every expert: a thread takes a few experts in a row
     {
         const int per = (p.E + kMxThreads - 1) / kMxThreads, e0 = min(p.E, int(threadIdx.x) * per), e1 = min(p.E, e0 + per);
@@ -413,8 +419,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         for (int e = e0; e < e1; ++e) {
             int a = 0, b = p.S;
             if (p.offsets) {   // (what a plan says beyond the rows that there are is left out)
-                a = min(max(p.offsets[e], 0), p.S);
-                b = min(max(p.offsets[e + 1], a), p.S);
+                a = min(max(__ldcg(p.offsets + e), 0), p.S);
+                b = min(max(__ldcg(p.offsets + e + 1), a), p.S);
             }
             const int count = b - a, blocks = (count + kTok - 1) / kTok;
             const int width = blocks ? ((count + blocks - 1) / blocks + 15) & ~15 : 0;   // as even as multiples of 16 allow
@@ -492,10 +498,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = t.row0 + min(four * 4 + i, t.live - 1);
-                slot[i] = p.slot_of ? __ldg(p.slot_of + r) : r;
+                slot[i] = p.slot_of ? __ldcg(p.slot_of + r) : r;
             }
             const int r = t.row0 + min(stok, t.live - 1);
-            sslot = p.slot_of ? __ldg(p.slot_of + r) : r;
+            sslot = p.slot_of ? __ldcg(p.slot_of + r) : r;
         };
         auto x_row = [&](int s) {
             const int x = p.slot_of ? (s < 0 ? 0 : int(unsigned(s) / unsigned(p.K))) : s;
@@ -511,10 +517,12 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
             load_words(words, ssrc, shalf * (kSegUnits / 2), units, s_wide, stok < t.width);
         };
         bool more = t.next(), ok = true;
-        if (more) {
-            look_up();
-            take_up();
+        if (more) look_up();
+        if (p.early) {
+            pdl_wait();
+            pdl_trigger();
         }
+        if (more) take_up();
         while (more && ok) {
             const int width = t.width, row0 = t.row0;
             int now[4];
@@ -611,6 +619,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         const int quarter = warp & 3, part = warp >> 2, r = quarter * 32 + lane;
         constexpr int kParts = kWarpsEpi / 4;
         uint32_t set = 0, phase = 0;
+        if (p.early) pdl_wait();
         const bool pairs = MODE != kYf32 && p.rows % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
         while (t.next()) {
             const bool lost = !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);   // a wait ran out: NaN, not a wrong number
@@ -937,9 +946,10 @@ int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_u
     uint8_t* base = static_cast<uint8_t*>(ws);
     const int S = T * K;
     int32_t *offsets = reinterpret_cast<int32_t*>(base + b.offsets), *slot_of = reinterpret_cast<int32_t*>(base + b.slot_of), *row_of = reinterpret_cast<int32_t*>(base + b.row_of);
-    int rc = quantize(who, x, ldx, x_dtype, T, n, base + b.xq, base + b.xs, stream);
+    // the sort before the quantizer: the products then find the plan made by a kernel that is not the one in front of them
+    int rc = sort_slots(ids, S, E, offsets, slot_of, row_of, reinterpret_cast<int*>(base), reinterpret_cast<int*>(base + b.sort), stream);
     if (rc != FRX_OK) return rc;
-    rc = sort_slots(ids, S, E, offsets, slot_of, row_of, reinterpret_cast<int*>(base), reinterpret_cast<int*>(base + b.sort), stream);
+    rc = quantize(who, x, ldx, x_dtype, T, n, base + b.xq, base + b.xs, stream);
     if (rc != FRX_OK) return rc;
     MxProduct p{};
     p.codes = base + b.xq;
@@ -957,6 +967,7 @@ int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_u
     p.y = base + b.hq;
     p.y_scales = base + b.hs;
     p.status = reinterpret_cast<int*>(base);
+    p.early = 1;
     if ((rc = launch_product(p, kYswiglu, stream, kKGateUp)) != FRX_OK) return rc;
     // an expert's rows are kept in bfloat16 on their way to a bfloat16 sum: that rounding is half of what such a sum is rounded to anyway,
     // and the rows are the largest thing that the layer writes and reads
@@ -972,7 +983,7 @@ int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_u
     p.ldy = n;
     const int y_type = out_dtype == FRX_BF16 ? FRX_BF16 : FRX_F32;
     if ((rc = launch_product(p, y_type, stream, kKDown)) != FRX_OK) return rc;
-    return rows_back(base + b.y, n, y_type, wts, row_of, S, T, K, n, out, ldo, out_dtype, stream);
+    return rows_back(base + b.y, n, y_type, wts, row_of, S, T, K, n, out, ldo, out_dtype, true, stream);
 }
 
 }  // extern "C"

@@ -160,7 +160,7 @@ struct TokenRows {
 };
 __device__ __forceinline__ void load_rows(TokenRows& list, const int32_t* __restrict__ row_of, size_t t, int K, int64_t rows) {
     if (threadIdx.x < 32) {
-        const int r = int(threadIdx.x) < K ? row_of[t * K + threadIdx.x] : -1;
+        const int r = int(threadIdx.x) < K ? __ldcg(row_of + t * K + threadIdx.x) : -1;
         const bool have = r >= 0 && r < rows;
         const unsigned all = __ballot_sync(0xffffffffu, have);
         const int at = __popc(all & ((1u << threadIdx.x) - 1u));
@@ -191,16 +191,17 @@ __global__ void __launch_bounds__(256) k_rows_out(const V* __restrict__ x, int64
     }
 }
 
-// out[t] = sum_k w * ys[row], kFlight rows in flight
+// out[t] = sum_k w * ys[row], kFlight rows in flight. early: the plan was complete before the kernel in front began, and is read before the wait for it.
 template <class T, class O, int N>
 __global__ void __launch_bounds__(256) k_rows_back(const T* __restrict__ ys, int64_t ldy, const float* __restrict__ wts, const int32_t* __restrict__ row_of, int K, int n,
-                                                   O* __restrict__ out, int64_t ldo, int64_t rows) {
+                                                   O* __restrict__ out, int64_t ldo, int64_t rows, bool early) {
     constexpr int kFlight = 8;
     __shared__ TokenRows list;
-    pdl_wait();
-    pdl_trigger();
+    if (!early) pdl_wait();
     const size_t t = blockIdx.x;
     load_rows(list, row_of, t, K, rows);
+    if (early) pdl_wait();
+    pdl_trigger();
     const int count = list.count;
     for (int i = threadIdx.x * N; i < n; i += blockDim.x * N) {
         float acc[N];
@@ -363,14 +364,14 @@ int sort_slots(const int32_t* ids, int S, int E, int32_t* offsets, int32_t* slot
 }
 
 int rows_back(const void* ys, int64_t ldy, int in_dtype, const float* wts, const int32_t* row_of, int64_t rows, int T, int K, int n, void* out, int64_t ldo,
-              int out_dtype, cudaStream_t stream) {
+              int out_dtype, bool early, cudaStream_t stream) {
     const bool vec = rows_vec16(ys, ldy, n, dtype_size(in_dtype)) && rows_vec16(out, ldo, n, dtype_size(out_dtype)) && (in_dtype == out_dtype || n % 8 == 0);
     auto launch = [&](auto in, auto o, auto width) {
         using T_ = decltype(in);
         using O_ = decltype(o);
         constexpr int N = decltype(width)::value;
         FRX_LAUNCH(kKCombine, stream, launch_pdl(k_rows_back<T_, O_, N>, dim3(T), dim3(row_threads((n + N - 1) / N)), 0, stream, static_cast<const T_*>(ys), ldy, wts, row_of,
-                                                 K, n, static_cast<O_*>(out), ldo, rows));
+                                                 K, n, static_cast<O_*>(out), ldo, rows, early));
     };
     if (in_dtype == out_dtype)
         with_rows(in_dtype, vec, [&](auto v, auto width) { launch(v, v, width); });
@@ -436,7 +437,7 @@ int frx_moe_sort_rows_backward(frx_stream_t stream, const void* gxs, int64_t ldg
     if (!row_of) return fail(FRX_ERR_ARG, "%s: null pointer (row_of)", who);
     if (rows > 0) FRX_TRY(row_buffer(who, "gxs", gxs, ldgxs, n, dtype));
     FRX_TRY(row_buffer(who, "gx", gx, ldgx, n, dtype));
-    return rows_back(gxs, ldgxs, dtype, nullptr, row_of, rows, T, K, n, gx, ldgx, dtype, stream);
+    return rows_back(gxs, ldgxs, dtype, nullptr, row_of, rows, T, K, n, gx, ldgx, dtype, false, stream);
 }
 
 int frx_moe_unsort_rows(frx_stream_t stream, const void* ys, int64_t ldys, int64_t rows, int dtype, const float* wts, const int32_t* row_of, int T, int K, int n, void* out,
@@ -447,7 +448,7 @@ int frx_moe_unsort_rows(frx_stream_t stream, const void* ys, int64_t ldys, int64
     if (!row_of || !wts) return fail(FRX_ERR_ARG, "%s: null pointer (row_of, wts)", who);
     if (rows > 0) FRX_TRY(row_buffer(who, "ys", ys, ldys, n, dtype));
     FRX_TRY(row_buffer(who, "out", out, ldo, n, dtype));
-    return rows_back(ys, ldys, dtype, wts, row_of, rows, T, K, n, out, ldo, dtype, stream);
+    return rows_back(ys, ldys, dtype, wts, row_of, rows, T, K, n, out, ldo, dtype, false, stream);
 }
 
 int frx_moe_unsort_rows_backward(frx_stream_t stream, const void* gout, int64_t ldg, const void* ys, int64_t ldys, int64_t rows, int dtype, const float* wts,
