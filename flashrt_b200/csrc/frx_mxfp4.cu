@@ -157,6 +157,7 @@ static_assert(kTok <= 16 * kWarpsAct, "sixteen rows a warp");
 // barriers, 8 bytes each, then the abort flag, the address of the tensor memory and the scan's sums
 constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBarSFull = kBarDFree + 2, kBarSFree = kBarSFull + kSegs,
               kBars = kBarSFree + kSegs;
+static_assert(256 + 8 * kMxThreads / 32 <= 1024, "the scan's sums");
 constexpr int kSmemSegs = 1024, kSmemHead = kSmemSegs + kSegs * kSegBytes;   // the scale segments, then the stages
 
 enum { kYf32 = FRX_F32, kYbf16 = FRX_BF16, kYf16 = FRX_F16, kYswiglu = 3 };
@@ -174,6 +175,7 @@ struct MxProduct {
     unsigned long long wait_ns;
     int E, rows, n, K, x_rows, S;   // rows: of a matrix; S: rows of y
     int stages;
+    int most;                // tiles of any plan whose experts' rows do not overlap
     int early;               // the plan was complete before the kernel in front began: it and the weights are read before the wait for that kernel
 };
 
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
     const uint32_t s0 = smem_u32(smem), stages0 = s0 + kSmemHead, bars = s0, abort = s0 + 240;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 240);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 244);
-    int* warp_sums = reinterpret_cast<int*>(smem + 256);   // one a warp
+    long long* warp_sums = reinterpret_cast<long long*>(smem + 256);   // one a warp
     const uint32_t n_stages = uint32_t(p.stages);
     MxTables tab;
     tab.tile_end = reinterpret_cast<int*>(smem + kSmemHead + n_stages * kStageBytes);
@@ -413,9 +415,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         pdl_trigger();
     }
     // tiles of every expert: a thread takes a few experts in a row
+    int experts = p.E;
     {
         const int per = (p.E + kMxThreads - 1) / kMxThreads, e0 = min(p.E, int(threadIdx.x) * per), e1 = min(p.E, e0 + per);
-        int sum = 0;
+        long long sum = 0;
         for (int e = e0; e < e1; ++e) {
             int a = 0, b = p.S;
             if (p.offsets) {   // (what a plan says beyond the rows that there are is left out)
@@ -427,27 +430,31 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
             tab.first[e] = a;
             tab.count[e] = count;
             tab.blocks[e] = blocks | width << 24;
-            sum += blocks * row_pairs;
-            tab.tile_end[e] = sum;
+            sum += (long long)blocks * row_pairs;
+            tab.tile_end[e] = int(sum);
         }
-        int inc = sum;
+        long long inc = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, inc, o);
+            const long long up = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += up;
         }
         if (lane == 31) warp_sums[warp] = inc;
         __syncthreads();
-        int before = inc - sum;
-        for (int i = 0; i < warp; ++i) before += warp_sums[i];
-        for (int e = e0; e < e1; ++e) tab.tile_end[e] += before;
+        long long before = inc - sum, total = 0;
+        for (int i = 0; i < kMxThreads / 32; ++i) {
+            before += i < warp ? warp_sums[i] : 0;
+            total += warp_sums[i];
+        }
+        for (int e = e0; e < e1; ++e) tab.tile_end[e] += int(before);
+        if (total > p.most) experts = 0;   // offsets that are not ascending: nothing is computed
     }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     MxWalk t;
-    t.begin(tab, p.E);
+    t.begin(tab, experts);
 
     // "free" barriers are waited on with the parity of the phase before the one about to be used, which a fresh barrier reports as complete
     if (warp == kWarpW) {
@@ -723,6 +730,7 @@ int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
     const int rc = codes_tensor_map(map, p.codes, p.x_rows, p.n, p.slot_of != nullptr);
     if (rc != FRX_OK) return rc;
     const int64_t most = (int64_t(p.S) / kTok + std::min(p.E, p.S)) * pairs;   // tiles at most (every expert's last block may be a part of one)
+    p.most = int(most);
     const unsigned grid = unsigned(std::min<int64_t>(sm_count(), std::max<int64_t>(1, most)));
     FRX_LAUNCH(cls, stream, launch_pdl(k_mx_product<MODE>, dim3(grid), dim3(kMxThreads), kSmemHead + size_t(p.stages) * kStageBytes + tables, stream, p, map));
     FRX_CUDA(cudaGetLastError());

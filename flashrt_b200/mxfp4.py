@@ -10,7 +10,7 @@ import torch
 
 from . import lib as _l
 from .lib import FrxError, check, fast, lib
-from .moe import DTYPES, _ids, _matrix, _on_device, _raw_stream, _typed, _ws_span, workspace
+from .moe import DTYPES, _ids, _matrix, _on_device, _raw_stream, _typed, _ws_span
 
 BLOCK, UNIT = 32, 128       # values that share a scale; columns of a unit of the packed layout
 
@@ -144,7 +144,7 @@ def moe_layer(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_gate: Pac
         out = x.new_empty(T, n, dtype=dtype or x.dtype)
     ldo = _matrix("out", out, None, (T, n))
     if ws is None:
-        ws = workspace(moe_layer_workspace_bytes(T, K, n, ff, E), x.device)
+        ws = x.new_empty(moe_layer_workspace_bytes(T, K, n, ff, E) + 256, dtype=torch.uint8)   # (nobody asks for its status)
     wp, wb = _ws_span(ws)
     check(fast.mxfp4_moe_layer(_raw_stream(stream), w_gate.data.data_ptr(), w_up.data.data_ptr(), w_down.data.data_ptr(), E, n, ff, x.data_ptr(), ldx, DTYPES[x.dtype],
                                ids.data_ptr(), wts.data_ptr(), T, K, out.data_ptr(), ldo, DTYPES[out.dtype], wp, wb))

@@ -580,8 +580,8 @@ int frx_mxfp4_matmul(frx_stream_t stream, const void* codes, const void* scales,
                      int dtype);
 /* The same by expert: for the rows r = offsets[e] .. offsets[e + 1] - 1 of expert e (frx_moe_sort) y[r] = W_e x[slot_of[r] / K], or W_e x[r] where
  * slot_of is null (then K is 1). x has T rows, y has S. The sorted rows of x are never written anywhere: they are read through slot_of. Rows of y that no
- * expert has (behind offsets[E]) are not written. offsets are taken to lie in [0, S], ascending, and slot_of to name rows of x: what lies outside is left
- * out (such a row of y holds anything). E <= 4096. */
+ * expert has (behind offsets[E]) are not written. offsets lie in [0, S] and ascend, slot_of names rows of x: what lies outside is left
+ * out (such a row of y holds anything), and offsets that descend may leave everything out. E <= 4096. */
 int frx_mxfp4_moe_matmul(frx_stream_t stream, const void* codes, const void* scales, int T, int n, const void* packed, int E, int rows,
                          const int32_t* offsets, const int32_t* slot_of, int K, int S, void* y, int64_t ldy, int dtype);
 /* The expert layer with experts in MXFP4, from the routing to the combined rows in one call:

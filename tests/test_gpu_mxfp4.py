@@ -260,6 +260,10 @@ def test_moe_matmul_plan_that_points_outside():
     mxfp4.moe_matmul(*dx, w, torch.tensor([-7, 10, 9, 30, 1 << 30], dtype=torch.int32).cuda(), slot_of.cuda(), K, out=y)
     keep = torch.tensor([r not in (3, 15) and r != 9 for r in range(T * K)])
     assert torch.equal(y.cpu()[keep], good.cpu()[keep])
+    # ranges that overlap, more of them than the rows allow: nothing is computed
+    y.fill_(77.0)
+    mxfp4.moe_matmul(*dx, w, torch.tensor([0, 40, 0, 40, 0], dtype=torch.int32).cuda(), slot_of.cuda(), K, out=y)
+    torch.cuda.synchronize()
 
 
 def layer_reference(x, ids, wts, W, E):
