@@ -247,28 +247,27 @@ def _on_device(*ts):
 
 def _typed(name: str, t: torch.Tensor, dtype, shape=None) -> None:
     """t is contiguous, of this type, and of this shape if one is given."""
-    if t.dtype != dtype or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
+    if t.dtype != dtype or not t.is_contiguous() or (shape is not None and t.shape != shape):
         raise FrxError(_l.ERR_ARG, f"{name}: a contiguous {dtype} tensor{'' if shape is None else f' of shape {tuple(shape)}'} is wanted")
 
 
 def _matrix(name: str, t: torch.Tensor, dtype=None, shape=None) -> int:
     """How many elements the rows of t are apart: rows are contiguous, and may lie apart."""
-    if t.dim() != 2 or t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype) or (shape is not None and tuple(t.shape) != tuple(shape)):
+    size = t.shape
+    if len(size) != 2 or t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype) or (shape is not None and size != shape):
         raise FrxError(_l.ERR_ARG, f"{name}: rows of {'float32, bfloat16 or float16' if dtype is None else dtype}{'' if shape is None else f', {tuple(shape)},'} are wanted")
-    rows, n = t.shape
-    if rows <= 1:
-        ld = n
-    else:
-        ld = t.stride(0)
-    if (n > 1 and t.stride(1) != 1) or ld < n:
-        raise FrxError(_l.ERR_ARG, f"{name}: the elements of a row must be contiguous and rows must not overlap")
-    return ld
+    if size[0] <= 1 or t.is_contiguous():
+        if size[1] <= 1 or t.stride(1) == 1:
+            return size[1]
+    elif (size[1] <= 1 or t.stride(1) == 1) and t.stride(0) >= size[1]:
+        return t.stride(0)
+    raise FrxError(_l.ERR_ARG, f"{name}: the elements of a row must be contiguous and rows must not overlap")
 
 
 def _ids(name: str, t: torch.Tensor, shape=None) -> None:
-    if t.dim() != 2:
-        raise FrxError(_l.ERR_ARG, f"{name}: int32 [tokens][experts per token] is wanted")
-    _typed(name, t, torch.int32, shape)
+    size = t.shape
+    if len(size) != 2 or t.dtype != torch.int32 or not t.is_contiguous() or (shape is not None and size != shape):
+        raise FrxError(_l.ERR_ARG, f"{name}: a contiguous int32 tensor of [tokens][experts per token]{'' if shape is None else f', {shape},'} is wanted")
 
 
 def moe_sort_workspace_bytes(T: int, K: int, E: int) -> int:

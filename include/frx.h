@@ -575,7 +575,8 @@ size_t frx_mxfp4_packed_bytes(int rows, int n);
 int frx_mxfp4_pack(frx_stream_t stream, const void* codes, const void* scales, int E, int rows, int n, void* packed);
 int frx_mxfp4_unpack(frx_stream_t stream, const void* packed, int E, int rows, int n, void* codes, void* scales);
 /* y[t] = W x[t]: x [T] rows of n values in MXFP4, W one packed matrix [rows][n], y [T] rows of `rows` elements of dtype, ldy apart. Products are
- * exact, sums are formed in 32 bits on the tensor cores and rounded once to dtype. Any T and any number of rows. */
+ * exact, sums are formed in 32 bits on the tensor cores and rounded once to dtype. Any T and any number of rows. A device-side wait that runs out
+ * (2 s, frx_debug_set_wait_limit_ns) leaves NaN in y; there is no workspace to report it in. */
 int frx_mxfp4_matmul(frx_stream_t stream, const void* codes, const void* scales, int T, int n, const void* packed, int rows, void* y, int64_t ldy,
                      int dtype);
 /* The same by expert: for the rows r = offsets[e] .. offsets[e + 1] - 1 of expert e (frx_moe_sort) y[r] = W_e x[slot_of[r] / K], or W_e x[r] where
