@@ -29,10 +29,10 @@ def quantize(x: torch.Tensor, stream=None):
 
 def _quantized(codes: torch.Tensor, scales: torch.Tensor):
     """T, n of quantized rows."""
-    if codes.dim() != 2:
-        raise FrxError(_l.ERR_ARG, "codes: uint8 [rows][n / 2] is wanted")
-    T, half = codes.shape
-    _typed("codes", codes, torch.uint8)
+    size = codes.shape
+    if len(size) != 2 or codes.dtype != torch.uint8 or not codes.is_contiguous():
+        raise FrxError(_l.ERR_ARG, "codes: a contiguous uint8 tensor of [rows][n / 2] is wanted")
+    T, half = size
     _typed("scales", scales, torch.uint8, (T, 2 * half // BLOCK))
     return T, 2 * half
 
@@ -77,23 +77,22 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, stream=None) -> Packed:
 
 def unpack(w: Packed, stream=None):
     """codes and scales of a Packed (the inverse of pack)."""
-    _packed("w", w)
+    _on_device(w.data)
     codes, scales = w.data.new_empty(w.E, w.rows, w.n // 2), w.data.new_empty(w.E, w.rows, w.n // BLOCK)
     check(lib.frx_mxfp4_unpack(_raw_stream(stream), w.data.data_ptr(), w.E, w.rows, w.n, codes.data_ptr(), scales.data_ptr()))
     return codes, scales
 
 
-def _packed(name: str, w: Packed, n: int | None = None) -> None:
-    _on_device(w.data)
-    if n is not None and w.n != n:
-        raise FrxError(_l.ERR_ARG, f"{name}: a matrix of {w.n} columns for rows of {n} values")
+def _columns(w: Packed, n: int) -> None:
+    if w.n != n:
+        raise FrxError(_l.ERR_ARG, f"a matrix of {w.n} columns for rows of {n} values")
 
 
 def matmul(codes: torch.Tensor, scales: torch.Tensor, w: Packed, out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """y[t] = W x[t] of quantized rows x and one packed matrix: [T][rows] in `dtype` (or that of `out`)."""
-    _on_device(codes, scales, out)
+    _on_device(codes, scales, out, w.data)
     T, n = _quantized(codes, scales)
-    _packed("w", w, n)
+    _columns(w, n)
     if w.E != 1:
         raise FrxError(_l.ERR_ARG, f"matmul: {w.E} matrices: moe_matmul takes several")
     if out is None:
@@ -107,9 +106,9 @@ def moe_matmul(codes: torch.Tensor, scales: torch.Tensor, w: Packed, offsets: to
                out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """y[r] = W_e x[slot_of[r] / K] for the sorted rows r of each expert e (offsets, slot_of: moe.moe_sort); without slot_of W_e x[r]. Rows of `out`
     that no expert has are left as they were."""
-    _on_device(codes, scales, offsets, slot_of, out)
+    _on_device(codes, scales, offsets, slot_of, out, w.data)
     T, n = _quantized(codes, scales)
-    _packed("w", w, n)
+    _columns(w, n)
     _typed("offsets", offsets, torch.int32, (w.E + 1,))
     if slot_of is not None:
         _typed("slot_of", slot_of, torch.int32)
@@ -130,22 +129,24 @@ def moe_layer(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_gate: Pac
               dtype: torch.dtype | None = None, ws: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The expert layer in MXFP4 (frx_mxfp4_moe_layer): out[t] = sum over k of wts[t][k] * expert_{ids[t][k]}(x[t]), [T][n] in `dtype` (that of
     `out`, or of x). Slots with a negative id take no part."""
-    _on_device(x, ids, wts, out, ws)
+    gate, E, ff, gate_n = w_gate
+    up, down = w_up[0], w_down[0]
+    _on_device(x, ids, wts, out, ws, gate, up, down)
     ldx = _matrix("x", x)
+    (T, n), shape = x.shape, ids.shape
     _ids("ids", ids)
-    (T, n), K, E, ff = x.shape, ids.shape[1], w_gate.E, w_gate.rows
-    _ids("ids", ids, (T, K))
-    _typed("wts", wts, torch.float32, (T, K))
-    for name, w, shape in (("w_gate", w_gate, (E, ff, n)), ("w_up", w_up, (E, ff, n)), ("w_down", w_down, (E, n, ff))):
-        _packed(name, w)
-        if (w.E, w.rows, w.n) != shape:
-            raise FrxError(_l.ERR_ARG, f"{name}: {(w.E, w.rows, w.n)} matrices, {shape} are wanted")
+    if shape[0] != T:
+        raise FrxError(_l.ERR_ARG, f"ids: {shape[0]} tokens, x has {T}")
+    K = shape[1]
+    _typed("wts", wts, torch.float32, shape)
+    if gate_n != n or w_up[1:] != (E, ff, n) or w_down[1:] != (E, n, ff):
+        raise FrxError(_l.ERR_ARG, f"matrices (experts, rows, columns) {w_gate[1:]}, {w_up[1:]}, {w_down[1:]} for rows of {n} values: two of {(E, ff, n)} and {(E, n, ff)} are wanted")
     if out is None:
         out = x.new_empty(T, n, dtype=dtype or x.dtype)
     ldo = _matrix("out", out, None, (T, n))
     if ws is None:
         ws = x.new_empty(moe_layer_workspace_bytes(T, K, n, ff, E) + 256, dtype=torch.uint8)   # (nobody asks for its status)
     wp, wb = _ws_span(ws)
-    check(fast.mxfp4_moe_layer(_raw_stream(stream), w_gate.data.data_ptr(), w_up.data.data_ptr(), w_down.data.data_ptr(), E, n, ff, x.data_ptr(), ldx, DTYPES[x.dtype],
+    check(fast.mxfp4_moe_layer(_raw_stream(stream), gate.data_ptr(), up.data_ptr(), down.data_ptr(), E, n, ff, x.data_ptr(), ldx, DTYPES[x.dtype],
                                ids.data_ptr(), wts.data_ptr(), T, K, out.data_ptr(), ldo, DTYPES[out.dtype], wp, wb))
     return out
