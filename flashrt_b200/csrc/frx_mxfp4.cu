@@ -133,13 +133,20 @@ __global__ void __launch_bounds__(kMxTileRows) k_mx_pack(uint4* __restrict__ cod
 
 // ---- product on the tensor cores
 //
-// A tile is 256 matrix rows (two row tiles of 128: the M of the instruction, or the gate and the up tile of 128 hidden rows) by
+// y[r] = sum over blocks b of 32 columns of 2^(ew[b] + ex[b]) * (sum of the 32 products of elements): kind::mxf4 does 64 columns, both scales included, per
+// instruction. A tile is 256 matrix rows (two row tiles of 128: the M of the instruction, or the gate and the up tile of 128 hidden rows) by
 // up to 112 y rows of one expert (its N), so weights are read once per 112 rows and an expert with few rows costs what its weights
-// cost. kind::mxf4 multiplies 64 columns per instruction with the block scales in tensor memory. A stage of the ring is 256 columns:
-// per row tile two 8,704-byte units of the packed layout, brought by one bulk copy, and 128 bytes of codes of each y row, gathered by
-// TMA four rows at a time into the 128-byte swizzle. The y rows' scale words, 4 bytes a row and unit, come in segments of 16 units
+// cost. A stage of the ring is 256 columns:
+// per row tile two 8,704-byte units of the packed layout, brought by one bulk copy, and 128 bytes of codes of each y row, by
+// TMA into the 128-byte swizzle. The y rows' scale words, 4 bytes a row and unit, come in segments of 16 units
 // through registers. Tensor memory: two sets of accumulators (2 x 2 x 112 columns), so that a tile's epilogue runs beside the next
 // tile's products, and four sets of scales (16 columns each).
+//
+// What bounds it. Up to a few rows an expert: the weights. 64 tokens of ten experts out of 512 (2048 / 512; gate and up): 408 MB from DRAM in 61 us between
+// launches, 6.7 TB/s; 10 us of the layer's 111 are the start of the two products and their uneven ends. 4,096 tokens: 100 us for 570 MB of weights. 16,384 tokens
+// (three blocks of 107 rows an expert): 262 us for 687 GFLOP at full clocks, the thread that issues (a stage's hand-offs, six copies of scales and eight MMAs take
+// 900 clocks, of which the MMAs are 464) and the L2, which delivers 55 bytes a clock and SM without any MMA; in a stream of such layers the GPU is at its power
+// limit (1,000 W) and at 1,650 MHz.
 constexpr int kTok = 112;                 // y rows of a tile at most
 constexpr int kRowTiles = 2;              // row tiles of a tile
 constexpr int kStageUnits = 2;            // units of a stage
@@ -175,6 +182,7 @@ struct MxProduct {
     unsigned long long wait_ns;
     int E, rows, n, K, x_rows, S;   // rows: of a matrix; S: rows of y
     int stages;
+    int single;              // tiles of one row tile instead of two
     int most;                // tiles of any plan whose experts' rows do not overlap
     int early;               // the plan was complete before the kernel in front began: it and the weights are read before the wait for that kernel
 };
@@ -385,7 +393,10 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
     tab.count = tab.first + p.E;
     tab.blocks = tab.count + p.E;
     const int units = p.n / kMxUnitK;
-    const int row_tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, row_pairs = MODE == kYswiglu ? row_tiles : (row_tiles + 1) / 2;
+    const int row_tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, row_pairs = MODE == kYswiglu || p.single ? row_tiles : (row_tiles + 1) / 2;
+    // first row tile of a tile's row pair, and whether it has a second one
+    auto row_tile = [&](int rp) { return MODE == kYswiglu || p.single ? rp : 2 * rp; };
+    auto has_second = [&](int rp) { return MODE == kYswiglu || (!p.single && 2 * rp + 1 < row_tiles); };
     static_assert(kBars * 8 <= 240, "the barriers' block");
 
     if (threadIdx.x == 0) {
@@ -470,9 +481,9 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
                 w0 = p.w[0] + at;
                 w1 = p.w[1] + at;
             } else {
-                w0 = p.w[0] + (size_t(t.e) * row_tiles + 2 * t.rp) * tile_bytes;
+                w0 = p.w[0] + (size_t(t.e) * row_tiles + row_tile(t.rp)) * tile_bytes;
                 w1 = w0 + tile_bytes;
-                second = 2 * t.rp + 1 < row_tiles;
+                second = has_second(t.rp);
             }
             for (int u = 0; u < units; u += kStageUnits) {
                 const uint32_t full = bars + (kBarFull + st) * 8, dst = stages0 + st * kStageBytes, bytes = uint32_t(min(kStageUnits, units - u)) * kMxUnitBytes;
@@ -576,7 +587,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         bool ok = true;
         while (ok && t.next()) {
             const uint32_t id0 = mx_idesc(t.width, 0), id1 = mx_idesc(t.width, 1);
-            const bool second = MODE == kYswiglu || 2 * t.rp + 1 < row_tiles;
+            const bool second = has_second(t.rp);
             if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
             tc_fence_after_sync();   // behind the epilogue's loads of these accumulators
             const uint32_t acc = tmem + set * kColsAcc;
@@ -661,8 +672,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
                     constexpr int size = MODE == kYf32 ? 4 : 2;
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
-                        const int row = (2 * t.rp + m) * kMxTileRows + r;
-                        store8<MODE>(v[m], static_cast<uint8_t*>(p.y) + (y0 * p.ldy + row) * size, p.ldy, live, row < p.rows, pairs);
+                        const int row = (row_tile(t.rp) + m) * kMxTileRows + r;
+                        store8<MODE>(v[m], static_cast<uint8_t*>(p.y) + (y0 * p.ldy + row) * size, p.ldy, live, row < p.rows && (m == 0 || has_second(t.rp)), pairs);
                     }
                 }
             }
@@ -711,7 +722,11 @@ int codes_tensor_map(CUtensorMap& map, const void* codes, int rows, int n, bool 
 template <int MODE>
 int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
     const size_t tables = size_t(p.E) * 4 * 4;
-    const int64_t row_tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, pairs = MODE == kYswiglu ? row_tiles : (row_tiles + 1) / 2;
+    // Two row tiles a tile halve how often y rows' activations are read; where single ones still find an SM each, they halve the time that an SM takes for its weights
+    // (1,024 x 2,048 by one token: 7.1 us a call instead of 7.7).
+    const int64_t row_tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, blocks = int64_t(p.S) / kTok + std::min(p.E, p.S);   // blocks of y rows at most
+    p.single = MODE != kYswiglu && row_tiles * blocks <= sm_count();
+    const int64_t pairs = MODE == kYswiglu || p.single ? row_tiles : (row_tiles + 1) / 2;
     if (int64_t(p.S) / kTok >= (1 << 24) || (int64_t(p.S) / kTok + p.E) * pairs > 0x7fff0000) return fail(FRX_ERR_SHAPE, "MXFP4 product: %d rows by %d is more than 2^31 tiles", p.S, p.rows);
     constexpr size_t kSmem = 227 * 1024;
     static std::mutex mu;
@@ -729,7 +744,7 @@ int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
     CUtensorMap map;
     const int rc = codes_tensor_map(map, p.codes, p.x_rows, p.n, p.slot_of != nullptr);
     if (rc != FRX_OK) return rc;
-    const int64_t most = (int64_t(p.S) / kTok + std::min(p.E, p.S)) * pairs;   // tiles at most (every expert's last block may be a part of one)
+    const int64_t most = blocks * pairs;
     p.most = int(most);
     const unsigned grid = unsigned(std::min<int64_t>(sm_count(), std::max<int64_t>(1, most)));
     FRX_LAUNCH(cls, stream, launch_pdl(k_mx_product<MODE>, dim3(grid), dim3(kMxThreads), kSmemHead + size_t(p.stages) * kStageBytes + tables, stream, p, map));
