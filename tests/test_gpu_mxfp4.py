@@ -212,6 +212,77 @@ def test_matmul_scales_of_every_size_and_nan():
     assert torch.equal(bad.cpu()[~nan], got.cpu()[~nan])
 
 
+@pytest.mark.parametrize("n,rows", [(256, 300), (2048, 128), (640, 64)])
+def test_matmul_of_operands_at_the_least_alignment(n, rows):
+    """Codes on 16 bytes, scales on 4, y on one element: the same bits as on the widest."""
+    T = 50
+    xq, wq = random_quantized((T, n), 11), random_quantized((rows, n), 12)
+    w = mxfp4.pack(wq[0].cuda(), wq[1].cuda())
+    want = mxfp4.matmul(xq[0].cuda(), xq[1].cuda(), w)
+    shifted = []
+    for t, by in ((xq[0], 16), (xq[1], 4), (w.data, 16)):
+        flat = torch.zeros(t.numel() + by, dtype=torch.uint8, device="cuda")
+        flat[by:] = t.reshape(-1).cuda()
+        shifted.append(flat[by:].view(t.shape))
+    moved = mxfp4.Packed(shifted[2], 1, rows, n)
+    assert torch.equal(mxfp4.matmul(shifted[0], shifted[1], moved), want)
+
+
+def test_layers_in_a_stream_without_a_wait():
+    """Calls that follow one another, each on values that the kernels in front have just made, with one workspace: what each gives alone."""
+    E, n, ff, K = 24, 512, 256, 4
+    raw = [random_quantized(s, i) for i, s in enumerate(((E, ff, n), (E, ff, n), (E, n, ff)))]
+    W = [mxfp4.pack(c.cuda(), (s - 6).cuda()) for c, s in raw]
+    sizes = [1, 700, 3, 64, 1500, 2, 300, 1]
+    ws = moe.workspace(max(mxfp4.moe_layer_workspace_bytes(T, K, n, ff, E) for T in sizes))
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    seeds = [(torch.randn(T, n, generator=g, device="cuda"), torch.randn(T, E, generator=g, device="cuda")) for T in sizes]
+    mix = torch.randn(n, n, generator=g, device="cuda") / n ** 0.5
+
+    def inputs(x, logits):
+        y = x
+        for _ in range(3):
+            y = torch.tanh(y @ mix)
+        ids, wts = moe.moe_route_topk(logits, K)
+        return y.contiguous(), torch.where(logits[:, :K] > 1.5, -1, ids), wts
+
+    torch.cuda.synchronize()
+    outs = []
+    for r in range(3):
+        for x, logits in seeds:
+            outs.append(mxfp4.moe_layer(*inputs(x + r, logits + r * mix[0, :E]), *W, ws=ws))
+    torch.cuda.synchronize()
+    for r in range(3):
+        for x, logits in seeds:
+            made = inputs(x + r, logits + r * mix[0, :E])
+            torch.cuda.synchronize()
+            want = mxfp4.moe_layer(*made, *W)
+            torch.cuda.synchronize()
+            assert torch.equal(outs.pop(0), want)
+
+
+def test_rows_more_than_32_bits_apart():
+    """Rows whose distance passes 2^31 bytes and 2^31 elements: x and out of the layer, x of the quantizer, y of the product."""
+    T, n, ff, E, K = 3, 256, 128, 4, 2
+    far = 1_200_000_000                                  # elements between rows; the third begins at 2.4 * 10^9
+    ids, wts = (t.cuda() for t in routed(T, K, E, 3))
+    raw = [random_quantized(s, i) for i, s in enumerate(((E, ff, n), (E, ff, n), (E, n, ff)))]
+    W = [mxfp4.pack(c.cuda(), (s - 6).cuda()) for c, s in raw]
+    x = torch.randn(T, n, generator=gen(1)).bfloat16().cuda()
+    place = torch.empty(2 * far + n, dtype=torch.bfloat16, device="cuda").as_strided((T, n), (far, 1))
+    place.copy_(x)
+    want_q, want = mxfp4.quantize(x), mxfp4.moe_layer(x, ids, wts, *W)
+    for a, b in zip(mxfp4.quantize(place), want_q):
+        assert torch.equal(a, b)
+    assert torch.equal(mxfp4.dequantize(*want_q, out=place), mxfp4.dequantize(*want_q, dtype=torch.bfloat16))
+    place.copy_(x)
+    got = mxfp4.moe_layer(place, ids, wts, *W, out=place)     # in place: x is read before the first row of out is written
+    assert torch.equal(got, want)
+    w = mxfp4.pack(raw[0][0][0].cuda(), raw[0][1][0].cuda())
+    assert torch.equal(mxfp4.matmul(*want_q, w, out=place[:, :ff]), mxfp4.matmul(*want_q, w))
+
+
 def routed(T, K, E, seed, drop=0.0, skew=False):
     g = gen(seed)
     score = torch.randn(T, E, generator=g)
@@ -226,7 +297,7 @@ def routed(T, K, E, seed, drop=0.0, skew=False):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("T,K,E,n,rows,drop,skew", [(1, 1, 1, 128, 128, 0, False), (1, 4, 64, 256, 130, 0, False), (37, 4, 16, 384, 257, 0.3, False), (300, 2, 5, 256, 128, 0.1, True),
                                                     (64, 8, 300, 128, 640, 0, False), (500, 3, 7, 640, 100, 0.5, True), (350, 2, 500, 2048, 256, 0, False), (90, 2, 40, 4224, 128, 0.1, False),
-                                                    (256, 1, 2, 2176, 300, 0, True)])
+                                                    (256, 1, 2, 2176, 300, 0, True), (300, 2, 4096, 512, 128, 0, False), (40, 3, 2049, 128, 256, 0.2, False)])
 def test_moe_matmul(T, K, E, n, rows, drop, skew, dtype):
     ids, _ = routed(T, K, E, T + E, drop, skew)
     xq, wq = random_quantized((T, n), 3), random_quantized((E, rows, n), 4)

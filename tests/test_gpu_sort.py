@@ -139,6 +139,28 @@ def test_rows_there_and_back(T, K, n, dtype, layout):
     assert bool((gw.cpu()[~live] == 0).all())
 
 
+def test_rows_more_than_32_bits_apart():
+    T, K, n, E = 3, 2, 64, 4
+    far = 1_200_000_000                                  # elements between rows; the third begins at 2.4 * 10^9
+    row_of = torch.tensor([[2, 0], [-1, 1], [0, -1]], dtype=torch.int32).cuda()
+    wts = torch.rand(T, K, generator=gen(1)).cuda()
+    flat = torch.empty(2 * far + n, dtype=torch.bfloat16, device="cuda")
+    place = flat.as_strided((T, n), (far, 1))
+    x = torch.randn(T, n, generator=gen(2)).bfloat16().cuda()
+    near = torch.zeros(T, n, dtype=torch.bfloat16, device="cuda")
+    place.zero_()
+    plan_of = torch.tensor([[2, -1], [1, -1], [0, -1]], dtype=torch.int32).cuda()
+    assert torch.equal(moe.moe_sort_rows(x, plan_of, out=place), moe.moe_sort_rows(x, plan_of, out=near))
+    assert torch.equal(moe.moe_unsort_rows(place, wts, row_of), moe.moe_unsort_rows(near, wts, row_of))
+    assert torch.equal(moe.moe_sort_rows_backward(place, row_of), moe.moe_sort_rows_backward(near, row_of))
+    gys = torch.zeros_like(near)
+    a = moe.moe_unsort_rows_backward(x, near, wts, plan_of, gys=gys)
+    far_gys = torch.empty(2 * far + n, dtype=torch.bfloat16, device="cuda").as_strided((T, n), (far, 1))
+    far_gys.zero_()
+    b = moe.moe_unsort_rows_backward(x, place, wts, plan_of, gys=far_gys)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_rows_with_infinities_and_nan_in_rows_that_nobody_has():
     """A row without a slot may hold anything: nothing of it is read into a sum."""
     ids = make_ids(20, 4, 8, 1, 0.4)
