@@ -237,6 +237,13 @@ def quantize_q8(x: torch.Tensor, stream=None):
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # FRX_F32, FRX_BF16, FRX_F16
 
 
+def _code(dtype: torch.dtype) -> int:
+    code = DTYPES.get(dtype)
+    if code is None:
+        raise FrxError(_l.ERR_ARG, f"rows of {dtype}: float32, bfloat16 or float16 are wanted")
+    return code
+
+
 def _on_device(*ts):
     """The tensors are on the current device, whose stream the call goes to."""
     dev = _current_device() if _current_device else None
@@ -297,8 +304,9 @@ def moe_sort_rows(x: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | Non
     (T, n), K = x.shape, row_of.shape[1]
     _ids("row_of", row_of, (T, K))
     if out is None:
-        out = x.new_empty(T * K, n)
-    ldo = _matrix("out", out, x.dtype, (out.shape[0], n))
+        out, ldo = x.new_empty(T * K, n), n
+    else:
+        ldo = _matrix("out", out, x.dtype, (out.shape[0], n))
     check(fast.moe_sort_rows(_raw_stream(stream), x.data_ptr(), ldx, DTYPES[x.dtype], row_of.data_ptr(), T, K, n, out.data_ptr(), ldo, out.shape[0]))
     return out
 
@@ -310,8 +318,9 @@ def moe_sort_rows_backward(gxs: torch.Tensor, row_of: torch.Tensor, out: torch.T
     _ids("row_of", row_of)
     (T, K), (rows, n) = row_of.shape, gxs.shape
     if out is None:
-        out = gxs.new_empty(T, n)
-    ldo = _matrix("out", out, gxs.dtype, (T, n))
+        out, ldo = gxs.new_empty(T, n), n
+    else:
+        ldo = _matrix("out", out, gxs.dtype, (T, n))
     check(fast.moe_sort_rows_backward(_raw_stream(stream), gxs.data_ptr(), ldg, rows, DTYPES[gxs.dtype], row_of.data_ptr(), T, K, n, out.data_ptr(), ldo))
     return out
 
@@ -325,8 +334,9 @@ def moe_unsort_rows(ys: torch.Tensor, wts: torch.Tensor, row_of: torch.Tensor, o
     (T, K), (rows, n) = row_of.shape, ys.shape
     _typed("wts", wts, torch.float32, (T, K))
     if out is None:
-        out = ys.new_empty(T, n)
-    ldo = _matrix("out", out, ys.dtype, (T, n))
+        out, ldo = ys.new_empty(T, n), n
+    else:
+        ldo = _matrix("out", out, ys.dtype, (T, n))
     check(fast.moe_unsort_rows(_raw_stream(stream), ys.data_ptr(), ldy, rows, DTYPES[ys.dtype], wts.data_ptr(), row_of.data_ptr(), T, K, n, out.data_ptr(), ldo))
     return out
 
@@ -341,8 +351,9 @@ def moe_unsort_rows_backward(gout: torch.Tensor, ys: torch.Tensor, wts: torch.Te
     ldg = _matrix("gout", gout, ys.dtype, (T, n))
     _typed("wts", wts, torch.float32, (T, K))
     if gys is None:
-        gys = ys.new_empty(rows, n)
-    ldgy = _matrix("gys", gys, ys.dtype, (rows, n))
+        gys, ldgy = ys.new_empty(rows, n), n
+    else:
+        ldgy = _matrix("gys", gys, ys.dtype, (rows, n))
     gwts = torch.empty_like(wts)
     check(fast.moe_unsort_rows_backward(_raw_stream(stream), gout.data_ptr(), ldg, ys.data_ptr(), ldy, rows, DTYPES[ys.dtype], wts.data_ptr(), row_of.data_ptr(), T, K, n,
                                         gys.data_ptr(), ldgy, gwts.data_ptr()))

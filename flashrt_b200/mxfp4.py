@@ -10,7 +10,7 @@ import torch
 
 from . import lib as _l
 from .lib import FrxError, check, fast, lib
-from .moe import DTYPES, _ids, _matrix, _on_device, _raw_stream, _typed, _ws_span
+from .moe import DTYPES, _code, _ids, _matrix, _on_device, _raw_stream, _typed, _ws_span
 
 BLOCK, UNIT = 32, 128       # values that share a scale; columns of a unit of the packed layout
 
@@ -42,9 +42,10 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     _on_device(codes, scales, out)
     T, n = _quantized(codes, scales)
     if out is None:
-        out = codes.new_empty(T, n, dtype=dtype)
-    ldo = _matrix("out", out, out.dtype if out.dtype in DTYPES else dtype, (T, n))
-    check(fast.mxfp4_dequantize(_raw_stream(stream), codes.data_ptr(), scales.data_ptr(), T, n, DTYPES[out.dtype], out.data_ptr(), ldo))
+        out, ldo = codes.new_empty(T, n, dtype=dtype), n
+    else:
+        ldo = _matrix("out", out, None, (T, n))
+    check(fast.mxfp4_dequantize(_raw_stream(stream), codes.data_ptr(), scales.data_ptr(), T, n, _code(out.dtype), out.data_ptr(), ldo))
     return out
 
 
@@ -96,9 +97,10 @@ def matmul(codes: torch.Tensor, scales: torch.Tensor, w: Packed, out: torch.Tens
     if w.E != 1:
         raise FrxError(_l.ERR_ARG, f"matmul: {w.E} matrices: moe_matmul takes several")
     if out is None:
-        out = codes.new_empty(T, w.rows, dtype=dtype)
-    ldo = _matrix("out", out, None, (T, w.rows))
-    check(fast.mxfp4_matmul(_raw_stream(stream), codes.data_ptr(), scales.data_ptr(), T, n, w.data.data_ptr(), w.rows, out.data_ptr(), ldo, DTYPES[out.dtype]))
+        out, ldo = codes.new_empty(T, w.rows, dtype=dtype), w.rows
+    else:
+        ldo = _matrix("out", out, None, (T, w.rows))
+    check(fast.mxfp4_matmul(_raw_stream(stream), codes.data_ptr(), scales.data_ptr(), T, n, w.data.data_ptr(), w.rows, out.data_ptr(), ldo, _code(out.dtype)))
     return out
 
 
@@ -114,10 +116,11 @@ def moe_matmul(codes: torch.Tensor, scales: torch.Tensor, w: Packed, offsets: to
         _typed("slot_of", slot_of, torch.int32)
     S = T if slot_of is None else slot_of.numel()
     if out is None:
-        out = codes.new_empty(S, w.rows, dtype=dtype)
-    ldo = _matrix("out", out, None, (S, w.rows))
+        out, ldo = codes.new_empty(S, w.rows, dtype=dtype), w.rows
+    else:
+        ldo = _matrix("out", out, None, (S, w.rows))
     check(fast.mxfp4_moe_matmul(_raw_stream(stream), codes.data_ptr(), scales.data_ptr(), T, n, w.data.data_ptr(), w.E, w.rows, offsets.data_ptr(),
-                                None if slot_of is None else slot_of.data_ptr(), K, S, out.data_ptr(), ldo, DTYPES[out.dtype]))
+                                None if slot_of is None else slot_of.data_ptr(), K, S, out.data_ptr(), ldo, _code(out.dtype)))
     return out
 
 
@@ -142,11 +145,12 @@ def moe_layer(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_gate: Pac
     if gate_n != n or w_up[1:] != (E, ff, n) or w_down[1:] != (E, n, ff):
         raise FrxError(_l.ERR_ARG, f"matrices (experts, rows, columns) {w_gate[1:]}, {w_up[1:]}, {w_down[1:]} for rows of {n} values: two of {(E, ff, n)} and {(E, n, ff)} are wanted")
     if out is None:
-        out = x.new_empty(T, n, dtype=dtype or x.dtype)
-    ldo = _matrix("out", out, None, (T, n))
+        out, ldo = x.new_empty(T, n, dtype=dtype or x.dtype), n
+    else:
+        ldo = _matrix("out", out, None, (T, n))
     if ws is None:
         ws = x.new_empty(moe_layer_workspace_bytes(T, K, n, ff, E) + 256, dtype=torch.uint8)   # (nobody asks for its status)
     wp, wb = _ws_span(ws)
     check(fast.mxfp4_moe_layer(_raw_stream(stream), gate.data_ptr(), up.data_ptr(), down.data_ptr(), E, n, ff, x.data_ptr(), ldx, DTYPES[x.dtype],
-                               ids.data_ptr(), wts.data_ptr(), T, K, out.data_ptr(), ldo, DTYPES[out.dtype], wp, wb))
+                               ids.data_ptr(), wts.data_ptr(), T, K, out.data_ptr(), ldo, _code(out.dtype), wp, wb))
     return out
