@@ -353,7 +353,7 @@ __device__ __forceinline__ void swiglu8(const uint32_t (&g)[8], const uint32_t (
         const float a = __uint_as_float(g[i]);
         float e, r;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * -1.44269504f));
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));   // (a subnormal from 2^126 on: the product with a is not one)
         h[i] = a * r * __uint_as_float(u[i]);
         top[i] = __reduce_max_sync(0xffffffffu, __float_as_uint(h[i]) & 0x7fffffffu);
         mine = (lane & 7u) == unsigned(i) ? top[i] : mine;
