@@ -202,8 +202,18 @@ __device__ __forceinline__ void tma_rows16(uint32_t dst, const CUtensorMap* map,
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t abort, uint64_t limit_ns) {
     bool ok = mbar_try_wait(bar, parity);
     if (!ok) {
-        mbar_spin_slow(bar, parity, abort, limit_ns);
-        ok = lds32(abort) == 0;
+        uint64_t t0 = 0;
+        for (uint32_t polls = 1; !(ok = mbar_try_wait(bar, parity)); ++polls) {   // (a poll suspends the thread for microseconds by itself)
+            if (polls & 7u) continue;
+            if (lds32(abort)) break;
+            const uint64_t now = global_ns();
+            if (t0 == 0) {
+                t0 = now;
+            } else if (now - t0 > limit_ns) {
+                sts32(abort, 1u);
+                break;
+            }
+        }
     }
     return __all_sync(0xffffffffu, ok);
 }

@@ -489,6 +489,34 @@ def test_moe_layer_captured_on_another_stream_and_two_at_once():
             assert torch.equal(out, w)
 
 
+def test_a_wait_that_runs_out_leaves_nan_and_is_reported():
+    """A row of a million columns keeps the epilogue waiting for milliseconds; with a limit of ten microseconds it gives up. Nothing hangs, no wrong number is
+    left, and the next call is right again."""
+    from flashrt_b200.lib import check, lib
+    n, rows, ff = 1 << 20, 128, 128
+    xq, wq = random_quantized((3, n), 1, 0), random_quantized((rows, n), 2, 0)
+    w, dx = mxfp4.pack(wq[0].cuda(), wq[1].cuda()), [t.cuda() for t in xq]
+    x, ids, wts = torch.randn(3, n, generator=gen(3)).cuda(), torch.zeros(3, 1, dtype=torch.int32).cuda(), torch.ones(3, 1).cuda()
+    down = mxfp4.pack(*(t.cuda() for t in random_quantized((1, n, ff), 4, 0)))
+    ws = moe.workspace(mxfp4.moe_layer_workspace_bytes(3, 1, n, ff, 1))
+    layer = mxfp4.moe_layer(x, ids, wts, w, w, down, ws=ws)
+    moe.workspace_status(ws)
+    try:
+        check(lib.frx_debug_set_wait_limit_ns(10_000))
+        y = mxfp4.matmul(*dx, w, dtype=torch.float32)
+        torch.cuda.synchronize()
+        assert bool(y.isnan().any()), "the wait did not run out"
+        lost = mxfp4.moe_layer(x, ids, wts, w, w, down, ws=ws)
+        with pytest.raises(moe.FrxError, match="ran out"):
+            moe.workspace_status(ws)
+        assert bool(lost.isnan().any())
+    finally:
+        check(lib.frx_debug_set_wait_limit_ns(0))
+    check_product(mxfp4.matmul(*dx, w, dtype=torch.float32), values(*xq), values(*wq), torch.float32)
+    assert torch.equal(mxfp4.moe_layer(x, ids, wts, w, w, down, ws=ws), layer)
+    moe.workspace_status(ws)
+
+
 def test_refusals():
     x, q = torch.zeros(4, 256, device="cuda"), random_quantized((4, 256), 1)
     dq = [t.cuda() for t in q]
