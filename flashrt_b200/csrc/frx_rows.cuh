@@ -27,6 +27,17 @@ struct alignas(sizeof(T) * N) Vec {
     T v[N];
 };
 
+// A vector that is not needed again after this read: its lines are the first to leave the L2.
+template <class V>
+__device__ __forceinline__ V load_last(const V* p) {
+    if constexpr (sizeof(V) == 16) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+        return *reinterpret_cast<const V*>(&u);
+    } else {
+        return *p;
+    }
+}
+
 // Whether rows of n elements at `p`, `ld` elements apart, can be moved 16 bytes at a time.
 inline bool rows_vec16(const void* p, int64_t ld, int n, int size) {
     return (reinterpret_cast<uintptr_t>(p) % 16) == 0 && (ld * size) % 16 == 0 && (int64_t(n) * size) % 16 == 0;

@@ -8,7 +8,8 @@
 // Every one is a pass over the S rows that must be read or written, so bandwidth is the bound. They all walk tokens, not
 // rows: a token's row is then read (or written) once and its K sorted rows are whole contiguous rows, so nothing is read
 // twice and sums over k need no atomics: they are made in k order, in 32 bits, and round once. 163,840 bf16 rows of 2,048 (16,384 tokens): out 119 us (6.2 TB/s),
-// back 111 (6.65), gradients of back 244 (5.8).
+// back 112 (6.6), gradients of back 231 (6.1). The sorted rows of the way back are read for the last time there (load_last): 4,096 tokens 27.6 us instead of 30.9, gradients
+// 61.7 instead of 65.4, since what is written next finds room in the L2.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(256) k_rows_back(const T* __restrict__ ys, int
 #pragma unroll
             for (int k = 0; k < FLIGHT; ++k) {   // (behind the last row the last again, with weight 0 and not added)
                 const int at = min(k0 + k, count - 1);
-                v[k] = *reinterpret_cast<const Vec<T, N>*>(ys + size_t(list.row[at]) * ldy + i);
+                v[k] = load_last(reinterpret_cast<const Vec<T, N>*>(ys + size_t(list.row[at]) * ldy + i));
                 w[k] = wts ? __ldg(wts + t * K + list.slot[at]) : 1.0f;
             }
 #pragma unroll
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(256) k_rows_back_grad(const T* __restrict__ go
             Vec<T, N> v[FLIGHT];
             const Vec<T, N> g = *reinterpret_cast<const Vec<T, N>*>(gout + t * ldg + i);
 #pragma unroll
-            for (int k = 0; k < FLIGHT; ++k) v[k] = *reinterpret_cast<const Vec<T, N>*>(ys + at[k] * ldy + i);
+            for (int k = 0; k < FLIGHT; ++k) v[k] = load_last(reinterpret_cast<const Vec<T, N>*>(ys + at[k] * ldy + i));
 #pragma unroll
             for (int k = 0; k < FLIGHT; ++k)
                 if (k0 + k < count) {
