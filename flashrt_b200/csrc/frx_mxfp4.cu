@@ -259,6 +259,7 @@ struct MxWalk {
     MxTables tab;
     int E, tile, e;
     int rp, row0, live, width;   // row pair, first y row, y rows, their number rounded up to 16
+    bool alone;                  // the expert has one block of y rows: this tile's weights are read by no other
     __device__ __forceinline__ void begin(const MxTables& tables, int experts) {
         tab = tables;
         E = experts;
@@ -283,6 +284,7 @@ struct MxWalk {
         }
         if (e >= E) return false;
         const int local = tile - (e ? tab.tile_end[e - 1] : 0), bw = tab.blocks[e], w = int(unsigned(bw) >> 24), blocks = bw & 0xffffff;
+        alone = blocks == 1;
         rp = blocks == 1 ? local : int(unsigned(local) / unsigned(blocks));
         const int b = local - rp * blocks;
         row0 = tab.first[e] + b * w;
@@ -482,6 +484,9 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         // ---------------- weights: one lane, a bulk copy per row tile and stage
         uint32_t st = 0, phase = 1;
         const size_t tile_bytes = size_t(units) * kMxUnitBytes;
+        // Weights that no other tile reads leave the L2 first: they would push out what is read again (hidden rows, y). A layer of 64 tokens 111.5 -> 107.5 us, of 4,096
+        // 244 -> 238.
+        const uint64_t once = l2_policy_evict_first(), again = l2_policy_evict_normal();
         bool ok = true;
         while (ok && t.next()) {
             const uint8_t *w0, *w1;
@@ -500,8 +505,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
                 if (!(ok = warp_wait(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns))) break;
                 if (lane == 0) {
                     mbar_expect_tx(full, (second ? 2 * bytes : bytes) + uint32_t(t.width) * kRowB);   // the gathered rows' bytes too
-                    bulk_g2s(dst, w0, bytes, full);
-                    if (second) bulk_g2s(dst + kTileW, w1, bytes, full);
+                    bulk_g2s_hint(dst, w0, bytes, full, t.alone ? once : again);
+                    if (second) bulk_g2s_hint(dst + kTileW, w1, bytes, full, t.alone ? once : again);
                 }
                 __syncwarp();
                 w0 += kTileW;
