@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kMxTileRows) k_mx_pack(uint4* __restrict__ cod
 // tile's products, and four sets of scales (16 columns each).
 //
 // What bounds it. Up to a few rows an expert: the weights. 64 tokens of ten experts out of 512 (2048 / 512; gate and up): 408 MB from DRAM in 61 us between
-// launches, 6.7 TB/s; 10 us of the layer's 111 are the start of the two products and their uneven ends. 4,096 tokens: 100 us for 570 MB of weights. 16,384 tokens
+// launches, 6.7 TB/s; 10 us of the layer's 108 are the start of the two products and their uneven ends. 4,096 tokens: 100 us for 570 MB of weights. 16,384 tokens
 // (three blocks of 107 rows an expert): 262 us for 687 GFLOP at full clocks, the thread that issues (a stage's hand-offs, six copies of scales and eight MMAs take
 // 900 clocks, of which the MMAs are 464) and the L2, which delivers 55 bytes a clock and SM without any MMA; in a stream of such layers the GPU is at its power
 // limit (1,000 W) and at 1,650 MHz.
