@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(256) k_rows_back(const T* __restrict__ ys, int
     if (early) pdl_wait();
     pdl_trigger();
     const int count = list.count;
-    for (int i = threadIdx.x * N; i < n; i += blockDim.x * N) {
+    for (int i = (blockIdx.y * blockDim.x + threadIdx.x) * N; i < n; i += gridDim.y * blockDim.x * N) {
         float acc[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] = 0.0f;
@@ -359,6 +359,8 @@ inline int rows_in_flight(int K, std::initializer_list<int> choices) {
     return best;
 }
 
+// Blocks that share a token's row: one, or with few tokens one for each 256 pieces of it (a token's loads then wait for one another once less).
+inline unsigned row_parts(int T, int pieces) { return T <= 128 ? unsigned(std::max(1, std::min(8, (pieces + 255) / 256))) : 1u; }
 inline unsigned row_threads(int pieces) { return unsigned(std::min(256, std::max(32, (pieces + 31) / 32 * 32))); }
 
 }  // namespace
@@ -386,7 +388,7 @@ int rows_back(const void* ys, int64_t ldy, int in_dtype, const float* wts, const
         using O_ = decltype(o);
         constexpr int N = decltype(width)::value;
         auto with_flight = [&](auto flight) {
-            FRX_LAUNCH(kKCombine, stream, launch_pdl(k_rows_back<T_, O_, N, decltype(flight)::value>, dim3(T), dim3(row_threads((n + N - 1) / N)), 0, stream,
+            FRX_LAUNCH(kKCombine, stream, launch_pdl(k_rows_back<T_, O_, N, decltype(flight)::value>, dim3(T, row_parts(T, (n + N - 1) / N)), dim3(row_threads((n + N - 1) / N)), 0, stream,
                                                      static_cast<const T_*>(ys), ldy, wts, row_of, K, n, static_cast<O_*>(out), ldo, rows, early));
         };
         switch (rows_in_flight(K, {2, 4, 5, 8})) {
@@ -400,6 +402,8 @@ int rows_back(const void* ys, int64_t ldy, int in_dtype, const float* wts, const
         with_rows(in_dtype, vec, [&](auto v, auto width) { launch(v, v, width); });
     else if (in_dtype == FRX_F32 && out_dtype == FRX_F16)   // (the expert layer's: rows kept in 32 bits)
         vec ? launch(float{}, __half{}, std::integral_constant<int, 4>{}) : launch(float{}, __half{}, std::integral_constant<int, 1>{});
+    else if (in_dtype == FRX_F32 && out_dtype == FRX_BF16)
+        vec ? launch(float{}, __nv_bfloat16{}, std::integral_constant<int, 4>{}) : launch(float{}, __nv_bfloat16{}, std::integral_constant<int, 1>{});
     else
         return fail(FRX_ERR_ARG, "rows of type %d to rows of type %d", in_dtype, out_dtype);
     FRX_CUDA(cudaGetLastError());
