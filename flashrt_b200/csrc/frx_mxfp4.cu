@@ -742,7 +742,7 @@ int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
     const int64_t row_tiles = (p.rows + kMxTileRows - 1) / kMxTileRows, blocks = int64_t(p.S) / kTok + std::min(p.E, p.S);   // blocks of y rows at most
     p.single = MODE != kYswiglu && row_tiles * blocks <= sm_count();
     const int64_t pairs = MODE == kYswiglu || p.single ? row_tiles : (row_tiles + 1) / 2;
-    if (int64_t(p.S) / kTok >= (1 << 24) || (int64_t(p.S) / kTok + p.E) * pairs > 0x7fff0000) return fail(FRX_ERR_SHAPE, "MXFP4 product: %d rows by %d is more than 2^31 tiles", p.S, p.rows);
+    if ((int64_t(p.S) + kTok - 1) / kTok >= (1 << 24) || (int64_t(p.S) / kTok + p.E) * pairs > 0x7fff0000) return fail(FRX_ERR_SHAPE, "MXFP4 product: %d rows by %d is more than 2^31 tiles", p.S, p.rows);
     constexpr size_t kSmem = 227 * 1024;
     static std::mutex mu;
     static bool done[64] = {};

@@ -12,7 +12,8 @@ from . import lib as _l
 from .lib import FrxError, check, fast, lib
 from .moe import DTYPES, _code, _ids, _matrix, _on_device, _raw_stream, _typed, _ws_span
 
-BLOCK, UNIT = 32, 128       # values that share a scale; columns of a unit of the packed layout
+BLOCK, UNIT = 32, 128       # values that share a scale; rows and columns of a unit of the packed layout
+UNIT_BYTES = 8704           # of a unit: its codes and scales
 
 
 def quantize(x: torch.Tensor, stream=None):
@@ -57,6 +58,13 @@ class Packed(NamedTuple):
     n: int
 
 
+def _whole(w: Packed) -> None:
+    """The matrices that a Packed names lie in its data (a slice of another one may not)."""
+    data, E, rows, n = w
+    if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() < E * (-(-rows // UNIT) * (n // UNIT) * UNIT_BYTES):
+        raise FrxError(_l.ERR_ARG, f"a packed matrix: {E} of {rows} x {n} are not in {data.numel()} contiguous elements of {data.dtype}")
+
+
 def packed_bytes(rows: int, n: int) -> int:
     return int(lib.frx_mxfp4_packed_bytes(rows, n))
 
@@ -79,12 +87,14 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, stream=None) -> Packed:
 def unpack(w: Packed, stream=None):
     """codes and scales of a Packed (the inverse of pack)."""
     _on_device(w.data)
+    _whole(w)
     codes, scales = w.data.new_empty(w.E, w.rows, w.n // 2), w.data.new_empty(w.E, w.rows, w.n // BLOCK)
     check(lib.frx_mxfp4_unpack(_raw_stream(stream), w.data.data_ptr(), w.E, w.rows, w.n, codes.data_ptr(), scales.data_ptr()))
     return codes, scales
 
 
 def _columns(w: Packed, n: int) -> None:
+    _whole(w)
     if w.n != n:
         raise FrxError(_l.ERR_ARG, f"a matrix of {w.n} columns for rows of {n} values")
 
@@ -144,6 +154,8 @@ def moe_layer(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_gate: Pac
     _typed("wts", wts, torch.float32, shape)
     if gate_n != n or w_up[1:] != (E, ff, n) or w_down[1:] != (E, n, ff):
         raise FrxError(_l.ERR_ARG, f"matrices (experts, rows, columns) {w_gate[1:]}, {w_up[1:]}, {w_down[1:]} for rows of {n} values: two of {(E, ff, n)} and {(E, n, ff)} are wanted")
+    for w in (w_gate, w_up, w_down):
+        _whole(w)
     if out is None:
         out, ldo = x.new_empty(T, n, dtype=dtype or x.dtype), n
     else:

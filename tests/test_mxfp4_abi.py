@@ -81,3 +81,26 @@ def test_layer_refusals(L):
                      (14, None, L.ERR_ARG), (14, odd, L.ERR_ARG), (15, n - 1, L.ERR_ARG), (16, -1, L.ERR_ARG), (17, None, L.ERR_ARG), (17, C.c_void_p(4100), L.ERR_ARG), (18, need - 1, L.ERR_WORKSPACE)):
         assert L.lib.frx_mxfp4_moe_layer(*with_(ok, i, v)) == rc, (i, v)
     assert L.lib.frx_mxfp4_moe_layer(*with_(with_(ok, 12, 0), 7, None)) == L.OK
+
+
+@pytest.mark.parametrize("bad", ["short", "type", "strides", "experts"])
+def test_a_packed_matrix_that_is_not_whole_is_refused(L, bad):
+    import torch
+
+    from flashrt_b200 import mxfp4
+    data = torch.zeros(2 * mxfp4.packed_bytes(200, 256), dtype=torch.uint8)
+    assert data.numel() == 2 * 4 * 8704
+    mxfp4._whole(mxfp4.Packed(data, 2, 200, 256))
+    w = {"short": (data[:-1], 2, 200, 256), "type": (data.view(torch.int8), 2, 200, 256), "strides": (data.repeat(2)[::2], 2, 200, 256), "experts": (data, 3, 200, 256)}[bad]
+    with pytest.raises(L.FrxError):
+        mxfp4._whole(mxfp4.Packed(*w))
+    with pytest.raises(L.FrxError):
+        mxfp4._columns(mxfp4.Packed(*w), 256)
+    with pytest.raises(L.FrxError):
+        mxfp4._columns(mxfp4.Packed(data, 2, 200, 256), 128)
+
+
+def test_more_rows_than_an_expert_holds_are_refused(L):
+    # an expert's blocks of 112 rows are counted in 24 bits
+    most = 112 * (2 ** 24 - 1)
+    assert L.lib.frx_mxfp4_matmul(None, P, P, most + 1, 128, P, 1, P, 1, 0) == L.ERR_SHAPE
