@@ -209,7 +209,7 @@ int frx_moe_sort(frx_stream_t stream, const int32_t* ids, int T, int K, int E, i
                  size_t ws_bytes);
 /* The rows: of n elements of `dtype`, ld* elements apart (ld >= n; any alignment of an element: rows that are 16-byte aligned and a
  * multiple of 16 bytes long are moved 16 bytes at a time). `rows` is how many rows the sorted buffer has; slots with no row in it
- * (row_of < 0 or >= rows) are left out of everything. Rows that no slot has are not written. Buffers do not overlap. Sums are formed in 32 bits, in
+ * (row_of < 0 or >= rows) are left out of everything. No two slots have the same row (frx_moe_sort gives none twice). Rows that no slot has are not written. Buffers do not overlap. Sums are formed in 32 bits, in
  * k order, and rounded once.
  *   sort_rows:            xs[row_of[t][k]] = x[t]
  *   sort_rows_backward:   gx[t] = sum_k gxs[row_of[t][k]]
