@@ -14,6 +14,7 @@ from .moe import DTYPES, _code, _ids, _matrix, _on_device, _raw_stream, _typed, 
 
 BLOCK, UNIT = 32, 128       # values that share a scale; rows and columns of a unit of the packed layout
 UNIT_BYTES = 8704           # of a unit: its codes and scales
+ROWS_BF16 = 16              # FRX_ROWS_BF16
 
 
 def quantize(x: torch.Tensor, stream=None):
@@ -139,9 +140,10 @@ def moe_layer_workspace_bytes(T: int, K: int, n: int, ff: int, E: int) -> int:
 
 
 def moe_layer(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_gate: Packed, w_up: Packed, w_down: Packed, out: torch.Tensor | None = None,
-              dtype: torch.dtype | None = None, ws: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+              dtype: torch.dtype | None = None, ws: torch.Tensor | None = None, stream=None, rows: torch.dtype = torch.float32) -> torch.Tensor:
     """The expert layer in MXFP4 (frx_mxfp4_moe_layer): out[t] = sum over k of wts[t][k] * expert_{ids[t][k]}(x[t]), [T][n] in `dtype` (that of
-    `out`, or of x). Slots with a negative id take no part."""
+    `out`, or of x). Slots with a negative id take no part. `rows`: what the experts' rows are kept in before their sum; bfloat16 for a bfloat16
+    output moves half the bytes and rounds twice."""
     gate, E, ff, gate_n = w_gate
     up, down = w_up[0], w_down[0]
     _on_device(x, ids, wts, out, ws, gate, up, down)
@@ -160,9 +162,14 @@ def moe_layer(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_gate: Pac
         out, ldo = x.new_empty(T, n, dtype=dtype or x.dtype), n
     else:
         ldo = _matrix("out", out, None, (T, n))
+    code = _code(out.dtype)
+    if rows != torch.float32:
+        if rows != torch.bfloat16 or out.dtype != torch.bfloat16:
+            raise FrxError(_l.ERR_ARG, f"moe_layer: rows of {rows} for an output of {out.dtype}: float32, or bfloat16 for a bfloat16 output")
+        code |= ROWS_BF16
     if ws is None:
         ws = x.new_empty(moe_layer_workspace_bytes(T, K, n, ff, E) + 256, dtype=torch.uint8)   # (nobody asks for its status)
     wp, wb = _ws_span(ws)
     check(fast.mxfp4_moe_layer(_raw_stream(stream), gate.data_ptr(), up.data_ptr(), down.data_ptr(), E, n, ff, x.data_ptr(), ldx, DTYPES[x.dtype],
-                               ids.data_ptr(), wts.data_ptr(), T, K, out.data_ptr(), ldo, _code(out.dtype), wp, wb))
+                               ids.data_ptr(), wts.data_ptr(), T, K, out.data_ptr(), ldo, code, wp, wb))
     return out

@@ -49,6 +49,7 @@ enum {
 
 /* Element types of rows, where a call takes several (`dtype` arguments). */
 enum { FRX_F32 = 0, FRX_BF16 = 1, FRX_F16 = 2 };
+enum { FRX_ROWS_BF16 = 16 };   /* or-ed to FRX_BF16 as the out_dtype of frx_mxfp4_moe_layer */
 
 int frx_version(void);
 const char* frx_last_error(void);
@@ -589,7 +590,8 @@ int frx_mxfp4_moe_matmul(frx_stream_t stream, const void* codes, const void* sca
  *   out[t] = sum over k of wts[t][k] * W_down Q(silu(W_gate Q(x_t)) * (W_up Q(x_t))) of expert ids[t][k], Q the quantizer above.
  * w_gate, w_up: E packed matrices [ff][n], w_down: E packed [n][ff]. x, out: rows of n elements of their dtype, ld* apart (out may be x). Slots with a negative id take
  * no part (a token without any gets zeros); an id of E or more is left out too and reported by frx_workspace_status. The experts' rows are kept in
- * bfloat16 where out is and T * n is 65,536 or more, else in float. The hidden rows' codes are those of sums in 32 bits: where such a sum lies within its error of a border between
+ * float and out is rounded once, so that a token's row has the same bits whatever shares its batch; with FRX_BF16 | FRX_ROWS_BF16 as out_dtype they are
+ * rounded to bfloat16 on their way to it (half the bytes, 1.41 times the error of out's own rounding). The hidden rows' codes are those of sums in 32 bits: where such a sum lies within its error of a border between
  * two codes, the code may be either. Any T; K <= 32, E <= 4096, n and ff multiples of 128 up to 2^20, T * K < 2^31. ws 16-byte aligned. */
 size_t frx_mxfp4_moe_layer_workspace_bytes(int T, int K, int n, int ff, int E);
 int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_up, const void* w_down, int E, int n, int ff, const void* x, int64_t ldx,

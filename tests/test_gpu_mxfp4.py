@@ -542,3 +542,50 @@ def test_refusals():
             call()
             raise AssertionError(f"call {i} was not refused")
     mxfp4.moe_layer(x, ids, wts, big, big, down)
+
+
+def layer_of(T, K, E, n, ff, seed=0):
+    ids, wts = (t.cuda() for t in routed(T, K, E, seed))
+    raw = [random_quantized(s, seed + i) for i, s in enumerate(((E, ff, n), (E, ff, n), (E, n, ff)))]
+    return torch.randn(T, n, generator=gen(seed)).cuda(), ids, wts, [mxfp4.pack(c.cuda(), (s - 6).cuda()) for c, s in raw]
+
+
+@pytest.mark.parametrize("T,n", [(1, 2048), (31, 2048), (32, 2048), (256, 256), (700, 512)])
+def test_moe_layer_output_is_rounded_once(T, n):
+    """A 16-bit output is the 32-bit one, rounded: the experts' rows lose nothing on their way to it, whatever the size."""
+    x, ids, wts, W = layer_of(T, 3, 8, n, 256)
+    full = mxfp4.moe_layer(x, ids, wts, *W, dtype=torch.float32)
+    for dtype in (torch.bfloat16, torch.float16):
+        assert torch.equal(mxfp4.moe_layer(x, ids, wts, *W, dtype=dtype), full.to(dtype))
+
+
+def test_moe_layer_a_token_alone_and_in_a_batch():
+    """The same bits whatever shares the batch."""
+    x, ids, wts, W = layer_of(300, 4, 6, 1024, 128)
+    for rows in (torch.float32, torch.bfloat16):
+        full = mxfp4.moe_layer(x, ids, wts, *W, dtype=torch.bfloat16, rows=rows)
+        for a, b in ((0, 1), (7, 8), (31, 63), (100, 300)):
+            assert torch.equal(mxfp4.moe_layer(x[a:b], ids[a:b], wts[a:b], *W, dtype=torch.bfloat16, rows=rows), full[a:b])
+
+
+@pytest.mark.parametrize("T", [5, 300])
+def test_moe_layer_rows_in_bfloat16(T):
+    """Where the caller asks for them: each of the K rows of a token is off by half a step (2^-8) of bfloat16, weighted, and the sum by its own."""
+    x, ids, wts, W = layer_of(T, 3, 8, 512, 256)
+    ws = moe.workspace(mxfp4.moe_layer_workspace_bytes(T, 3, 512, 256, 8))
+    got = mxfp4.moe_layer(x, ids, wts, *W, dtype=torch.bfloat16, rows=torch.bfloat16, ws=ws)
+    moe.workspace_status(ws)
+    want = mxfp4.moe_layer(x, ids, wts, *W, dtype=torch.float32).double()
+    mag = sum(mxfp4.moe_layer(x, ids[:, k:k + 1].contiguous(), wts[:, k:k + 1].contiguous(), *W, dtype=torch.float32).double().abs() for k in range(3))
+    half = torch.finfo(torch.bfloat16).eps / 2
+    bound = (half + 5 * 2.0 ** -24) * mag       # the rows' rounding, three products and additions of either side
+    bound = bound + half * (want.abs() + bound)
+    assert bool(((got.double() - want).abs() <= bound).all())
+    assert not torch.equal(got, want.bfloat16())
+
+
+def test_moe_layer_refuses_rows_that_no_kernel_has():
+    x, ids, wts, W = layer_of(4, 2, 4, 128, 128)
+    for dtype, rows in ((torch.float32, torch.bfloat16), (torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16), (torch.float16, torch.float16)):
+        with pytest.raises(moe.FrxError):
+            mxfp4.moe_layer(x, ids, wts, *W, dtype=dtype, rows=rows)

@@ -104,3 +104,12 @@ def test_more_rows_than_an_expert_holds_are_refused(L):
     # an expert's blocks of 112 rows are counted in 24 bits
     most = 112 * (2 ** 24 - 1)
     assert L.lib.frx_mxfp4_matmul(None, P, P, most + 1, 128, P, 1, P, 1, 0) == L.ERR_SHAPE
+
+
+def test_layer_rows_in_bfloat16_are_for_a_bfloat16_output(L):
+    n, ff, E = 256, 128, 8
+    need = L.lib.frx_mxfp4_moe_layer_workspace_bytes(4, 2, n, ff, E)
+    ok = [None, P, P, P, E, n, ff, P, n, 0, P, P, 4, 2, P, n, 1, P, need]
+    for out_dtype in (16, 18, 32, 33):              # float32 or float16 with the flag, flags that there are not
+        assert L.lib.frx_mxfp4_moe_layer(*with_(ok, 16, out_dtype)) == L.ERR_ARG
+    assert L.lib.frx_mxfp4_moe_layer(*with_(with_(ok, 16, 17), 18, need - 1)) == L.ERR_WORKSPACE     # taken; what is short is the workspace
