@@ -654,8 +654,11 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         uint32_t set = 0, phase = 0;
         if (p.early) pdl_wait();
         const bool pairs = MODE != kYf32 && p.rows % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
+        // A wait ran out: NaN, not a wrong number, and no more waits. (Of the uses of a set of accumulators behind the lost one, every second would find the
+        // parity of the last complete one, and take sums that nobody has finished.)
+        bool lost = false;
         while (t.next()) {
-            const bool lost = !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);   // a wait ran out: NaN, not a wrong number
+            lost = lost || !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);
             tc_fence_after_sync();
             const uint32_t acc = tmem + (uint32_t(quarter * 32) << 16) + set * kColsAcc;
             const int eights = t.width >> 3;

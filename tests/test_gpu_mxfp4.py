@@ -589,3 +589,29 @@ def test_moe_layer_refuses_rows_that_no_kernel_has():
     for dtype, rows in ((torch.float32, torch.bfloat16), (torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16), (torch.float16, torch.float16)):
         with pytest.raises(moe.FrxError):
             mxfp4.moe_layer(x, ids, wts, *W, dtype=dtype, rows=rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tiles_behind_a_wait_that_ran_out_are_nan_too(dtype):
+    """Six tiles a block of some hundreds of microseconds each, and a limit of ten: every output is the right one or NaN, in the tiles behind the first lost one too."""
+    from flashrt_b200.lib import check, lib
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    T, n, rows = 6 * 112 * sms, 1 << 17, 128
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    codes = torch.randint(0, 256, (T, n // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.full((T, n // 32), 120, device="cuda", dtype=torch.uint8)
+    wq = random_quantized((rows, n), 2, 0)
+    w = mxfp4.pack(wq[0].cuda(), wq[1].cuda())
+    want = mxfp4.matmul(codes, scales, w, dtype=dtype)
+    assert not bool(want.isnan().any())
+    try:
+        check(lib.frx_debug_set_wait_limit_ns(10_000))
+        y = mxfp4.matmul(codes, scales, w, dtype=dtype)
+        torch.cuda.synchronize()
+    finally:
+        check(lib.frx_debug_set_wait_limit_ns(0))
+    lost = y.isnan()
+    assert bool(lost.any()), "no wait ran out"
+    assert bool((lost | (y == want)).all())
+    assert torch.equal(mxfp4.matmul(codes, scales, w, dtype=dtype), want)
