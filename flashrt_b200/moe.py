@@ -38,6 +38,16 @@ def _stream(stream=None):
     return C.c_void_p(_raw_stream(stream))
 
 
+def _on(stream, call, *args, **kwargs):
+    """The call with `stream` as the current one, for calls that allocate: their tensors, and above all a workspace that is dropped on return, then belong to the
+    stream that uses them. (Memory of the current stream may still be in use by its kernels when another stream gets it, and is given away
+    while that one still uses it.)"""
+    if _current_device and stream.device_index == _current_device() and stream.cuda_stream == _current_raw_stream(_current_device()):
+        return call(*args, **kwargs)
+    with torch.cuda.stream(stream):
+        return call(*args, **kwargs)
+
+
 def _addr(t: torch.Tensor | None):
     """The address of t, or None: a tensor that must be there is refused by the library, with its own error."""
     return None if t is None else t.data_ptr()
@@ -65,6 +75,8 @@ def expert_stride(n: int, ff: int) -> int:
 
 def repack(ggml_rows: torch.Tensor, rows: int, cols: int, stream=None) -> torch.Tensor:
     """q2_0::repack on the device: ggml blocks (uint8) -> planar matrix (uint8)."""
+    if stream is not None:
+        return _on(stream, repack, ggml_rows, rows, cols)
     _dev(ggml_rows)
     out = torch.empty(mat_bytes(rows, cols), dtype=torch.uint8, device=ggml_rows.device)
     check(lib.frx_q2_repack(_ptr(ggml_rows), rows, cols, _ptr(out), _stream(stream)))
@@ -74,6 +86,8 @@ def repack(ggml_rows: torch.Tensor, rows: int, cols: int, stream=None) -> torch.
 def tile_experts(planar: torch.Tensor, n: int, ff: int, n_experts: int, src_stride: int | None = None,
                  dst_stride: int | None = None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Planar expert blobs -> the tiled layout the kernels read."""
+    if stream is not None:
+        return _on(stream, tile_experts, planar, n, ff, n_experts, src_stride=src_stride, dst_stride=dst_stride, out=out)
     _dev(planar, out)
     src_stride = expert_bytes(n, ff) if src_stride is None else src_stride
     dst_stride = expert_stride(n, ff) if dst_stride is None else dst_stride
@@ -85,6 +99,8 @@ def tile_experts(planar: torch.Tensor, n: int, ff: int, n_experts: int, src_stri
 
 def untile_experts(tiled: torch.Tensor, n: int, ff: int, n_experts: int, src_stride: int | None = None,
                    dst_stride: int | None = None, stream=None) -> torch.Tensor:
+    if stream is not None:
+        return _on(stream, untile_experts, tiled, n, ff, n_experts, src_stride=src_stride, dst_stride=dst_stride)
     _dev(tiled)
     src_stride = expert_stride(n, ff) if src_stride is None else src_stride
     dst_stride = expert_bytes(n, ff) if dst_stride is None else dst_stride
@@ -95,6 +111,8 @@ def untile_experts(tiled: torch.Tensor, n: int, ff: int, n_experts: int, src_str
 
 def dequant_expert(tiled_blob: torch.Tensor, n: int, ff: int, stream=None):
     """(q - 1) * d of one tiled expert: gate [ff][n], up [ff][n], down [n][ff] fp32."""
+    if stream is not None:
+        return _on(stream, dequant_expert, tiled_blob, n, ff)
     _dev(tiled_blob)
     dev = tiled_blob.device
     g = torch.empty(ff, n, dtype=torch.float32, device=dev)
@@ -137,6 +155,8 @@ class ExpertArena:
 
     def read_planar(self, layer: int, expert0: int, count: int, stream=None) -> torch.Tensor:
         """The planar form of `count` blobs of the arena (the inverse of load_planar): uint8 [count][blob_bytes]."""
+        if stream is not None:
+            return _on(stream, self.read_planar, layer, expert0, count)
         out = torch.zeros(count, self.blob_bytes, dtype=torch.uint8, device="cuda")
         check(lib.frx_q2_untile_experts(C.c_void_p(self.blob(layer, expert0)), self.stride, _ptr(out), self.blob_bytes, count, self.n, self.ff,
                                         _stream(stream)))
@@ -200,6 +220,8 @@ def moe_route_topk(logits: torch.Tensor, k: int, counts: torch.Tensor | None = N
                    tail_counts: torch.Tensor | None = None, tail_from: int = 1 << 30, stream=None):
     """qwen4exp::moe_route_topk: ids int32 [T][k] (descending probability, ties to the lower
     index) and weights float [T][k]."""
+    if stream is not None:
+        return _on(stream, moe_route_topk, logits, k, counts=counts, tail_counts=tail_counts, tail_from=tail_from)
     _dev(logits, counts, tail_counts)
     T, E = logits.shape
     ids = logits.new_empty(T, k, dtype=torch.int32)
@@ -211,6 +233,8 @@ def moe_route_topk(logits: torch.Tensor, k: int, counts: torch.Tensor | None = N
 def router_logits(w_router: torch.Tensor, w_gate: torch.Tensor | None, x: torch.Tensor, stream=None):
     """The projection in front of the router (frx_router_logits): w_router bf16 [E][n], w_gate bf16 [n]
     or None, x fp32 [T][n] -> (logits fp32 [T][E], gate_logit fp32 [T] or None)."""
+    if stream is not None:
+        return _on(stream, router_logits, w_router, w_gate, x)
     _dev(w_router, w_gate, x)
     if w_router.dtype != torch.bfloat16 or (w_gate is not None and w_gate.dtype != torch.bfloat16) or x.dtype != torch.float32:
         raise FrxError(_l.ERR_ARG, "router_logits: bf16 weights and fp32 activations")
@@ -224,6 +248,8 @@ def router_logits(w_router: torch.Tensor, w_gate: torch.Tensor | None, x: torch.
 
 def quantize_q8(x: torch.Tensor, stream=None):
     """q2_0::quantize_q8 for every row of x [T][n]: codes int8 [T][n], scales float [T][n/32]."""
+    if stream is not None:
+        return _on(stream, quantize_q8, x)
     _dev(x)
     T, n = x.shape
     q = x.new_empty(T, n, dtype=torch.int8)
@@ -285,6 +311,8 @@ def moe_sort(ids: torch.Tensor, E: int, ws: torch.Tensor | None = None, stream=N
     """The plan that sorts the slots of ids int32 [T][K] by expert (frx_moe_sort): offsets int32 [E + 1], slot_of int32 [T * K],
     row_of int32 [T][K]; -1 where a slot has no row (its id is negative) or a row no slot. An id of E or more has none either, and is reported by
     workspace_status(ws) where a workspace is given."""
+    if stream is not None:
+        return _on(stream, moe_sort, ids, E, ws=ws)
     _on_device(ids, ws)
     _ids("ids", ids)
     T, K = ids.shape
@@ -298,6 +326,8 @@ def moe_sort(ids: torch.Tensor, E: int, ws: torch.Tensor | None = None, stream=N
 
 def moe_sort_rows(x: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """xs[row_of[t][k]] = x[t]: x [T][n] float32, bfloat16 or float16 -> xs [T * K][n]. Rows that no slot has are left as they were."""
+    if stream is not None:
+        return _on(stream, moe_sort_rows, x, row_of, out=out)
     _on_device(x, row_of, out)
     ldx = _matrix("x", x)
     _ids("row_of", row_of)
@@ -313,6 +343,8 @@ def moe_sort_rows(x: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | Non
 
 def moe_sort_rows_backward(gxs: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """gx[t] = sum over k of gxs[row_of[t][k]]: the gradient of moe_sort_rows."""
+    if stream is not None:
+        return _on(stream, moe_sort_rows_backward, gxs, row_of, out=out)
     _on_device(gxs, row_of, out)
     ldg = _matrix("gxs", gxs)
     _ids("row_of", row_of)
@@ -328,6 +360,8 @@ def moe_sort_rows_backward(gxs: torch.Tensor, row_of: torch.Tensor, out: torch.T
 def moe_unsort_rows(ys: torch.Tensor, wts: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """out[t] = sum over k of wts[t][k] * ys[row_of[t][k]]: sorted rows back to their tokens, with the routing weights applied. A token
     none of whose slots has a row gets zeros."""
+    if stream is not None:
+        return _on(stream, moe_unsort_rows, ys, wts, row_of, out=out)
     _on_device(ys, wts, row_of, out)
     ldy = _matrix("ys", ys)
     _ids("row_of", row_of)
@@ -344,6 +378,8 @@ def moe_unsort_rows(ys: torch.Tensor, wts: torch.Tensor, row_of: torch.Tensor, o
 def moe_unsort_rows_backward(gout: torch.Tensor, ys: torch.Tensor, wts: torch.Tensor, row_of: torch.Tensor, gys: torch.Tensor | None = None, stream=None):
     """The gradients of moe_unsort_rows: gys [rows][n] (rows that no slot has are left as they were) and gwts float32 [T][K] (0 for a slot
     without a row)."""
+    if stream is not None:
+        return _on(stream, moe_unsort_rows_backward, gout, ys, wts, row_of, gys=gys)
     _on_device(gout, ys, wts, row_of, gys)
     ldy = _matrix("ys", ys)
     _ids("row_of", row_of)
@@ -363,6 +399,8 @@ def moe_unsort_rows_backward(gout: torch.Tensor, ys: torch.Tensor, wts: torch.Te
 def moe_route_topk_backward(gwts: torch.Tensor, wts: torch.Tensor, ids: torch.Tensor, E: int, stream=None) -> torch.Tensor:
     """The gradient of moe_route_topk: glogits float32 [T][E] from the gradient gwts [T][k] of its weights. `ids` are the chosen experts as the
     router gave them: slots dropped later keep theirs and have the gradient 0 (moe_unsort_rows_backward gives it)."""
+    if stream is not None:
+        return _on(stream, moe_route_topk_backward, gwts, wts, ids, E)
     _on_device(gwts, wts, ids)
     _ids("ids", ids)
     T, k = ids.shape
@@ -410,6 +448,8 @@ def moe_decode(experts: int, stride: int, E: int, shared: int | None, n: int, ff
                yslot: torch.Tensor | None = None, ws: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """out[t] = sum_k w * expert(x_t) (+ shared(x_t) * sigmoid(gate_logit[t])). `experts` and
     `shared` are device addresses of tiled blobs (ExpertArena.blob)."""
+    if stream is not None:
+        return _on(stream, moe_decode, experts, stride, E, shared, n, ff, x, ids, wts, gate_logit, out=out, yslot=yslot, ws=ws)
     _dev(x, ids, wts, gate_logit, out, yslot)
     T, K = ids.shape
     if out is None:
@@ -437,6 +477,8 @@ def moe_layer(experts: int, stride: int, E: int, shared: int | None, n: int, ff:
               gate_logit: torch.Tensor | None, K: int, out: torch.Tensor | None = None, ids_out: torch.Tensor | None = None,
               wts_out: torch.Tensor | None = None, ws: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Router + experts + combine in one call (device tensors)."""
+    if stream is not None:
+        return _on(stream, moe_layer, experts, stride, E, shared, n, ff, x, logits, gate_logit, K, out=out, ids_out=ids_out, wts_out=wts_out, ws=ws)
     _dev(x, logits, gate_logit, out, ids_out, wts_out)
     T = x.shape[0]
     if out is None:
@@ -547,6 +589,8 @@ def moe_hits(hit_ptr: torch.Tensor, hit_n: torch.Tensor, K: int, x: torch.Tensor
              scratch: torch.Tensor | None = None, T: int = 1, stream=None) -> torch.Tensor:
     """qwen4exp::moe_hits: hit_ptr int64 [T][K] device addresses of tiled blobs, hit_n int32 [T];
     yh [T][K][n], rows k >= hit_n[t] are left untouched."""
+    if stream is not None:
+        return _on(stream, moe_hits, hit_ptr, hit_n, K, x, n, ff, yh, scratch=scratch, T=T)
     _dev(hit_ptr, hit_n, x, yh, scratch)
     if scratch is None:
         scratch = workspace(moe_hits_scratch_bytes(K, n, ff, T), x.device)
@@ -558,6 +602,8 @@ def moe_hits(hit_ptr: torch.Tensor, hit_n: torch.Tensor, K: int, x: torch.Tensor
 def moe_combine(yh: torch.Tensor, w: torch.Tensor, hit_n: torch.Tensor | None, shexp: torch.Tensor | None,
                 gate: torch.Tensor | None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """k_moe_combine: out[t] = sum_{k < hit_n[t]} w[t][k] * yh[t][k] + shexp[t] * sigmoid(gate[t])."""
+    if stream is not None:
+        return _on(stream, moe_combine, yh, w, hit_n, shexp, gate, out=out)
     _dev(yh, w, hit_n, shexp, gate, out)
     T, K, n = yh.shape
     if out is None:
@@ -578,6 +624,8 @@ class moe_q2:
             ws: torch.Tensor | None = None, stream=None, form: str = "auto") -> torch.Tensor:
         """yd[t*K + k] = down(silu(gate x_t) * up x_t) of expert ids[t][k], fp32 [T*K][n].
         form: "auto" (by size), "umma" (tcgen05 / tensor memory) or "stream"."""
+        if stream is not None:
+            return _on(stream, moe_q2.run, experts, stride, E, n, ff, x, ids, yd=yd, ws=ws, form=form)
         _dev(x, ids, yd)
         T, K = ids.shape
         if yd is None:
@@ -593,6 +641,8 @@ class moe_q2:
     def run_ex(experts: int, stride: int, E: int, n: int, ff: int, x: torch.Tensor, ids: torch.Tensor, block64: bool = False,
                yd_bf16: bool = False, ws: torch.Tensor | None = None, stream=None, form: str = "auto") -> torch.Tensor:
         """moe_q2::run with its two options: activation scale blocks of 64, and bf16 output rows."""
+        if stream is not None:
+            return _on(stream, moe_q2.run_ex, experts, stride, E, n, ff, x, ids, block64=block64, yd_bf16=yd_bf16, ws=ws, form=form)
         _dev(x, ids)
         T, K = ids.shape
         yd = torch.empty(T * K, n, dtype=torch.bfloat16 if yd_bf16 else torch.float32, device=x.device)
@@ -622,6 +672,8 @@ class gemv:
 
     @staticmethod
     def quantize_q8_1(x: torch.Tensor, stream=None) -> torch.Tensor:
+        if stream is not None:
+            return _on(stream, gemv.quantize_q8_1, x)
         _dev(x)
         n_tok, ncols = x.shape
         xq = x.new_empty(gemv._q8_1_bytes(ncols, n_tok), dtype=torch.uint8)
@@ -630,6 +682,8 @@ class gemv:
 
     @staticmethod
     def swiglu_q8_1(g: torch.Tensor, u: torch.Tensor, stream=None) -> torch.Tensor:
+        if stream is not None:
+            return _on(stream, gemv.swiglu_q8_1, g, u)
         _dev(g, u)
         n_tok, ncols = g.shape
         xq = g.new_empty(gemv._q8_1_bytes(ncols, n_tok), dtype=torch.uint8)
@@ -640,6 +694,8 @@ class gemv:
     def moe_q(ggml_type: int, w: torch.Tensor, gate: torch.Tensor | None, xq: torch.Tensor, ids: torch.Tensor, ncols: int, nrows: int,
               expert_stride_bytes: int, act_per_expert: bool, stream=None) -> torch.Tensor:
         """dst [n_tok][k][nrows] = W_{ids[t][j]} x (silu(G x) * (W x) with gate)."""
+        if stream is not None:
+            return _on(stream, gemv.moe_q, ggml_type, w, gate, xq, ids, ncols, nrows, expert_stride_bytes, act_per_expert)
         _dev(w, gate, xq, ids)
         n_tok, k = ids.shape
         dst = w.new_empty(n_tok, k, nrows, dtype=torch.float32)
@@ -650,6 +706,8 @@ class gemv:
     @staticmethod
     def moe_q2_0(w: torch.Tensor, gate: torch.Tensor | None, xq: torch.Tensor, ids: torch.Tensor, ncols: int, nrows: int,
                  slot_stride_bytes: int, per_channel_act: bool, stream=None) -> torch.Tensor:
+        if stream is not None:
+            return _on(stream, gemv.moe_q2_0, w, gate, xq, ids, ncols, nrows, slot_stride_bytes, per_channel_act)
         _dev(w, gate, xq, ids)
         n_ids = ids.numel()
         dst = w.new_empty(n_ids, nrows, dtype=torch.float32)
@@ -659,6 +717,8 @@ class gemv:
 
     @staticmethod
     def matvec(ggml_type: int, W: torch.Tensor, x: torch.Tensor, nrows: int, stream=None) -> torch.Tensor:
+        if stream is not None:
+            return _on(stream, gemv.matvec, ggml_type, W, x, nrows)
         _dev(W, x)
         n_tok, ncols = x.shape
         y = x.new_empty(n_tok, nrows, dtype=torch.float32)
@@ -692,6 +752,8 @@ class gemm:
 
     @staticmethod
     def moe_run(plan: _GemmPlan, W: torch.Tensor, expert_stride_bytes: int, nrows: int, stream=None) -> torch.Tensor:
+        if stream is not None:
+            return _on(stream, gemm.moe_run, plan, W, expert_stride_bytes, nrows)
         _dev(W)
         y = W.new_empty(plan.T, plan.K, nrows, dtype=torch.float32)
         check(fast.gemm_moe_run(C.addressof(plan), W.data_ptr(), expert_stride_bytes, y.data_ptr(), nrows, _raw_stream(stream)))
@@ -700,6 +762,8 @@ class gemm:
 
 def convert_q8_0_to_q2_0(src: torch.Tensor, stream=None) -> torch.Tensor:
     """qwen4exp::convert_q8_0_to_q2_0 on the device: uint8 [n * 68] Q8_0 block pairs -> uint8 [n * 18] Q2_0 blocks."""
+    if stream is not None:
+        return _on(stream, convert_q8_0_to_q2_0, src)
     _dev(src)
     n = src.numel() // 68
     dst = torch.empty(n * 18, dtype=torch.uint8, device=src.device)
@@ -709,6 +773,8 @@ def convert_q8_0_to_q2_0(src: torch.Tensor, stream=None) -> torch.Tensor:
 
 def chain_rmsnorm_unit(x: torch.Tensor, y: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The layer join of the chained-stack benchmark: (x + y) / sqrt(mean((x + y)^2) + 1e-6) per row."""
+    if stream is not None:
+        return _on(stream, chain_rmsnorm_unit, x, y, out=out)
     _dev(x, y, out)
     T, n = x.shape
     if out is None:

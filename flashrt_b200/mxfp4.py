@@ -10,7 +10,7 @@ import torch
 
 from . import lib as _l
 from .lib import FrxError, check, fast, lib
-from .moe import DTYPES, _code, _ids, _matrix, _on_device, _raw_stream, _typed, _ws_span
+from .moe import DTYPES, _code, _ids, _matrix, _on, _on_device, _raw_stream, _typed, _ws_span
 
 BLOCK, UNIT = 32, 128       # values that share a scale; rows and columns of a unit of the packed layout
 UNIT_BYTES = 8704           # of a unit: its codes and scales
@@ -19,6 +19,8 @@ ROWS_BF16 = 16              # FRX_ROWS_BF16
 
 def quantize(x: torch.Tensor, stream=None):
     """x [T][n] float32, bfloat16 or float16 (n a multiple of 32) -> codes uint8 [T][n / 2], scales uint8 [T][n / 32]."""
+    if stream is not None:
+        return _on(stream, quantize, x)
     _on_device(x)
     ldx = _matrix("x", x)
     T, n = x.shape
@@ -41,6 +43,8 @@ def _quantized(codes: torch.Tensor, scales: torch.Tensor):
 
 def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The values that codes and scales stand for, float32 or bfloat16 [T][n]."""
+    if stream is not None:
+        return _on(stream, dequantize, codes, scales, dtype=dtype, out=out)
     _on_device(codes, scales, out)
     T, n = _quantized(codes, scales)
     if out is None:
@@ -72,6 +76,8 @@ def packed_bytes(rows: int, n: int) -> int:
 
 def pack(codes: torch.Tensor, scales: torch.Tensor, stream=None) -> Packed:
     """codes uint8 [E][rows][n / 2], scales uint8 [E][rows][n / 32] (or one matrix without E) -> Packed; once, when weights are loaded."""
+    if stream is not None:
+        return _on(stream, pack, codes, scales)
     _on_device(codes, scales)
     if codes.dim() == 2:
         codes, scales = codes.unsqueeze(0), scales.unsqueeze(0)
@@ -87,6 +93,8 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, stream=None) -> Packed:
 
 def unpack(w: Packed, stream=None):
     """codes and scales of a Packed (the inverse of pack)."""
+    if stream is not None:
+        return _on(stream, unpack, w)
     _on_device(w.data)
     _whole(w)
     codes, scales = w.data.new_empty(w.E, w.rows, w.n // 2), w.data.new_empty(w.E, w.rows, w.n // BLOCK)
@@ -102,6 +110,8 @@ def _columns(w: Packed, n: int) -> None:
 
 def matmul(codes: torch.Tensor, scales: torch.Tensor, w: Packed, out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """y[t] = W x[t] of quantized rows x and one packed matrix: [T][rows] in `dtype` (or that of `out`)."""
+    if stream is not None:
+        return _on(stream, matmul, codes, scales, w, out=out, dtype=dtype)
     _on_device(codes, scales, out, w.data)
     T, n = _quantized(codes, scales)
     _columns(w, n)
@@ -119,6 +129,8 @@ def moe_matmul(codes: torch.Tensor, scales: torch.Tensor, w: Packed, offsets: to
                out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """y[r] = W_e x[slot_of[r] / K] for the sorted rows r of each expert e (offsets, slot_of: moe.moe_sort); without slot_of W_e x[r]. Rows of `out`
     that no expert has are left as they were."""
+    if stream is not None:
+        return _on(stream, moe_matmul, codes, scales, w, offsets, slot_of=slot_of, K=K, out=out, dtype=dtype)
     _on_device(codes, scales, offsets, slot_of, out, w.data)
     T, n = _quantized(codes, scales)
     _columns(w, n)
@@ -144,6 +156,8 @@ def moe_layer(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_gate: Pac
     """The expert layer in MXFP4 (frx_mxfp4_moe_layer): out[t] = sum over k of wts[t][k] * expert_{ids[t][k]}(x[t]), [T][n] in `dtype` (that of
     `out`, or of x). Slots with a negative id take no part. `rows`: what the experts' rows are kept in before their sum; bfloat16 for a bfloat16
     output moves half the bytes and rounds twice."""
+    if stream is not None:
+        return _on(stream, moe_layer, x, ids, wts, w_gate, w_up, w_down, out=out, dtype=dtype, ws=ws, rows=rows)
     gate, E, ff, gate_n = w_gate
     up, down = w_up[0], w_down[0]
     _on_device(x, ids, wts, out, ws, gate, up, down)
