@@ -12,6 +12,7 @@
 // 61.7 instead of 65.4, since what is written next finds room in the L2.
 #include <algorithm>
 #include <initializer_list>
+#include <mutex>
 #include <type_traits>
 
 #include "frx_rows.cuh"
@@ -154,6 +155,7 @@ __global__ void __launch_bounds__(kChunkSlots) k_sort_place(const int32_t* __res
     row_of[s] = row;
 }
 constexpr int kOwnScan = 64;
+constexpr int kMaxExperts = 4096;
 inline size_t sort_place_smem(int E) { return size_t(kSortWarps) * warp_counts(E) + size_t(E) * 4; }
 
 // ---- rows out and back. A block per token; the token's K rows are looked up once, in shared memory.
@@ -370,7 +372,16 @@ size_t sort_scratch_bytes(long long S, int E) { return S <= kChunkSlots ? 0 : si
 int sort_slots(const int32_t* ids, int S, int E, int32_t* offsets, int32_t* slot_of, int32_t* row_of, int* status, int* scratch, cudaStream_t stream) {
     const int chunks = std::max(1, int((int64_t(S) + kChunkSlots - 1) / kChunkSlots));
     const bool scan = chunks > kOwnScan;
-    if (sort_place_smem(E) > 48 * 1024) FRX_CUDA(cudaFuncSetAttribute(k_sort_place, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sort_place_smem(E))));
+    if (sort_place_smem(E) > 48 * 1024) {
+        // The limit belongs to the kernel, not to a call: once per device, what the most experts need. (Calls of other threads may lie between this and the launch.)
+        static std::once_flag once[64];
+        int dev = 0;
+        FRX_CUDA(cudaGetDevice(&dev));
+        cudaError_t rc = cudaSuccess;
+        auto allow = [&] { rc = cudaFuncSetAttribute(k_sort_place, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sort_place_smem(kMaxExperts))); };
+        dev >= 0 && dev < 64 ? std::call_once(once[dev], allow) : allow();
+        FRX_CUDA(rc);
+    }
     if (chunks > 1)
         FRX_LAUNCH(kKGroup, stream, launch_pdl(k_sort_count, dim3(chunks), dim3(kChunkSlots), size_t(E) * 4, stream, ids, S, E, scratch, status));
     if (scan) FRX_LAUNCH(kKGroup, stream, launch_pdl(k_sort_scan, dim3((E + 31) / 32), dim3(32), 0, stream, scratch, chunks, E));
@@ -417,7 +428,7 @@ using namespace frx;
 extern "C" {
 
 size_t frx_moe_sort_workspace_bytes(int T, int K, int E) {
-    if (T < 0 || K < 1 || K > kMaxK || E < 1 || E > 4096 || (long long)T * K > 0x7fffffffLL) return 0;
+    if (T < 0 || K < 1 || K > kMaxK || E < 1 || E > kMaxExperts || (long long)T * K > 0x7fffffffLL) return 0;
     return kAlign + align_up(sort_scratch_bytes((long long)T * K, E));
 }
 

@@ -320,3 +320,33 @@ def test_refusals():
         with pytest.raises(moe.FrxError):
             call()
             raise AssertionError(f"call {i} was not refused")
+
+
+def test_sorts_of_several_threads_with_other_numbers_of_experts():
+    """Threads that sort for 1,400, 2,500 and 4,096 experts at once, whose kernels take different amounts of shared memory: no call is refused, all plans are right."""
+    import ctypes as C
+    import threading
+
+    from flashrt_b200.lib import lib
+    T, K = 50, 4
+    jobs = []
+    for E in (1400, 2500, 4096):
+        ids = make_ids(T, K, E, E)
+        jobs.append((E, ids, ids.cuda(), [torch.empty(m, dtype=torch.int32, device="cuda") for m in (E + 1, T * K, T * K)], torch.cuda.Stream(), []))
+    torch.cuda.synchronize()
+
+    def run(E, ids, on_device, outs, stream, codes):
+        ptr = [C.c_void_p(t.data_ptr()) for t in (on_device, *outs)]
+        for _ in range(4000):
+            codes.append(lib.frx_moe_sort(C.c_void_p(stream.cuda_stream), ptr[0], T, K, E, ptr[1], ptr[2], ptr[3], None, 0))
+
+    threads = [threading.Thread(target=run, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for E, ids, _, outs, _, codes in jobs:
+        assert set(codes) == {0}, (E, sum(c != 0 for c in codes))
+        for got, want in zip(outs, plan(ids, E)):
+            assert np.array_equal(got.cpu().numpy(), want.reshape(-1))
