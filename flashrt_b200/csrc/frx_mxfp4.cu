@@ -16,9 +16,10 @@ namespace frx {
 namespace {
 
 // ---- quantizer. A thread takes 16 values (two threads a block of 32), U times: per value 2 or 4 bytes in, 17 / 32 out, so bandwidth bounds it, and U
-// is how many loads a thread has in flight.
+// is how many loads a thread has in flight. (x is not __restrict__: the kernel in front may still write it when this one starts, so its loads must stay
+// behind pdl_wait().)
 template <class T, int U>
-__global__ void __launch_bounds__(256) k_mx_quantize(const T* __restrict__ x, int64_t ldx, uint32_t pieces, uint32_t per_row, uint2* __restrict__ codes,
+__global__ void __launch_bounds__(256) k_mx_quantize(const T* x, int64_t ldx, uint32_t pieces, uint32_t per_row, uint2* __restrict__ codes,
                                                      uint8_t* __restrict__ scales) {
     pdl_wait();
     pdl_trigger();
@@ -56,7 +57,7 @@ __global__ void __launch_bounds__(256) k_mx_quantize(const T* __restrict__ x, in
 }
 // rows that do not start on 16 bytes: a warp per block of 32, a lane per value
 template <class T>
-__global__ void __launch_bounds__(256) k_mx_quantize_any(const T* __restrict__ x, int64_t ldx, uint32_t blocks, uint32_t per_row, uint32_t* __restrict__ codes,
+__global__ void __launch_bounds__(256) k_mx_quantize_any(const T* x, int64_t ldx, uint32_t blocks, uint32_t per_row, uint32_t* __restrict__ codes,
                                                          uint8_t* __restrict__ scales) {
     pdl_wait();
     pdl_trigger();
@@ -76,7 +77,7 @@ __global__ void __launch_bounds__(256) k_mx_quantize_any(const T* __restrict__ x
 
 // eight values a thread, U times
 template <class T, int N, int U>
-__global__ void __launch_bounds__(256) k_mx_dequantize(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t pieces, uint32_t per_row, T* __restrict__ x,
+__global__ void __launch_bounds__(256) k_mx_dequantize(const uint32_t* codes, const uint8_t* scales, uint32_t pieces, uint32_t per_row, T* __restrict__ x,
                                                        int64_t ldx) {
     pdl_wait();
     pdl_trigger();

@@ -350,3 +350,46 @@ def test_sorts_of_several_threads_with_other_numbers_of_experts():
         assert set(codes) == {0}, (E, sum(c != 0 for c in codes))
         for got, want in zip(outs, plan(ids, E)):
             assert np.array_equal(got.cpu().numpy(), want.reshape(-1))
+
+
+def test_calls_on_values_that_the_call_in_front_rewrites_in_place():
+    """Chains of this library's own kernels, each of which lets the next one start early, over the same buffers with other values every time, without a wait: what every
+    call gives when the GPU is waited for in between."""
+    from flashrt_b200 import mxfp4
+    T, K, E, n, steps = 600, 6, 24, 1024, 12
+    S = T * K
+    g = gen(4)
+    codes = [torch.randint(0, 256, (S, n // 2), generator=g, dtype=torch.uint8).cuda() for _ in range(steps)]
+    scales = torch.full((S, n // 32), 125, dtype=torch.uint8).cuda()
+    logits = [torch.randn(T, E, generator=g).cuda() for _ in range(steps)]
+    buffers = [torch.zeros(S, n, device="cuda") for _ in range(4)]
+
+    def chain(wait):
+        x, ys, gys, out = buffers
+        results = []
+
+        def do(call, *args, **kwargs):
+            got = call(*args, **kwargs)
+            if wait:
+                torch.cuda.synchronize()
+            return got
+
+        for c, l in zip(codes, logits):
+            ids, wts = do(moe.moe_route_topk, l, K)
+            _, _, row_of = do(moe.moe_sort, ids, E)
+            do(mxfp4.dequantize, c, scales, out=x)
+            do(moe.moe_sort_rows, x[:T], row_of, out=ys)
+            do(moe.moe_unsort_rows, ys, wts, row_of, out=out[:T])
+            _, gw = do(moe.moe_unsort_rows_backward, out[:T], ys, wts, row_of, gys=gys)
+            do(moe.moe_sort_rows_backward, gys, row_of, out=out[T:2 * T])
+            gl = do(moe.moe_route_topk_backward, gw, wts, ids, E)
+            q = do(mxfp4.quantize, out[:2 * T])
+            results.append([t.clone() for t in (out[:2 * T], gys, gw, gl, *q)])
+        torch.cuda.synchronize()
+        return results
+
+    want = chain(True)
+    for _ in range(3):
+        for a, b in zip(chain(False), want):
+            for s, t in zip(a, b):
+                assert torch.equal(s, t)
