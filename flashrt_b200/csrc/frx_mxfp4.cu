@@ -362,7 +362,8 @@ __device__ __forceinline__ void swiglu8(const uint32_t (&g)[8], const uint32_t (
     uint32_t top[8], mine = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        // exp and the reciprocal to about 2^-22, like the sums that they are taken of
+        // The exponential's relative error is 2^-22 and |g| * 1.25 * 2^-24 of its rounded argument, which is what a sum g that is itself rounded to 32 bits
+        // leaves open; the reciprocal's is 2^-23 (2^-21 as a subnormal, below g = -87.3; 0 below -88.7).
         const float a = __uint_as_float(g[i]);
         float e, r;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * -1.44269504f));

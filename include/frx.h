@@ -591,8 +591,9 @@ int frx_mxfp4_moe_matmul(frx_stream_t stream, const void* codes, const void* sca
  * w_gate, w_up: E packed matrices [ff][n], w_down: E packed [n][ff]. x, out: rows of n elements of their dtype, ld* apart (out may be x). Slots with a negative id take
  * no part (a token without any gets zeros); an id of E or more is left out too and reported by frx_workspace_status. The experts' rows are kept in
  * float and out is rounded once, so that a token's row has the same bits whatever shares its batch; with FRX_BF16 | FRX_ROWS_BF16 as out_dtype they are
- * rounded to bfloat16 on their way to it (half the bytes, 1.41 times the error of out's own rounding). The hidden rows' codes are those of sums in 32 bits: where such a sum lies within its error of a border between
- * two codes, the code may be either. Any T; K <= 32, E <= 4096, n and ff multiples of 128 up to 2^20, T * K < 2^31. ws 16-byte aligned. */
+ * rounded to bfloat16 on their way to it (half the bytes, 1.41 times the error of out's own rounding). The hidden rows' codes are
+ * those of sums in 32 bits, and of silu(g) * u with a relative error of (16 + 1.25 |g|) * 2^-24 (0 where exp(-g) passes 32 bits): where such a value lies within its
+ * error of a border between two codes, the code may be either. Any T; K <= 32, E <= 4096, n and ff multiples of 128 up to 2^20, T * K < 2^31. ws 16-byte aligned. */
 size_t frx_mxfp4_moe_layer_workspace_bytes(int T, int K, int n, int ff, int E);
 int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_up, const void* w_down, int E, int n, int ff, const void* x, int64_t ldx,
                         int x_dtype, const int32_t* ids, const float* wts, int T, int K, void* out, int64_t ldo, int out_dtype, void* ws, size_t ws_bytes);

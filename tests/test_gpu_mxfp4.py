@@ -615,3 +615,52 @@ def test_tiles_behind_a_wait_that_ran_out_are_nan_too(dtype):
     assert bool(lost.any()), "no wait ran out"
     assert bool((lost | (y == want)).all())
     assert torch.equal(mxfp4.matmul(codes, scales, w, dtype=dtype), want)
+
+
+def test_hidden_codes_of_exact_sums():
+    """Gate and up sums of one and two terms, which 32 bits hold exactly, a down matrix that passes the hidden values on: what is left is the error of silu(g) * u,
+    and every code must be that of a value within its bound. The bound, in steps of 2^-24 of the value: the exponential is 2^fl(-g * fl(log2 e)), a product rounded by 2^-24
+    and a constant that is off by 2^-26, hence (1 + 0.25) |g|; 4 for ex2.approx (2^-22), 2 for rcp.approx (2^-23), one for each of the sum 1 + e and the two products: 9,
+    taken as 16. From g = -87.3 down the reciprocal is a subnormal (2^-21), from -88.7 on it is 0, as in a plain form of 32 bits."""
+    T, n, ff = 96, 128, 128
+    g = gen(9)
+    grid = GRID.float()
+
+    def matrix(rows, columns, at):
+        codes = torch.zeros(1, rows, columns, dtype=torch.uint8)
+        for c in at:
+            codes[0, :, c] = torch.randint(0, 16, (rows,), generator=g, dtype=torch.uint8)
+        scales = torch.full((1, rows, columns // 32), 127, dtype=torch.uint8)
+        packed = (codes[..., 0::2] | (codes[..., 1::2] << 4)).contiguous()
+        return values(packed, scales)[0], mxfp4.pack(packed.cuda(), scales.cuda())
+
+    wg, gate = matrix(ff, n, (0, 64))
+    wu, up = matrix(ff, n, (32,))
+    eye = torch.zeros(1, n, ff, dtype=torch.uint8)
+    eye[0, range(n), range(ff)] = 2                       # 1.0
+    down = mxfp4.pack((eye[..., 0::2] | (eye[..., 1::2] << 4)).contiguous().cuda(), torch.full((1, n, ff // 32), 127, dtype=torch.uint8).cuda())
+    x = torch.zeros(T, n)
+    x[:, 0] = grid[torch.randint(1, 8, (T,), generator=g)] * 2 * torch.where(torch.rand(T, generator=g) < 0.5, -1.0, 1.0)
+    x[:, 64] = grid[torch.randint(1, 8, (T,), generator=g)] * 0.5
+    x[:, 32] = grid[torch.randint(1, 8, (T,), generator=g)]
+    assert torch.equal(quantized(x)[2], x.double())
+    ids, wts = torch.zeros(T, 1, dtype=torch.int32).cuda(), torch.ones(T, 1).cuda()
+    got = mxfp4.moe_layer(x.cuda(), ids, wts, gate, up, down, dtype=torch.float32).cpu().double()
+    a, u = x.double() @ wg.t(), x.double() @ wu.t()
+    assert float(a.min()) < -80 and float(a.max()) > 80
+    h = a * torch.sigmoid(a) * u
+    eh = (16 + 1.25 * a.abs()) * 2.0 ** -24 * h.abs()
+    eh = torch.where(a < -87.3, 2.0 ** -20 * h.abs(), eh)
+    eh = torch.where(a < -88.7, h.abs(), eh)
+    blocks = lambda v: v.view(T, -1, 32)                                             # noqa: E731
+    fits, first, single = torch.zeros(T, ff, dtype=torch.bool), None, torch.ones(T, ff, dtype=torch.bool)
+    top, room = blocks(h.abs()), blocks(eh)
+    for big in ((top - room).clamp(min=0).amax(2), (top + room).amax(2)):
+        ex = scale_exponent(big).unsqueeze(2)
+        for v in (h - eh, h, h + eh):
+            one = (torch.ldexp(GRID[elements(blocks(v), ex)], ex) * torch.where(blocks(v) < 0, -1.0, 1.0)).view_as(h)
+            fits |= got == one
+            first = one if first is None else first
+            single &= one == first
+    assert bool(fits.all())
+    assert float(single.double().mean()) > 0.98          # (nearly every code is settled by the bound)
