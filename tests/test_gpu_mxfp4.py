@@ -664,3 +664,86 @@ def test_hidden_codes_of_exact_sums():
             single &= one == first
     assert bool(fits.all())
     assert float(single.double().mean()) > 0.98          # (nearly every code is settled by the bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,n,rows", [(300, 128, 6499), (300, 256, 6598), (450, 384, 6400), (1, 128, 19001), (120, 640, 12929)])
+def test_matmul_of_two_row_tiles_a_tile(T, n, rows, dtype):
+    """More row tiles than SMs, two a tile: odd and even numbers of them, the last one whole, partial, of odd and even rows."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert -(-rows // 128) * (T // 112 + 1) > sms
+    xq, wq = random_quantized((T, n), 1 + T), random_quantized((rows, n), 2 + rows)
+    if dtype == torch.float16:
+        wq[1].sub_(5)
+    w = mxfp4.pack(wq[0].cuda(), wq[1].cuda())
+    dx = [t.cuda() for t in xq]
+    got = mxfp4.matmul(*dx, w, dtype=dtype)
+    check_product(got, values(*xq), values(*wq), dtype)
+    for off, apart in ((1, 3), (2, 2), (0, 1)):           # rows that lie apart, by odd and even numbers, from odd and even starts: nothing beside them is written
+        wide = torch.full((T * (rows + apart) + off,), 77.0, dtype=dtype, device="cuda")
+        view = wide[off:].view(T, rows + apart)[:, :rows]
+        mxfp4.matmul(*dx, w, out=view)
+        assert torch.equal(view, got)
+        view.fill_(77.0)
+        assert bool((wide == 77).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,K,E,n,rows", [(200, 4, 40, 256, 1001), (700, 2, 9, 128, 1410), (50, 8, 300, 384, 130)])
+def test_moe_matmul_of_two_row_tiles_a_tile(T, K, E, n, rows, dtype):
+    """The same by expert: partial last row tiles beside whole ones, 16-bit rows of odd length, rows of y that no expert has."""
+    ids, _ = routed(T, K, E, T + E, 0.1, True)
+    xq, wq = random_quantized((T, n), 3), random_quantized((E, rows, n), 4)
+    if dtype == torch.float16:
+        wq[1].sub_(5)
+    offsets, slot_of, _ = moe.moe_sort(ids.cuda(), E)
+    y = torch.full((T * K, rows), 77.0, dtype=dtype, device="cuda")
+    mxfp4.moe_matmul(*(t.cuda() for t in xq), mxfp4.pack(wq[0].cuda(), wq[1].cuda()), offsets, slot_of, K, out=y)
+    x, W, at, slots = values(*xq), values(*wq), offsets.tolist(), slot_of.cpu().long()
+    for e in range(E):
+        if at[e + 1] > at[e]:
+            check_product(y[at[e]:at[e + 1]], x[slots[at[e]:at[e + 1]] // K], W[e], dtype)
+    assert at[-1] < T * K and bool((y[at[-1]:] == 77).all())
+
+
+def test_moe_matmul_ranges_that_overlap():
+    """More blocks of rows than any plan without overlaps has (12; 300 // 112 + 8 at most): nothing is computed."""
+    T, E, n, rows = 300, 8, 128, 128
+    xq, wq = random_quantized((T, n), 3), random_quantized((E, rows, n), 4)
+    y = torch.full((T, rows), 77.0, device="cuda")
+    offsets = torch.tensor([0, 300, 0, 300, 0, 300, 0, 300, 0], dtype=torch.int32).cuda()
+    mxfp4.moe_matmul(*(t.cuda() for t in xq), mxfp4.pack(wq[0].cuda(), wq[1].cuda()), offsets, out=y)
+    assert bool((y == 77).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,n", [(4032, 2080), (4033, 2080), (4099, 2080), (262145, 32), (131073, 96)])
+@pytest.mark.parametrize("layout", ["contiguous", "apart"])
+def test_quantize_many_values(T, n, dtype, layout):
+    """Around and beyond the 2^23 values from which a thread has several loads in flight, with a last block that is not full: what the rows give a few at a time, which
+    is tested above, and nothing written beside the results."""
+    from flashrt_b200.lib import check, lib
+    g = torch.Generator(device="cuda")
+    g.manual_seed(T + n)
+    x = (torch.randn(T, n, generator=g, device="cuda") * torch.exp2(torch.randint(-9, 9, (T, 1), generator=g, device="cuda").float())).to(dtype)
+    if layout == "apart":
+        wide = torch.full((T, n + 16), float("nan"), dtype=dtype, device="cuda")
+        wide[:, :n] = x
+        x = wide[:, :n]
+    pad = 4096
+    codes, scales = torch.full((T * n // 2 + pad,), 0x5a, dtype=torch.uint8, device="cuda"), torch.full((T * n // 32 + pad,), 0x5a, dtype=torch.uint8, device="cuda")
+    check(lib.frx_mxfp4_quantize(moe._stream(), moe._ptr(x), x.stride(0), mxfp4.DTYPES[dtype], T, n, moe._ptr(codes), moe._ptr(scales)))
+    assert bool((codes[-pad:] == 0x5a).all()) and bool((scales[-pad:] == 0x5a).all())
+    codes, scales = codes[:-pad].view(T, n // 2), scales[:-pad].view(T, n // 32)
+    few = max(1, (1 << 20) // n)                        # rows of a part: an eighth of the limit
+    parts = [mxfp4.quantize(x[a:a + few]) for a in range(0, T, few)]
+    assert torch.equal(codes, torch.cat([p[0] for p in parts])) and torch.equal(scales, torch.cat([p[1] for p in parts]))
+    check_quantized(x[-7:], codes[-7:], scales[-7:])    # the end, by the plain form too
+    if dtype == torch.float16:
+        return
+    flat = torch.full((T * (n + 16),), 77.0, dtype=dtype, device="cuda")
+    back = flat.view(T, n + 16)[:, :n] if layout == "apart" else flat[:T * n].view(T, n)
+    mxfp4.dequantize(codes, scales, out=back)
+    assert torch.equal(back, torch.cat([mxfp4.dequantize(*p, dtype=dtype) for p in parts]))
+    back.fill_(77.0)
+    assert bool((flat == 77).all())
