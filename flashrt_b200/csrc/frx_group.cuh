@@ -5,11 +5,11 @@
 // launch: what bounds them is their start and one or two round trips to memory each.
 #pragma once
 
-constexpr int kCookie = 0x46525831;   // marks a workspace whose status words have been initialised
+#include "frx_scan.cuh"
 
 // ---------------------------------------------------------------------------------------------
-// Slots are cut into chunks of 1024, these into parts of 128.
-constexpr int kChunkSlots = 1024, kPartSlots = 128, kParts = kChunkSlots / kPartSlots;
+// Slots are cut into chunks of kChunkSlots, these into parts of 128.
+constexpr int kPartSlots = 128, kParts = kChunkSlots / kPartSlots;
 
 // Expert parallel: with `e_map` (one entry per expert of the whole layer, E_all of them), ids name
 // experts of the whole layer, e_map[id] is the index of the expert among those held here or -1, and
@@ -58,28 +58,6 @@ __global__ void __launch_bounds__(256) k_pf_hist(const int32_t* __restrict__ ids
     }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += blockDim.x) chunk_cnt[size_t(blockIdx.x) * E + e] = hist[e];
-}
-
-// Sum of v over the threads in front of this one, and over all of them (`total`), for a block of 1024; tot: scratch.
-__device__ __forceinline__ int block_scan(int v, int* tot, int& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += u;
-    }
-    __syncthreads();   // (tot may still be read from the scan before)
-    if (lane == 31) tot[warp] = inc;
-    __syncthreads();
-    int w = tot[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += u;
-    }
-    total = __shfl_sync(0xffffffffu, w, 31);
-    return inc - v + (warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0);
 }
 
 // The token blocks of the tensor-memory form: every expert's slots cut into blocks of at most tok, as equal as multiples

@@ -2,8 +2,6 @@
 // element is E2M1: sign, 2 bits of exponent, 1 of mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6).
 #pragma once
 
-#include <cuda_fp4.h>
-
 #include "frx_common.cuh"
 
 namespace frx {

@@ -21,7 +21,7 @@
 namespace frx {
 namespace {
 
-#include "frx_group.cuh"
+#include "frx_scan.cuh"
 
 // Every kernel here may start while the one in front still writes what it reads. So nothing that is read is declared as data that no one writes (const
 // __restrict__, __ldg): such loads could be moved across pdl_wait(). With and without the declaration: 16,384 tokens of
