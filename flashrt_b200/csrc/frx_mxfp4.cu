@@ -144,10 +144,10 @@ __global__ void __launch_bounds__(kMxTileRows) k_mx_pack(uint4* __restrict__ cod
 // tile's products, and four sets of scales (16 columns each).
 //
 // What bounds it. Up to a few rows an expert: the weights. 64 tokens of ten experts out of 512 (2048 / 512; gate and up): 408 MB from DRAM in 61 us between
-// launches, 6.7 TB/s; 10 us of the layer's 108 are the start of the two products and their uneven ends. 4,096 tokens: 100 us for 570 MB of weights. 16,384 tokens
+// launches, 6.7 TB/s (reads alone; a copy reaches 6.55); 10 us of the layer's 110 are the start of the two products and their uneven ends. 4,096 tokens: 100 us for 570 MB of weights. 16,384 tokens
 // (three blocks of 107 rows an expert): 262 us for 687 GFLOP at full clocks, the thread that issues (a stage's hand-offs, six copies of scales and eight MMAs take
 // 900 clocks, of which the MMAs are 464) and the L2, which delivers 55 bytes a clock and SM without any MMA; in a stream of such layers the GPU is at its power
-// limit (1,000 W) and at 1,650 MHz.
+// limit (1,000 W) and at 1,650 MHz. The down product of these tokens writes 1.34 GB of rows in 32 bits: 333 us, 218 in bfloat16 (4,096 tokens 109 and 87).
 constexpr int kTok = 112;                 // y rows of a tile at most
 constexpr int kRowTiles = 2;              // row tiles of a tile
 constexpr int kStageUnits = 2;            // units of a stage
@@ -1002,7 +1002,7 @@ int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_u
     p.codes = base + b.xq;
     p.scales = base + b.xs;
     p.offsets = offsets;
-    p.slot_of = slot_of;   // (sorted copies of the rows instead, which the product reads 16 at a time: 16,384 tokens 219 instead of 248 us, but 24 more in
+    p.slot_of = slot_of;   // (sorted copies of the rows instead, which the product reads 16 at a time: 16,384 tokens 219 instead of 248 us where the two were compared, but 24 more in
     p.E = E;               // the quantizer; 4,096 tokens 113 instead of 103)
     p.rows = ff;
     p.n = n;

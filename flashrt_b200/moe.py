@@ -259,6 +259,7 @@ def quantize_q8(x: torch.Tensor, stream=None):
 
 
 # ---- tokens sorted by expert, and back -----------------------------------------------------------
+# The gradients are calls of their own: nothing here takes part in torch.autograd.
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # FRX_F32, FRX_BF16, FRX_F16
 
