@@ -86,7 +86,7 @@ def repack(ggml_rows: torch.Tensor, rows: int, cols: int, stream=None) -> torch.
 def tile_experts(planar: torch.Tensor, n: int, ff: int, n_experts: int, src_stride: int | None = None,
                  dst_stride: int | None = None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Planar expert blobs -> the tiled layout the kernels read."""
-    if stream is not None:
+    if stream is not None and out is None:
         return _on(stream, tile_experts, planar, n, ff, n_experts, src_stride=src_stride, dst_stride=dst_stride, out=out)
     _dev(planar, out)
     src_stride = expert_bytes(n, ff) if src_stride is None else src_stride
@@ -327,7 +327,7 @@ def moe_sort(ids: torch.Tensor, E: int, ws: torch.Tensor | None = None, stream=N
 
 def moe_sort_rows(x: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """xs[row_of[t][k]] = x[t]: x [T][n] float32, bfloat16 or float16 -> xs [T * K][n]. Rows that no slot has are left as they were."""
-    if stream is not None:
+    if stream is not None and out is None:
         return _on(stream, moe_sort_rows, x, row_of, out=out)
     _on_device(x, row_of, out)
     ldx = _matrix("x", x)
@@ -344,7 +344,7 @@ def moe_sort_rows(x: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | Non
 
 def moe_sort_rows_backward(gxs: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """gx[t] = sum over k of gxs[row_of[t][k]]: the gradient of moe_sort_rows."""
-    if stream is not None:
+    if stream is not None and out is None:
         return _on(stream, moe_sort_rows_backward, gxs, row_of, out=out)
     _on_device(gxs, row_of, out)
     ldg = _matrix("gxs", gxs)
@@ -361,7 +361,7 @@ def moe_sort_rows_backward(gxs: torch.Tensor, row_of: torch.Tensor, out: torch.T
 def moe_unsort_rows(ys: torch.Tensor, wts: torch.Tensor, row_of: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """out[t] = sum over k of wts[t][k] * ys[row_of[t][k]]: sorted rows back to their tokens, with the routing weights applied. A token
     none of whose slots has a row gets zeros."""
-    if stream is not None:
+    if stream is not None and out is None:
         return _on(stream, moe_unsort_rows, ys, wts, row_of, out=out)
     _on_device(ys, wts, row_of, out)
     ldy = _matrix("ys", ys)
@@ -449,7 +449,7 @@ def moe_decode(experts: int, stride: int, E: int, shared: int | None, n: int, ff
                yslot: torch.Tensor | None = None, ws: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """out[t] = sum_k w * expert(x_t) (+ shared(x_t) * sigmoid(gate_logit[t])). `experts` and
     `shared` are device addresses of tiled blobs (ExpertArena.blob)."""
-    if stream is not None:
+    if stream is not None and (out is None or ws is None):
         return _on(stream, moe_decode, experts, stride, E, shared, n, ff, x, ids, wts, gate_logit, out=out, yslot=yslot, ws=ws)
     _dev(x, ids, wts, gate_logit, out, yslot)
     T, K = ids.shape
@@ -478,7 +478,7 @@ def moe_layer(experts: int, stride: int, E: int, shared: int | None, n: int, ff:
               gate_logit: torch.Tensor | None, K: int, out: torch.Tensor | None = None, ids_out: torch.Tensor | None = None,
               wts_out: torch.Tensor | None = None, ws: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Router + experts + combine in one call (device tensors)."""
-    if stream is not None:
+    if stream is not None and (out is None or ws is None):
         return _on(stream, moe_layer, experts, stride, E, shared, n, ff, x, logits, gate_logit, K, out=out, ids_out=ids_out, wts_out=wts_out, ws=ws)
     _dev(x, logits, gate_logit, out, ids_out, wts_out)
     T = x.shape[0]
@@ -590,7 +590,7 @@ def moe_hits(hit_ptr: torch.Tensor, hit_n: torch.Tensor, K: int, x: torch.Tensor
              scratch: torch.Tensor | None = None, T: int = 1, stream=None) -> torch.Tensor:
     """qwen4exp::moe_hits: hit_ptr int64 [T][K] device addresses of tiled blobs, hit_n int32 [T];
     yh [T][K][n], rows k >= hit_n[t] are left untouched."""
-    if stream is not None:
+    if stream is not None and scratch is None:
         return _on(stream, moe_hits, hit_ptr, hit_n, K, x, n, ff, yh, scratch=scratch, T=T)
     _dev(hit_ptr, hit_n, x, yh, scratch)
     if scratch is None:
@@ -603,7 +603,7 @@ def moe_hits(hit_ptr: torch.Tensor, hit_n: torch.Tensor, K: int, x: torch.Tensor
 def moe_combine(yh: torch.Tensor, w: torch.Tensor, hit_n: torch.Tensor | None, shexp: torch.Tensor | None,
                 gate: torch.Tensor | None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """k_moe_combine: out[t] = sum_{k < hit_n[t]} w[t][k] * yh[t][k] + shexp[t] * sigmoid(gate[t])."""
-    if stream is not None:
+    if stream is not None and out is None:
         return _on(stream, moe_combine, yh, w, hit_n, shexp, gate, out=out)
     _dev(yh, w, hit_n, shexp, gate, out)
     T, K, n = yh.shape
@@ -625,7 +625,7 @@ class moe_q2:
             ws: torch.Tensor | None = None, stream=None, form: str = "auto") -> torch.Tensor:
         """yd[t*K + k] = down(silu(gate x_t) * up x_t) of expert ids[t][k], fp32 [T*K][n].
         form: "auto" (by size), "umma" (tcgen05 / tensor memory) or "stream"."""
-        if stream is not None:
+        if stream is not None and (yd is None or ws is None):
             return _on(stream, moe_q2.run, experts, stride, E, n, ff, x, ids, yd=yd, ws=ws, form=form)
         _dev(x, ids, yd)
         T, K = ids.shape
@@ -774,7 +774,7 @@ def convert_q8_0_to_q2_0(src: torch.Tensor, stream=None) -> torch.Tensor:
 
 def chain_rmsnorm_unit(x: torch.Tensor, y: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The layer join of the chained-stack benchmark: (x + y) / sqrt(mean((x + y)^2) + 1e-6) per row."""
-    if stream is not None:
+    if stream is not None and out is None:
         return _on(stream, chain_rmsnorm_unit, x, y, out=out)
     _dev(x, y, out)
     T, n = x.shape

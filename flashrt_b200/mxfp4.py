@@ -43,7 +43,7 @@ def _quantized(codes: torch.Tensor, scales: torch.Tensor):
 
 def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The values that codes and scales stand for, float32 or bfloat16 [T][n]."""
-    if stream is not None:
+    if stream is not None and out is None:
         return _on(stream, dequantize, codes, scales, dtype=dtype, out=out)
     _on_device(codes, scales, out)
     T, n = _quantized(codes, scales)
@@ -110,7 +110,7 @@ def _columns(w: Packed, n: int) -> None:
 
 def matmul(codes: torch.Tensor, scales: torch.Tensor, w: Packed, out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """y[t] = W x[t] of quantized rows x and one packed matrix: [T][rows] in `dtype` (or that of `out`)."""
-    if stream is not None:
+    if stream is not None and out is None:
         return _on(stream, matmul, codes, scales, w, out=out, dtype=dtype)
     _on_device(codes, scales, out, w.data)
     T, n = _quantized(codes, scales)
@@ -129,7 +129,7 @@ def moe_matmul(codes: torch.Tensor, scales: torch.Tensor, w: Packed, offsets: to
                out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """y[r] = W_e x[slot_of[r] / K] for the sorted rows r of each expert e (offsets, slot_of: moe.moe_sort); without slot_of W_e x[r]. Rows of `out`
     that no expert has are left as they were."""
-    if stream is not None:
+    if stream is not None and out is None:
         return _on(stream, moe_matmul, codes, scales, w, offsets, slot_of=slot_of, K=K, out=out, dtype=dtype)
     _on_device(codes, scales, offsets, slot_of, out, w.data)
     T, n = _quantized(codes, scales)
@@ -156,7 +156,7 @@ def moe_layer(x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_gate: Pac
     """The expert layer in MXFP4 (frx_mxfp4_moe_layer): out[t] = sum over k of wts[t][k] * expert_{ids[t][k]}(x[t]), [T][n] in `dtype` (that of
     `out`, or of x). Slots with a negative id take no part. `rows`: what the experts' rows are kept in before their sum; bfloat16 for a bfloat16
     output moves half the bytes and rounds twice."""
-    if stream is not None:
+    if stream is not None and (out is None or ws is None):
         return _on(stream, moe_layer, x, ids, wts, w_gate, w_up, w_down, out=out, dtype=dtype, ws=ws, rows=rows)
     gate, E, ff, gate_n = w_gate
     up, down = w_up[0], w_down[0]

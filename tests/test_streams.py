@@ -102,12 +102,30 @@ def test_every_argument_is_handed_on(trace, monkeypatch):
     for f in functions:
         if "stream" not in inspect.signature(f).parameters or "_on(stream" not in inspect.getsource(f):
             continue
-        handed.clear()
-        given = {p: object() for p in inspect.signature(f).parameters}
-        f(**given)
-        assert handed == {p: v for p, v in given.items() if p != "stream"}, f.__qualname__
-        checked += 1
+        made = [p for p in inspect.signature(f).parameters if p in ("out", "yd", "ws", "scratch")]
+        for absent in made or [None]:               # where the caller may give what a call would allocate: each of these left out
+            handed.clear()
+            given = {p: None if p == absent else object() for p in inspect.signature(f).parameters}
+            f(**given)
+            assert handed == {p: v for p, v in given.items() if p != "stream"}, f.__qualname__
+            checked += 1
     assert checked >= 30
+
+
+def test_a_call_that_allocates_nothing_stays_as_it_is(trace, monkeypatch):
+    """With results and workspace given there is nothing to allocate: the call does not change the current stream, which costs microseconds."""
+    seen, allocations = trace
+    monkeypatch.setattr(torch.cuda, "stream", lambda stream: pytest.fail("the current stream was changed"))
+    made = calls()
+    x, ids, wts, up, _, down = made["mxfp4.moe_layer"][1:]
+    ws, out, rows = torch.zeros(4096 + 256, dtype=torch.uint8), torch.zeros(600, 256), torch.zeros(1200, 256)
+    with allocations():
+        mxfp4.moe_layer(x, ids, wts, up, up, down, out=out, ws=ws, stream=Side())
+        moe.moe_sort_rows(x, ids, out=rows, stream=Side())
+        moe.moe_unsort_rows(rows, wts, ids, out=out, stream=Side())
+        moe.moe_decode(*made["moe_decode"][1:], out=out, ws=ws, stream=Side())
+        moe.moe_layer(*made["moe_layer"][1:], out=out, ws=ws, stream=Side())
+    assert not seen["allocated"] and seen["called"]
 
 
 @pytest.mark.gpu
