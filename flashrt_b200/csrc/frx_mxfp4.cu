@@ -1,12 +1,9 @@
 // MXFP4: the quantizer, the way back, the layout that the product reads, the product (dense, and grouped by expert), and
 // the expert layer made of them.
-#include <cuda.h>
-
 #include <algorithm>
-#include <atomic>
-#include <mutex>
 #include <type_traits>
 
+#include "frx_groups.cuh"
 #include "frx_mx.cuh"
 #include "frx_rows.cuh"
 #include "frx_sort.cuh"
@@ -168,7 +165,7 @@ constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, k
 static_assert(256 + 8 * kMxThreads / 32 <= 1024, "the scan's sums");
 constexpr int kSmemSegs = 1024, kSmemHead = kSmemSegs + kSegs * kSegBytes;   // the scale segments, then the stages
 
-enum { kYf32 = FRX_F32, kYbf16 = FRX_BF16, kYf16 = FRX_F16, kYswiglu = 3 };
+enum { kYswiglu = 3 };   // beside the element types of y
 
 struct MxProduct {
     const uint8_t* w[2];     // packed matrices; the second: the up matrices of the SwiGLU form
@@ -198,30 +195,6 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void tma_rows16(uint32_t dst, const CUtensorMap* map, int x, int row, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar) : "memory");
 }
-// A bounded wait of a whole warp: false, in all its lanes, when it, or another one of the block, ran out. The role then leaves its loop: what is
-// issued behind a wait that was given up could run the barriers' byte counts over.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t abort, uint64_t limit_ns) {
-    bool ok = mbar_try_wait(bar, parity);
-    if (!ok) {
-        uint64_t t0 = 0;
-        for (uint32_t polls = 1; !(ok = mbar_try_wait(bar, parity)); ++polls) {   // (a poll suspends the thread for microseconds by itself)
-            if (polls & 7u) continue;
-            if (lds32(abort)) break;
-            const uint64_t now = global_ns();
-            if (t0 == 0) {
-                t0 = now;
-            } else if (now - t0 > limit_ns) {
-                sts32(abort, 1u);
-                break;
-            }
-        }
-    }
-    return __all_sync(0xffffffffu, ok);
-}
-// umma_desc for rows of 128 bytes in the 128-byte swizzle (the 16-byte pieces of row r in the order piece ^ (r % 8)), groups of eight rows 1024 bytes
-// apart; a column offset is added to the address
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) { return umma_desc(smem_addr, 16, 1024) | (uint64_t(2) << 61); }
-
 // Instruction descriptor of kind::mxf4 with scales of 32: A and B E2M1 (1), scales UE8M0, both K-major, D fp32 128 x n; the byte pair of
 // the scale words that belongs to these 64 columns is part of it.
 __device__ __forceinline__ uint32_t mx_idesc(int n, int pair) {
@@ -251,52 +224,6 @@ __device__ __forceinline__ void tmem_ld8x2(uint32_t a0, uint32_t a1, uint32_t (&
         : "memory");
 }
 
-// The tiles of a block, one after the other: expert after expert, within one row pair after row pair, within these the blocks of y rows
-// (so that blocks that share weights run at the same time).
-struct MxTables {
-    int *tile_end, *first, *count, *blocks;   // per expert: tiles up to it, its first row, its rows, blocks of y rows | width << 24
-};
-struct MxWalk {
-    MxTables tab;
-    int E, tile, e;
-    int rp, row0, live, width;   // row pair, first y row, y rows, their number rounded up to 16
-    bool alone;                  // the expert has one block of y rows: this tile's weights are read by no other
-    __device__ __forceinline__ void begin(const MxTables& tables, int experts) {
-        tab = tables;
-        E = experts;
-        tile = int(blockIdx.x) - int(gridDim.x);
-        e = 0;
-    }
-    __device__ __forceinline__ bool next() {
-        tile += int(gridDim.x);
-        const int lane = threadIdx.x & 31;
-        // 32 experts at a time, those that end at or before the tile: from the last one on, then, if all of these do, over the whole list
-        // in 32 steps
-        unsigned done = __ballot_sync(0xffffffffu, e + lane < E && tab.tile_end[e + lane] <= tile);
-        e += __popc(done);
-        if (done == 0xffffffffu) {
-            const int step = (E + 31) >> 5, at = min(E, (lane + 1) * step);
-            e = max(e, __popc(__ballot_sync(0xffffffffu, tab.tile_end[at - 1] <= tile)) * step);
-            while (e < E) {
-                done = __ballot_sync(0xffffffffu, e + lane < E && tab.tile_end[e + lane] <= tile);
-                e += __popc(done);
-                if (done != 0xffffffffu) break;
-            }
-        }
-        if (e >= E) return false;
-        const int local = tile - (e ? tab.tile_end[e - 1] : 0), bw = tab.blocks[e], w = int(unsigned(bw) >> 24), blocks = bw & 0xffffff;
-        alone = blocks == 1;
-        rp = blocks == 1 ? local : int(unsigned(local) / unsigned(blocks));
-        const int b = local - rp * blocks;
-        row0 = tab.first[e] + b * w;
-        live = min(w, tab.count[e] - b * w);
-        width = (live + 15) & ~15;
-        // (the shuffles tell the compiler that the values are the same in all lanes)
-        width = __shfl_sync(0xffffffffu, width, 0);
-        return true;
-    }
-};
-
 // The scale words of units u .. u + 7 of a row (as far as there are so many). Of scattered rows every access costs one a row, whatever its width.
 __device__ __forceinline__ void load_words(uint32_t (&w)[8], const uint8_t* row, int u, int units, bool wide, bool on) {
     if (!on) return;
@@ -312,46 +239,6 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[8], const uint8_t* row,
         for (int j = 0; j < 8; ++j)
             if (u + j < units) w[j] = __ldcg(reinterpret_cast<const uint32_t*>(row + (u + j) * 4));
     }
-}
-
-// y of eight y rows for one matrix row a lane: y points at the matrix row's element of the first y row
-template <int MODE>
-__device__ __forceinline__ void store8(const uint32_t (&v)[8], void* y, int64_t ldy, int live, bool have, bool pairs) {
-    if (MODE == kYf32) {
-        float* p = static_cast<float*>(y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i, p += ldy)
-            if (i < live && have) *p = __uint_as_float(v[i]);
-        return;
-    }
-    const bool odd = threadIdx.x & 1;
-    if (pairs) {   // two lanes exchange a value so that each has two neighbouring matrix rows of one y row
-        uint16_t* p = static_cast<uint16_t*>(y) + (odd ? ldy - 1 : 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i, p += 2 * ldy) {
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? v[2 * i] : v[2 * i + 1], 1);
-            const float lo = __uint_as_float(odd ? got : v[2 * i]), hi = __uint_as_float(odd ? v[2 * i + 1] : got);
-            uint32_t w;
-            if (MODE == kYbf16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-                w = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-                const __half2 h = __floats2half2_rn(lo, hi);
-                w = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            if (2 * i + int(odd) < live && have) *reinterpret_cast<uint32_t*>(p) = w;
-        }
-        return;
-    }
-    uint16_t* p = static_cast<uint16_t*>(y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i, p += ldy)
-        if (i < live && have) {
-            if (MODE == kYbf16)
-                *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(__uint_as_float(v[i]));
-            else
-                *reinterpret_cast<__half*>(p) = __float2half_rn(__uint_as_float(v[i]));
-        }
 }
 
 // silu(g) * u of eight y rows for one hidden row a lane; the warp's 32 hidden rows are one block. codes: where this lane's word goes,
@@ -401,7 +288,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 244);
     long long* warp_sums = reinterpret_cast<long long*>(smem + 256);   // one a warp
     const uint32_t n_stages = uint32_t(p.stages);
-    MxTables tab;
+    GroupTables tab;
     tab.tile_end = reinterpret_cast<int*>(smem + kSmemHead + n_stages * kStageBytes);
     tab.first = tab.tile_end + p.E;
     tab.count = tab.first + p.E;
@@ -439,46 +326,13 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         pdl_wait();
         pdl_trigger();
     }
-    // tiles of every expert: a thread takes a few experts in a row
-    int experts = p.E;
-    {
-        const int per = (p.E + kMxThreads - 1) / kMxThreads, e0 = min(p.E, int(threadIdx.x) * per), e1 = min(p.E, e0 + per);
-        long long sum = 0;
-        for (int e = e0; e < e1; ++e) {
-            int a = 0, b = p.S;
-            if (p.offsets) {   // (what a plan says beyond the rows that there are is left out)
-                a = min(max(__ldcg(p.offsets + e), 0), p.S);
-                b = min(max(__ldcg(p.offsets + e + 1), a), p.S);
-            }
-            const int count = b - a, blocks = (count + kTok - 1) / kTok;
-            const int width = blocks ? ((count + blocks - 1) / blocks + 15) & ~15 : 0;   // as even as multiples of 16 allow
-            tab.first[e] = a;
-            tab.count[e] = count;
-            tab.blocks[e] = blocks | width << 24;
-            sum += (long long)blocks * row_pairs;
-            tab.tile_end[e] = int(sum);
-        }
-        long long inc = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += up;
-        }
-        if (lane == 31) warp_sums[warp] = inc;
-        __syncthreads();
-        long long before = inc - sum, total = 0;
-        for (int i = 0; i < kMxThreads / 32; ++i) {
-            before += i < warp ? warp_sums[i] : 0;
-            total += warp_sums[i];
-        }
-        for (int e = e0; e < e1; ++e) tab.tile_end[e] += int(before);
-        if (total > p.most) experts = 0;   // offsets that are not ascending: nothing is computed
-    }
+    // offsets that are not ascending: nothing is computed
+    const int experts = group_tables<kMxThreads>(tab, p.offsets, p.E, p.S, kTok, row_pairs, warp_sums) > p.most ? 0 : p.E;
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    MxWalk t;
+    GroupWalk t;
     t.begin(tab, experts);
 
     // "free" barriers are waited on with the parity of the phase before the one about to be used, which a fresh barrier reports as complete
@@ -655,7 +509,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
         constexpr int kParts = kWarpsEpi / 4;
         uint32_t set = 0, phase = 0;
         if (p.early) pdl_wait();
-        const bool pairs = MODE != kYf32 && p.rows % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
+        const bool pairs = MODE != FRX_F32 && p.rows % 2 == 0 && p.ldy % 2 == 0 && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
         // A wait ran out: NaN, not a wrong number, and no more waits. (Of the uses of a set of accumulators behind the lost one, every second would find the
         // parity of the last complete one, and take sums that nobody has finished.)
         bool lost = false;
@@ -689,7 +543,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
                         if (lane < 8) p.y_scales[y * (p.rows / kMxBlock) + at / kMxBlock] = uint8_t(scale);
                     }
                 } else {
-                    constexpr int size = MODE == kYf32 ? 4 : 2;
+                    constexpr int size = MODE == FRX_F32 ? 4 : 2;
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
                         const int row = (row_tile(t.rp) + m) * kMxTileRows + r;
@@ -722,21 +576,9 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx_product(const MxProduct p,
 
 // The codes [rows][n / 2] as a tensor map whose box is 128 bytes of one row (gathered) or of sixteen, in the 128-byte swizzle; what lies beyond the rows is zeros.
 int codes_tensor_map(CUtensorMap& map, const void* codes, int rows, int n, bool gathered) {
-    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static std::atomic<void*> entry{nullptr};   // the driver's function: looked up once
-    void* fn = entry.load(std::memory_order_acquire);
-    if (!fn) {
-        cudaDriverEntryPointQueryResult found;
-        FRX_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
-        if (found != cudaDriverEntryPointSuccess || !fn) return fail(FRX_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
-        entry.store(fn, std::memory_order_release);
-    }
     const cuuint64_t dims[2] = {cuuint64_t(n / 2), cuuint64_t(rows)}, strides[1] = {cuuint64_t(n / 2)};
-    const cuuint32_t box[2] = {cuuint32_t(kRowB), gathered ? 1u : 16u}, steps[2] = {1, 1};
-    const CUresult r = reinterpret_cast<Encode>(fn)(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? FRX_OK : fail(FRX_ERR_CUDA, "cuTensorMapEncodeTiled: error %d (%d rows of %d bytes)", int(r), rows, n / 2);
+    const cuuint32_t box[2] = {cuuint32_t(kRowB), gathered ? 1u : 16u};
+    return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box);
 }
 
 template <int MODE>
@@ -748,21 +590,13 @@ int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
     p.single = MODE != kYswiglu && row_tiles * blocks <= sm_count();
     const int64_t pairs = MODE == kYswiglu || p.single ? row_tiles : (row_tiles + 1) / 2;
     if ((int64_t(p.S) + kTok - 1) / kTok >= (1 << 24) || (int64_t(p.S) / kTok + p.E) * pairs > 0x7fff0000) return fail(FRX_ERR_SHAPE, "MXFP4 product: %d rows by %d is more than 2^31 tiles", p.S, p.rows);
-    constexpr size_t kSmem = 227 * 1024;
-    static std::mutex mu;
-    static bool done[64] = {};
-    {
-        int dev = 0;
-        FRX_CUDA(cudaGetDevice(&dev));
-        std::lock_guard<std::mutex> lk(mu);
-        if (dev < 0 || dev >= 64 || !done[dev]) FRX_CUDA(cudaFuncSetAttribute(k_mx_product<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
-        if (dev >= 0 && dev < 64) done[dev] = true;
-    }
-    p.stages = int(std::min<size_t>(kMaxStages, (kSmem - kSmemHead - tables) / kStageBytes));
-    static_assert((kSmem - kSmemHead - 4096 * 4 * 4) / kStageBytes >= 2, "stages beside the tables of 4096 experts");
+    int rc = allow_smem<k_mx_product<MODE>>();
+    if (rc != FRX_OK) return rc;
+    p.stages = int(std::min<size_t>(kMaxStages, (kSmemMost - kSmemHead - tables) / kStageBytes));
+    static_assert((kSmemMost - kSmemHead - 4096 * 4 * 4) / kStageBytes >= 2, "stages beside the tables of 4096 experts");
     p.wait_ns = wait_limit_ns();
     CUtensorMap map;
-    const int rc = codes_tensor_map(map, p.codes, p.x_rows, p.n, p.slot_of != nullptr);
+    rc = codes_tensor_map(map, p.codes, p.x_rows, p.n, p.slot_of != nullptr);
     if (rc != FRX_OK) return rc;
     const int64_t most = blocks * pairs;
     p.most = int(most);
@@ -773,9 +607,9 @@ int launch_mode(MxProduct& p, cudaStream_t stream, int cls) {
 }
 int launch_product(MxProduct& p, int mode, cudaStream_t stream, int cls) {
     switch (mode) {
-        case kYf32: return launch_mode<kYf32>(p, stream, cls);
-        case kYbf16: return launch_mode<kYbf16>(p, stream, cls);
-        case kYf16: return launch_mode<kYf16>(p, stream, cls);
+        case FRX_F32: return launch_mode<FRX_F32>(p, stream, cls);
+        case FRX_BF16: return launch_mode<FRX_BF16>(p, stream, cls);
+        case FRX_F16: return launch_mode<FRX_F16>(p, stream, cls);
         default: return launch_mode<kYswiglu>(p, stream, cls);
     }
 }
