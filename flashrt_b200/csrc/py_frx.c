@@ -49,6 +49,10 @@ BIND(moe_sort_rows, 11, frx_moe_sort_rows(S(0), P(1), v[2], I(3), P(4), I(5), I(
 BIND(moe_sort_rows_backward, 11, frx_moe_sort_rows_backward(S(0), P(1), v[2], v[3], I(4), P(5), I(6), I(7), I(8), P(9), v[10]))
 BIND(moe_unsort_rows, 12, frx_moe_unsort_rows(S(0), P(1), v[2], v[3], I(4), P(5), P(6), I(7), I(8), I(9), P(10), v[11]))
 BIND(moe_unsort_rows_backward, 15, frx_moe_unsort_rows_backward(S(0), P(1), v[2], P(3), v[4], v[5], I(6), P(7), P(8), I(9), I(10), I(11), P(12), v[13], P(14)))
+BIND(moe_matmul, 15, frx_moe_matmul(S(0), P(1), v[2], P(3), v[4], v[5], I(6), P(7), I(8), I(9), I(10), I(11), P(12), v[13], I(14)))
+BIND(moe_matmul_backward_x, 15, frx_moe_matmul_backward_x(S(0), P(1), v[2], P(3), v[4], v[5], I(6), P(7), I(8), I(9), I(10), I(11), P(12), v[13], I(14)))
+BIND(moe_matmul_backward_w, 16,
+     frx_moe_matmul_backward_w(S(0), P(1), v[2], P(3), v[4], I(5), P(6), I(7), I(8), I(9), I(10), P(11), v[12], v[13], I(14), I(15)))
 BIND(router_logits, 9, frx_router_logits(S(0), P(1), P(2), P(3), I(4), I(5), I(6), P(7), P(8)))
 BIND(quantize_q8, 6, frx_quantize_q8(S(0), P(1), I(2), I(3), P(4), P(5)))
 BIND(moe_decode, 17, frx_moe_decode(P(0), Z(1), I(2), P(3), I(4), I(5), P(6), P(7), P(8), P(9), I(10), I(11), P(12), P(13), P(14), Z(15), S(16)))
@@ -80,6 +84,9 @@ static PyMethodDef methods[] = {ENTRY(route_topk),
                                 ENTRY(moe_sort_rows_backward),
                                 ENTRY(moe_unsort_rows),
                                 ENTRY(moe_unsort_rows_backward),
+                                ENTRY(moe_matmul),
+                                ENTRY(moe_matmul_backward_x),
+                                ENTRY(moe_matmul_backward_w),
                                 ENTRY(router_logits),
                                 ENTRY(quantize_q8),
                                 ENTRY(moe_decode),

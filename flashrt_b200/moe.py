@@ -412,6 +412,95 @@ def moe_route_topk_backward(gwts: torch.Tensor, wts: torch.Tensor, ids: torch.Te
     return gl
 
 
+# ---- products with matrices of the experts, in 16 bits ---------------------------------------------
+# Between moe_sort_rows and moe_unsort_rows, for experts that a program trains or serves in 16 bits. The gradients are calls of their own here too.
+
+def _matrices(name: str, w: torch.Tensor, dtype=None, shape=None):
+    """E, rows, n of matrices whose rows are contiguous, and how many elements their rows and they themselves are apart."""
+    size = w.shape
+    if len(size) != 3 or w.dtype not in DTYPES or (dtype is not None and w.dtype != dtype) or (shape is not None and size != shape):
+        raise FrxError(_l.ERR_ARG, f"{name}: matrices [E][rows][n] of {'float32, bfloat16 or float16' if dtype is None else dtype}{'' if shape is None else f', {tuple(shape)},'} are wanted")
+    E, rows, n = size
+    if w.is_contiguous():
+        return E, rows, n, n, rows * n
+    lde, ldw, one = w.stride()
+    ldw = n if rows == 1 else ldw
+    lde = ldw * rows if E == 1 else lde
+    if (one == 1 or n == 1) and ldw >= n and lde >= (rows - 1) * ldw + n:
+        return E, rows, n, ldw, lde
+    raise FrxError(_l.ERR_ARG, f"{name}: the elements of a row must be contiguous, and neither rows nor matrices may overlap")
+
+
+def _half(name: str, t: torch.Tensor) -> int:
+    if t.dtype != torch.bfloat16 and t.dtype != torch.float16:
+        raise FrxError(_l.ERR_ARG, f"{name}: bfloat16 or float16 is wanted, not {t.dtype}")
+    return DTYPES[t.dtype]
+
+
+def moe_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor | None = None, dtype: torch.dtype | None = None, stream=None) -> torch.Tensor:
+    """y[r] = W_e x[r] for the sorted rows r of each expert e (offsets: moe_sort): x [S][n] and w [E][rows][n] bfloat16 or float16 -> [S][rows] in `dtype`
+    (that of `out`, or of x). Rows and matrices may lie apart, rows on 16-byte boundaries. Rows of `out` that no expert has are left as they were."""
+    if stream is not None and out is None:
+        return _on(stream, moe_matmul, x, w, offsets, out=out, dtype=dtype)
+    _on_device(x, w, offsets, out)
+    ldx, code = _matrix("x", x), _half("x", x)
+    E, rows, n, ldw, lde = _matrices("w", w, x.dtype)
+    S = x.shape[0]
+    if x.shape[1] != n:
+        raise FrxError(_l.ERR_ARG, f"matrices of {n} columns for rows of {x.shape[1]} values")
+    _typed("offsets", offsets, torch.int32, (E + 1,))
+    if out is None:
+        out, ldo = x.new_empty(S, rows, dtype=dtype or x.dtype), rows
+    else:
+        ldo = _matrix("out", out, dtype, (S, rows))
+    check(fast.moe_matmul(_raw_stream(stream), x.data_ptr(), ldx, w.data_ptr(), ldw, lde, code, offsets.data_ptr(), E, rows, n, S, out.data_ptr(), ldo, _code(out.dtype)))
+    return out
+
+
+def moe_matmul_backward_x(gy: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor | None = None, dtype: torch.dtype | None = None, stream=None) -> torch.Tensor:
+    """gx[r] = W_e^T gy[r], [S][n]: the gradient of moe_matmul for x from the gradient gy [S][rows] of its result. Types and layouts as there."""
+    if stream is not None and out is None:
+        return _on(stream, moe_matmul_backward_x, gy, w, offsets, out=out, dtype=dtype)
+    _on_device(gy, w, offsets, out)
+    ldgy, code = _matrix("gy", gy), _half("gy", gy)
+    E, rows, n, ldw, lde = _matrices("w", w, gy.dtype)
+    S = gy.shape[0]
+    if gy.shape[1] != rows:
+        raise FrxError(_l.ERR_ARG, f"matrices of {rows} rows for gradients of {gy.shape[1]} values")
+    _typed("offsets", offsets, torch.int32, (E + 1,))
+    if out is None:
+        out, ldo = gy.new_empty(S, n, dtype=dtype or gy.dtype), n
+    else:
+        ldo = _matrix("out", out, dtype, (S, n))
+    check(fast.moe_matmul_backward_x(_raw_stream(stream), gy.data_ptr(), ldgy, w.data_ptr(), ldw, lde, code, offsets.data_ptr(), E, rows, n, S, out.data_ptr(), ldo,
+                                     _code(out.dtype)))
+    return out
+
+
+def moe_matmul_backward_w(gy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor | None = None, dtype: torch.dtype | None = None, add: bool = False,
+                          stream=None) -> torch.Tensor:
+    """gW_e = the sum over the rows r of expert e of gy[r] x[r]^T, [E][rows][n]: the gradient of moe_matmul for w. Zeros for an expert without rows. With `add` it
+    is added to `out` (in 32 bits, rounded once), as a step of several batches needs it."""
+    if stream is not None and out is None:
+        return _on(stream, moe_matmul_backward_w, gy, x, offsets, out=out, dtype=dtype, add=add)
+    _on_device(gy, x, offsets, out)
+    ldgy, ldx, code = _matrix("gy", gy), _matrix("x", x, gy.dtype), _half("gy", gy)
+    (S, rows), n = gy.shape, x.shape[1]
+    if x.shape[0] != S:
+        raise FrxError(_l.ERR_ARG, f"{S} rows of gradients for {x.shape[0]} rows of x")
+    _typed("offsets", offsets, torch.int32)
+    E = offsets.numel() - 1
+    if out is None:
+        if add:
+            raise FrxError(_l.ERR_ARG, "moe_matmul_backward_w: nothing to add to: `out` is wanted")
+        out, ldo, lde = gy.new_empty(max(E, 0), rows, n, dtype=dtype or gy.dtype), n, rows * n
+    else:
+        _, _, _, ldo, lde = _matrices("out", out, dtype, (E, rows, n))
+    check(fast.moe_matmul_backward_w(_raw_stream(stream), gy.data_ptr(), ldgy, x.data_ptr(), ldx, code, offsets.data_ptr(), E, rows, n, S, out.data_ptr(), ldo, lde, _code(out.dtype),
+                                     int(add)))
+    return out
+
+
 # ---- the layer ---------------------------------------------------------------------------------
 
 def moe_decode_workspace_bytes(T: int, K: int, n: int, ff: int) -> int:

@@ -225,6 +225,25 @@ int frx_moe_unsort_rows(frx_stream_t stream, const void* ys, int64_t ldys, int64
 int frx_moe_unsort_rows_backward(frx_stream_t stream, const void* gout, int64_t ldg, const void* ys, int64_t ldys, int64_t rows, int dtype,
                                  const float* wts, const int32_t* row_of, int T, int K, int n, void* gys, int64_t ldgys, float* gwts);
 
+/* ---- products of sorted rows with matrices of their experts, in 16 bits, and their gradients (for experts that a program trains, or serves in 16 bits, between
+ * frx_moe_sort_rows and frx_moe_unsort_rows; the reference has no counterpart)
+ * The rows of expert e are offsets[e] .. offsets[e + 1] - 1 (frx_moe_sort) of S; w: E matrices of `rows` rows of n elements, rows ldw and matrices lde elements apart.
+ *   matmul:      y[r]  = W_e x[r]            x [S] rows of n, y [S] rows of `rows`
+ *   backward_x:  gx[r] = W_e^T gy[r]         gy [S] rows of `rows`, gx [S] rows of n
+ *   backward_w:  gW_e  = sum over the rows r of e of gy[r] x[r]^T: `rows` rows of n, ldgw apart, matrices ldge apart; zeros for an expert without
+ *                rows. With add it is added to what gw holds (and experts without rows are left as they were).
+ * dtype (FRX_BF16 or FRX_F16) is that of x, w and gy; out_dtype any. Products are exact, sums are formed in 32 bits on the tensor cores and rounded once. What is
+ * read (x, gy, w) begins every row on a 16-byte boundary: aligned bases and ld* multiples of 8 elements; n and `rows` are any (up to 2^20). What is written has any alignment of an
+ * element. Rows that no expert has (behind offsets[E]) are neither read into a sum nor written. offsets lie in [0, S] and ascend: what lies outside is left out, and offsets
+ * that descend may leave everything out. The same inputs give the same bits. Buffers do not overlap. E <= 4096. A device-side wait that runs out (2 s,
+ * frx_debug_set_wait_limit_ns) leaves NaN in the output; there is no workspace to report it in. */
+int frx_moe_matmul(frx_stream_t stream, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t lde, int dtype, const int32_t* offsets, int E, int rows, int n, int S,
+                   void* y, int64_t ldy, int out_dtype);
+int frx_moe_matmul_backward_x(frx_stream_t stream, const void* gy, int64_t ldgy, const void* w, int64_t ldw, int64_t lde, int dtype, const int32_t* offsets, int E, int rows, int n,
+                              int S, void* gx, int64_t ldgx, int out_dtype);
+int frx_moe_matmul_backward_w(frx_stream_t stream, const void* gy, int64_t ldgy, const void* x, int64_t ldx, int dtype, const int32_t* offsets, int E, int rows, int n, int S, void* gw,
+                              int64_t ldgw, int64_t ldge, int out_dtype, int add);
+
 /* ---- activation quantizer: q2_0::quantize_q8 (quant/q2_0/q2_0.cpp:101-117) ----
  * Per 32 values: d = amax / 127, q = roundf(x / d) (half away from zero), d stored after a
  * round trip through fp16. x [T][n]; q [T][n] int8; d [T][n/32] float. n % 32 == 0. */
