@@ -75,6 +75,10 @@ BIND(mxfp4_moe_matmul, 15,
      frx_mxfp4_moe_matmul(S(0), P(1), P(2), I(3), I(4), P(5), I(6), I(7), P(8), P(9), I(10), I(11), P(12), v[13], I(14)))
 BIND(mxfp4_moe_layer, 19,
      frx_mxfp4_moe_layer(S(0), P(1), P(2), P(3), I(4), I(5), I(6), P(7), v[8], I(9), P(10), P(11), I(12), I(13), P(14), v[15], I(16), P(17), Z(18)))
+BIND(mxint8_quantize, 8, frx_mxint8_quantize(S(0), P(1), v[2], I(3), I(4), I(5), P(6), P(7)))
+BIND(mxint8_dequantize, 8, frx_mxint8_dequantize(S(0), P(1), P(2), I(3), I(4), I(5), P(6), v[7]))
+BIND(mxint8_swiglu, 10, frx_mxint8_swiglu(S(0), P(1), v[2], I(3), I(4), I(5), P(6), P(7), P(8), v[9]))
+BIND(mxint8_swiglu_backward, 12, frx_mxint8_swiglu_backward(S(0), P(1), v[2], P(3), P(4), I(5), I(6), I(7), P(8), v[9], P(10), v[11]))
 
 #define ENTRY(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {ENTRY(route_topk),
@@ -107,6 +111,10 @@ static PyMethodDef methods[] = {ENTRY(route_topk),
                                 ENTRY(mxfp4_matmul),
                                 ENTRY(mxfp4_moe_matmul),
                                 ENTRY(mxfp4_moe_layer),
+                                ENTRY(mxint8_quantize),
+                                ENTRY(mxint8_dequantize),
+                                ENTRY(mxint8_swiglu),
+                                ENTRY(mxint8_swiglu_backward),
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_frxpy", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__frxpy(void) { return PyModule_Create(&module); }

@@ -151,6 +151,10 @@ SIGNATURES = {
     "frx_mxfp4_moe_matmul": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp, _i64, _i]),
     "frx_mxfp4_moe_layer_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "frx_mxfp4_moe_layer": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _i, _i, _vp, _i64, _i, _vp, _sz]),
+    "frx_mxint8_quantize": (_i, [_vp, _vp, _i64, _i, _i, _i, _vp, _vp]),
+    "frx_mxint8_dequantize": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _i64]),
+    "frx_mxint8_swiglu": (_i, [_vp, _vp, _i64, _i, _i, _i, _vp, _vp, _vp, _i64]),
+    "frx_mxint8_swiglu_backward": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _i64, _vp, _i64]),
     "frx_convert_q8_0_to_q2_0": (_i, [_vp, _vp, _sz, _vp]),
 }
 

@@ -617,6 +617,23 @@ size_t frx_mxfp4_moe_layer_workspace_bytes(int T, int K, int n, int ff, int E);
 int frx_mxfp4_moe_layer(frx_stream_t stream, const void* w_gate, const void* w_up, const void* w_down, int E, int n, int ff, const void* x, int64_t ldx,
                         int x_dtype, const int32_t* ids, const float* wts, int T, int K, void* out, int64_t ldo, int out_dtype, void* ws, size_t ws_bytes);
 
+/* ---- MXINT8: the OCP microscaling format of 8-bit integers, for activations that a backward pass needs again (8.25 bits a value; the reference has no counterpart).
+ * Blocks of 32 values along a row share a scale 2^e, held as the byte e + 127: e = floor(log2(largest magnitude)), at least -127. An element is the value / 2^(e - 6) to
+ * nearest, ties to even, at most 127 in magnitude: what is kept is off by at most 2^(e - 7) (by less than 2^(e - 6) where the magnitude passes 127 steps). A block with a NaN or an infinity in
+ * it has the scale byte 255 and codes 0: all its values are NaN. Codes [T][n] int8, 8-byte aligned, scales [T][n / 32]. Rows of dtype are ld* elements apart, with any alignment
+ * of an element (16-byte aligned rows are faster). n and ff multiples of 32. */
+int frx_mxint8_quantize(frx_stream_t stream, const void* x, int64_t ldx, int dtype, int T, int n, void* codes, void* scales);
+/* and the values that they stand for: exact in FRX_F32 and FRX_BF16, rounded where FRX_F16 does not hold them */
+int frx_mxint8_dequantize(frx_stream_t stream, const void* codes, const void* scales, int T, int n, int dtype, void* x, int64_t ldx);
+/* h = silu(g) * u of T rows [g | u], gu rows of 2 ff, h rows of ff, and the same rows in 8 bits: codes [T][2 ff], scales [T][2 ff / 32]; all in one pass. h is computed in 32 bits from gu as
+ * it is (not as it is kept) and rounded once: for FRX_F32 with the exponential and division of the library, else with a relative error of (16 + 1.25 |g|) * 2^-24
+ * in front of the rounding (0 where exp(-|g|) is below 2^-126). */
+int frx_mxint8_swiglu(frx_stream_t stream, const void* gu, int64_t ldgu, int dtype, int T, int ff, void* codes, void* scales, void* h, int64_t ldh);
+/* From gh, the gradient of h [T] rows of ff, and what was kept: the gradient of gu, rows of 2 ff, gh u s (1 + g (1 - s)) and gh g s with s = 1 / (1 + exp(-g)), and, where h is not null,
+ * h again, rows of ff: all of the values as they are kept. */
+int frx_mxint8_swiglu_backward(frx_stream_t stream, const void* gh, int64_t ldgh, const void* codes, const void* scales, int dtype, int T, int ff, void* ggu, int64_t ldggu, void* h,
+                               int64_t ldh);
+
 /* convert_q8_0_to_q2_0 (arch/qwen4exp/mtp.hpp:40, mtp.cu:129-215) on the device: nblocks64 pairs of
  * Q8_0 blocks {fp16 d; 32 int8} (68 bytes) -> ggml Q2_0 blocks (18 bytes): for each 64 values the
  * scale among 24 candidates (amax / 2.5 .. amax, through fp16) with the least squared error, codes
