@@ -161,6 +161,36 @@ __device__ __forceinline__ void store8(const uint32_t (&v)[8], void* y, int64_t 
         }
 }
 
+// ---- 16-bit operands
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+
+// A whole tile's step of 16 of depth, both operands in shared memory, issued by one thread
+__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 16 columns of this warp's lanes, complete on return
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[2][8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[0][4]), "=r"(v[0][5]), "=r"(v[0][6]), "=r"(v[0][7]), "=r"(v[1][0]), "=r"(v[1][1]),
+          "=r"(v[1][2]), "=r"(v[1][3]), "=r"(v[1][4]), "=r"(v[1][5]), "=r"(v[1][6]), "=r"(v[1][7])
+        : "r"(addr)
+        : "memory");
+}
+
 // ---- host side
 
 // A tensor map with the 128-byte swizzle (box[0] elements are 128 bytes) over rows of dims[0] elements; strides in bytes, of the dimensions from the second on. What
@@ -196,4 +226,34 @@ inline int allow_smem() {
     return FRX_OK;
 }
 
+// Instruction descriptor of kind::f16 without N: sums in 32 bits, both operands of one type (0 fp16, 1 bf16), `mn` bits where an operand is MN-major, 128 lanes
+inline uint32_t f16_idesc(int dtype, bool lanes_mn, bool cols_mn) {
+    const uint32_t type = dtype == FRX_BF16;
+    return (1u << 4) | type << 7 | type << 10 | uint32_t(lanes_mn) << 15 | uint32_t(cols_mn) << 16 | uint32_t(128 >> 4) << 24;
+}
+inline CUtensorMapDataType map_type(int dtype) { return dtype == FRX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
+
+// rows of n elements, `box` of them a load
+inline int rows_map(CUtensorMap& map, const void* x, int64_t ld, int dtype, int rows, int n, int box) {
+    const cuuint64_t dims[2] = {cuuint64_t(n), cuuint64_t(rows)}, strides[1] = {cuuint64_t(ld) * 2};
+    const cuuint32_t boxes[2] = {64, cuuint32_t(box)};
+    return encode_tensor_map(map, map_type(dtype), 2, x, dims, strides, boxes);
+}
+inline int matrices_map(CUtensorMap& map, const void* w, int64_t ldw, int64_t lde, int dtype, int E, int rows, int n, int box) {
+    const cuuint64_t dims[3] = {cuuint64_t(n), cuuint64_t(rows), cuuint64_t(E)}, strides[2] = {cuuint64_t(ldw) * 2, cuuint64_t(lde) * 2};
+    const cuuint32_t boxes[3] = {64, cuuint32_t(box), 1};
+    return encode_tensor_map(map, map_type(dtype), 3, w, dims, strides, boxes);
+}
+
+inline bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// What TMA reads of 16-bit elements: rows `ld` apart, at least n long, on 16-byte boundaries. One row alone has no distance to the next.
+inline int operand(const char* who, const char* what, const void* x, int64_t& ld, int64_t rows, int64_t n) {
+    if (!x) return fail(FRX_ERR_ARG, "%s: null pointer (%s)", who, what);
+    if (ld < n) return fail(FRX_ERR_ARG, "%s: rows of %s are %lld elements apart and %lld long", who, what, (long long)ld, (long long)n);
+    if (rows == 1) ld = (n + 7) / 8 * 8;
+    if (!aligned(x, 16) || ld % 8 || ld >= (int64_t(1) << 38))
+        return fail(FRX_ERR_ARG, "%s: rows of %s must begin on 16-byte boundaries (they are %lld elements apart)", who, what, (long long)ld);
+    return FRX_OK;
+}
 }  // namespace frx

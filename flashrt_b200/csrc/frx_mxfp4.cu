@@ -614,8 +614,6 @@ int launch_product(MxProduct& p, int mode, cudaStream_t stream, int cls) {
     }
 }
 
-bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
-
 // where the layer keeps what it forms, in its workspace
 struct LayerBuffers {
     size_t offsets, slot_of, row_of, sort, xq, xs, hq, hs, y, total;

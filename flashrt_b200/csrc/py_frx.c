@@ -53,6 +53,8 @@ BIND(moe_matmul, 15, frx_moe_matmul(S(0), P(1), v[2], P(3), v[4], v[5], I(6), P(
 BIND(moe_matmul_backward_x, 15, frx_moe_matmul_backward_x(S(0), P(1), v[2], P(3), v[4], v[5], I(6), P(7), I(8), I(9), I(10), I(11), P(12), v[13], I(14)))
 BIND(moe_matmul_backward_w, 16,
      frx_moe_matmul_backward_w(S(0), P(1), v[2], P(3), v[4], I(5), P(6), I(7), I(8), I(9), I(10), P(11), v[12], v[13], I(14), I(15)))
+BIND(adapter_add, 24,
+     frx_adapter_add(S(0), P(1), v[2], P(3), v[4], v[5], P(6), v[7], v[8], I(9), I(10), I(11), I(12), I(13), P(14), P(15), I(16), P(17), I(18), P(19), v[20], P(21), v[22], I(23)))
 BIND(router_logits, 9, frx_router_logits(S(0), P(1), P(2), P(3), I(4), I(5), I(6), P(7), P(8)))
 BIND(quantize_q8, 6, frx_quantize_q8(S(0), P(1), I(2), I(3), P(4), P(5)))
 BIND(moe_decode, 17, frx_moe_decode(P(0), Z(1), I(2), P(3), I(4), I(5), P(6), P(7), P(8), P(9), I(10), I(11), P(12), P(13), P(14), Z(15), S(16)))
@@ -91,6 +93,7 @@ static PyMethodDef methods[] = {ENTRY(route_topk),
                                 ENTRY(moe_matmul),
                                 ENTRY(moe_matmul_backward_x),
                                 ENTRY(moe_matmul_backward_w),
+                                ENTRY(adapter_add),
                                 ENTRY(router_logits),
                                 ENTRY(quantize_q8),
                                 ENTRY(moe_decode),

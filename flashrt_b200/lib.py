@@ -66,6 +66,7 @@ SIGNATURES = {
     "frx_moe_matmul": (_i, [_vp, _vp, _i64, _vp, _i64, _i64, _i, _vp, _i, _i, _i, _i, _vp, _i64, _i]),
     "frx_moe_matmul_backward_x": (_i, [_vp, _vp, _i64, _vp, _i64, _i64, _i, _vp, _i, _i, _i, _i, _vp, _i64, _i]),
     "frx_moe_matmul_backward_w": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _vp, _i, _i, _i, _i, _vp, _i64, _i64, _i, _i]),
+    "frx_adapter_add": (_i, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _i, _vp, _i64, _vp, _i64, _i]),
     "frx_quantize_q8": (_i, [_vp, _vp, _i, _i, _vp, _vp]),
     "frx_moe_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "frx_moe_decode_workspace_offset": (_sz, [_i, _i, _i, _i, C.c_char_p]),

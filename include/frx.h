@@ -244,6 +244,17 @@ int frx_moe_matmul_backward_x(frx_stream_t stream, const void* gy, int64_t ldgy,
 int frx_moe_matmul_backward_w(frx_stream_t stream, const void* gy, int64_t ldgy, const void* x, int64_t ldx, int dtype, const int32_t* offsets, int E, int rows, int n, int S, void* gw,
                               int64_t ldgw, int64_t ldge, int out_dtype, int add);
 
+/* ---- low-rank adapters of many requests beside a shared projection (whatever computes that: frx_mxfp4_matmul, frx_moe_matmul, a library; the reference has no counterpart)
+ *   out[t] = y[t] + scale[j] * B_j (A_j x[t])   for the tokens t = offsets[i] .. offsets[i + 1] - 1 of request i, j = which[i]
+ * and out[t] = y[t] for the tokens of a request whose which is negative (or L or more). y: what the projection gave; out may be y. x [T] rows of n; a: L matrices of `rank` rows of n
+ * elements, lda apart, matrices stride_a apart; b: L matrices of `rows` rows of `rank` elements, ldb and stride_b apart; scale [L], or null for 1; y, out [T] rows of `rows` elements of
+ * y_dtype. dtype (FRX_BF16 or FRX_F16) is that of x, a and b. Adapters of a smaller rank are filled up with zeros. Products are exact, both sums are formed in 32 bits on the tensor cores,
+ * A_j x is kept in 32 bits between them, and out is rounded once; where A_j x holds infinities out may be NaN. x, a and b begin every row on a 16-byte boundary (ld* multiples of 8); y
+ * and out have any alignment of an element. offsets [R + 1] lie in [0, T] and ascend: what lies outside is left out, and offsets that descend may leave out
+ * anything. Tokens of no request (behind offsets[R]) are left as they were. rank <= 128; n and rows up to 2^20. A device-side wait that runs out leaves NaN in out. */
+int frx_adapter_add(frx_stream_t stream, const void* x, int64_t ldx, const void* a, int64_t lda, int64_t stride_a, const void* b, int64_t ldb, int64_t stride_b, int dtype, int L, int rank,
+                    int n, int rows, const int32_t* offsets, const int32_t* which, int R, const float* scale, int T, const void* y, int64_t ldy, void* out, int64_t ldo, int y_dtype);
+
 /* ---- activation quantizer: q2_0::quantize_q8 (quant/q2_0/q2_0.cpp:101-117) ----
  * Per 32 values: d = amax / 127, q = roundf(x / d) (half away from zero), d stored after a
  * round trip through fp16. x [T][n]; q [T][n] int8; d [T][n/32] float. n % 32 == 0. */
