@@ -9,21 +9,26 @@ namespace {
 
 // out[t] = y[t] + scale_j B_j (A_j x[t]), j the adapter of t's request. What has to move is x, y and out, and each adapter once; the products are few. So one kernel does
 // both of them and v = A_j x never leaves the SM:
-//   first   v[t][k] = sum_c x[t][c] A_j[k][c]     up to 128 tokens of a request are the lanes, the rank is N
-//   second  d[m][t] = sum_k B_j[m][k] v[t][k]     128 rows of B_j are the lanes (contiguous in y), 64 tokens are N
+//   first   v[t][k] = sum_c x[t][c] A_j[k][c]     up to 64 tokens of a request are the lanes (of 128), the rank is N
+//   second  d[t][m] = sum_k v[t][k] B_j[m][k]     the tokens are the lanes, twice (so that all warps have some), 128 rows of B_j are N
 // v is kept in 32 bits: it goes into the second product as three 16-bit pieces whose sum it is (for float16, whose exponents do not reach, as multiples of a power of two of its token).
-// A tile (128 tokens of a request) is the work of a cluster of up to eight blocks, as many as fit the GPU at once: they share the first product's depth, add their
-// parts up through one another's shared memory (in the order of the blocks), and share the second product's rows. y is read ahead of the sums it is added to.
-constexpr int kTok = 128, kHalf = 64, kRows = 128, kDepth = 64;
-constexpr int kStages = 3, kBufs = 2;
+// A tile (64 tokens of a request) is the work of a cluster of up to eight blocks, as many as fit the GPU at once: they share the first product's depth, add their
+// parts up through one another's shared memory (in the order of the blocks), and share the second product's rows. y is read two steps (32 bits: one) ahead of the sums it is added
+// to, from before the first product on.
+constexpr int kTok = 64, kRows = 128, kDepth = 64;
+constexpr int kMaxStages = 6, kMinStages = 3, kBufs = 2;
 constexpr int kWarpsEpi = 8, kWarpLoad = 8, kWarpMma = 9, kThreads = 32 * 10;
-constexpr int kBarFull = 0, kBarFree = kBarFull + kStages, kBarBFull = kBarFree + kStages, kBarBFree = kBarBFull + kBufs, kBarDFull = kBarBFree + kBufs, kBarDFree = kBarDFull + 2,
+constexpr int kBarFull = 0, kBarFree = kBarFull + kMaxStages, kBarBFull = kBarFree + kMaxStages, kBarBFree = kBarBFull + kBufs, kBarDFull = kBarBFree + kBufs, kBarDFree = kBarDFull + 2,
               kBarV = kBarDFree + 2, kBarVIn = kBarV + 1, kBarPart = kBarVIn + 1, kBars = kBarPart + 1;
 constexpr int kAbort = 256, kSlot = 260, kFound = 264, kSums = 320, kTokScale = 512, kTokMax = kTokScale + 4 * kTok, kHead = 2048;
 static_assert(kBars * 8 <= kAbort && kSums + 8 * kThreads / 32 <= kTokScale && kTokMax + 8 * kTok <= kHead, "the block's head");
-constexpr int kPiece = kTok * 128;   // bytes of 64 of the rank of a piece of v, or of 128 rows of B_j
-constexpr int kColD = 128, kCols = 256;   // tensor memory: v's sums, then two sets of 64 columns; two blocks an SM
+constexpr int kPieceV = 2 * kTok * 128, kPieceB = kRows * 128;   // bytes of 64 of the rank: of a piece of v, of 128 rows of B_j
+constexpr int kCols = 256;   // tensor memory: two sets of 128 columns, the first of them also for v's sums; two blocks an SM
+constexpr int kSmemTwo = 228 * 512 - 1024;   // shared memory of a block of which an SM holds two
 
+// y and out move in accesses of 32 bytes a lane, four lanes 128 bytes of a row, where rows allow it (2.5 of 4 TB/s more than 64 bytes a lane, a row a lane). The sums come out of
+// tensor memory in the form of 16 lanes x 8 columns, in which a thread has columns 2 i, 2 i + 1 (i = lane % 4) of every eight: so the rows of B_j go into shared memory in the order that
+// makes these consecutive. Of G = 16 (32-bit y: 8) rows an access, column 8 k + 2 i + b of 4 G columns is row G i + 2 k + b: three dimensions of the tensor map.
 struct Adapters {
     const int32_t* offsets;   // [R + 1]
     const int32_t* which;     // [R]
@@ -33,8 +38,9 @@ struct Adapters {
     int64_t ldy, ldo;
     unsigned long long wait_ns;
     int T, R, L, n, rows, rank, rank16;   // rank16: the rank rounded up to 16
-    int box, stage_bytes, ring_bytes;     // rows of a load of x; bytes of a stage; of all of them (v's pieces come to the same place)
+    int box, stages, stage_bytes, ring_bytes;   // rows of a load of x; stages, bytes of one, of all of them (v's pieces come to the same place)
     uint32_t idesc;
+    int whole;                                  // y and out allow accesses of 32 bytes
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -71,6 +77,22 @@ __device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity,
         : "memory");
     return __all_sync(0xffffffffu, ok != 0);
 }
+__device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int u, int v, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v),
+                 "r"(bar)
+                 : "memory");
+}
+// 64 columns of 16 lanes (two rows of eight columns a lane and step: v[k][0], [1] of row lane / 4, [2], [3] of row lane / 4 + 8, columns 8 k + 2 (lane % 4) and the next), complete on return
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t addr, uint32_t (&v)[8][4]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[1][0]), "=r"(v[1][1]), "=r"(v[1][2]), "=r"(v[1][3]), "=r"(v[2][0]), "=r"(v[2][1]), "=r"(v[2][2]),
+          "=r"(v[2][3]), "=r"(v[3][0]), "=r"(v[3][1]), "=r"(v[3][2]), "=r"(v[3][3]), "=r"(v[4][0]), "=r"(v[4][1]), "=r"(v[4][2]), "=r"(v[4][3]), "=r"(v[5][0]), "=r"(v[5][1]),
+          "=r"(v[5][2]), "=r"(v[5][3]), "=r"(v[6][0]), "=r"(v[6][1]), "=r"(v[6][2]), "=r"(v[6][3]), "=r"(v[7][0]), "=r"(v[7][1]), "=r"(v[7][2]), "=r"(v[7][3])
+        : "r"(addr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_ld8(uint32_t addr, float (&v)[8]) {
     uint32_t u[8];
     asm volatile(
@@ -101,31 +123,18 @@ __device__ __forceinline__ uint32_t take_piece(float& f) {
     return bits;
 }
 
-// y's values of 16 columns (tokens) for this lane's row, read ahead of the sums they are added to. 16-bit elements of even rows apart come two rows a lane: of an even column
-// to even lanes, of an odd one to odd lanes, which is also how they are written.
-template <int TYPE>
-struct Ahead {
-    uint32_t w[16];
-    __device__ __forceinline__ void load(const void* y, int64_t ldy, int live, bool have, bool pairs) {
-        if (TYPE == FRX_F32) {
-            const float* p = static_cast<const float*>(y);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < live && have) w[i] = __float_as_uint(p[i * ldy]);
-        } else if (pairs) {
-            const int odd = threadIdx.x & 1;
-            const uint16_t* p = static_cast<const uint16_t*>(y) + (odd ? ldy - 1 : 0);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (2 * i + odd < live && have) w[i] = *reinterpret_cast<const uint32_t*>(p + 2 * i * ldy);
-        } else {
-            const uint16_t* p = static_cast<const uint16_t*>(y);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < live && have) w[i] = p[i * ldy];
-        }
-    }
-};
+// 32 bytes of y, of which nothing is waited for here (as a conditional assignment the load became a branch that was: one load after the other)
+__device__ __forceinline__ void load_if(uint32_t* w, const void* p, bool on) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.u32 q, %9, 0;\n\t"
+        "@q ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t}"
+        : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3]), "+r"(w[4]), "+r"(w[5]), "+r"(w[6]), "+r"(w[7])
+        : "l"(p), "r"(uint32_t(on)));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
 template <int TYPE>
 __device__ __forceinline__ float wide(uint32_t bits) {   // of the low half
     if (TYPE == FRX_BF16) return __uint_as_float(bits << 16);
@@ -140,29 +149,53 @@ __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// eight columns of sums added to what was read ahead, rounded once and written
+// 32 bytes of y with as many sums added, rounded once and written
 template <int TYPE>
-__device__ __forceinline__ void add_and_store8(const float (&v)[8], const Ahead<TYPE>& a, int h, void* out, int64_t ldo, int live, bool have, bool pairs) {
-    if (TYPE == FRX_F32) {
-        float* p = static_cast<float*>(out);
+__device__ __forceinline__ void add_and_store(const float* f, const uint32_t* y, void* out) {
+    uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < live && have) p[i * ldo] = v[i] + __uint_as_float(a.w[8 * h + i]);
-    } else if (pairs) {
-        const bool odd = threadIdx.x & 1;
-        uint16_t* p = static_cast<uint16_t*>(out) + (odd ? ldo - 1 : 0);
+    for (int i = 0; i < 8; ++i)
+        w[i] = TYPE == FRX_F32 ? __float_as_uint(f[i] + __uint_as_float(y[i])) : narrow2<TYPE>(f[2 * i] + wide<TYPE>(y[i]), f[2 * i + 1] + wide<TYPE>(y[i] >> 16));
+    store32(out, w);
+}
+// the same of 16 elements one by one, as far as there are so many
+template <int TYPE>
+__device__ __forceinline__ void add_and_store_each(const float (&f)[16], const void* y, void* out, int live) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[2 * i] : v[2 * i + 1], 1);
-            const float lo = odd ? got : v[2 * i], hi = odd ? v[2 * i + 1] : got;
-            const uint32_t old = a.w[4 * h + i];
-            if (2 * i + int(odd) < live && have) *reinterpret_cast<uint32_t*>(p + 2 * i * ldo) = narrow2<TYPE>(lo + wide<TYPE>(old), hi + wide<TYPE>(old >> 16));
+    for (int i = 0; i < 16; ++i)
+        if (i < live) {
+            if (TYPE == FRX_F32)
+                static_cast<float*>(out)[i] = f[i] + static_cast<const float*>(y)[i];
+            else
+                static_cast<uint16_t*>(out)[i] = uint16_t(narrow2<TYPE>(f[i] + wide<TYPE>(static_cast<const uint16_t*>(y)[i]), 0.0f));
         }
-    } else {
-        uint16_t* p = static_cast<uint16_t*>(out);
+}
+
+// rows t0 .. t0 + live - 1 of `size`-byte elements to another place, a row a warp: 16 bytes a lane where both sides allow it, eight accesses in flight
+template <class Access>
+__device__ __forceinline__ void copy_row(const Access* from, Access* to, int count) {
+    const int lane = threadIdx.x & 31;
+    for (int i = lane; i < count; i += 8 * 32) {
+        Access v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < live && have) p[i * ldo] = uint16_t(narrow2<TYPE>(v[i] + wide<TYPE>(a.w[8 * h + i]), 0.0f));
+        for (int k = 0; k < 8; ++k)
+            if (i + 32 * k < count) v[k] = from[i + 32 * k];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (i + 32 * k < count) to[i + 32 * k] = v[k];
+    }
+}
+template <int SIZE>
+__device__ __forceinline__ void copy_rows(const void* from, int64_t ld_from, void* to, int64_t ld_to, int t0, int live, int n, int warp, int warps) {
+    using Element = std::conditional_t<SIZE == 4, uint32_t, uint16_t>;
+    const bool wide = ((reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to) | uintptr_t(ld_from * SIZE) | uintptr_t(ld_to * SIZE) | uintptr_t(n * SIZE)) & 15) == 0;
+    for (int t = warp; t < live; t += warps) {
+        const Element* a = static_cast<const Element*>(from) + (t0 + t) * ld_from;
+        Element* b = static_cast<Element*>(to) + (t0 + t) * ld_to;
+        if (wide)
+            copy_row(reinterpret_cast<const uint4*>(a), reinterpret_cast<uint4*>(b), n * SIZE / 16);
+        else
+            copy_row(a, b, n);
     }
 }
 
@@ -173,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t s0 = smem_u32(smem), ring = s0 + kHead, bbuf = ring + uint32_t(p.ring_bytes), bars = s0, abort = s0 + kAbort;
     const int chunks = p.rank16 > 64 ? 2 : 1;   // of 64 of the rank
-    const uint32_t bbuf_bytes = uint32_t(chunks) * kPiece, part = bbuf + kBufs * bbuf_bytes;
+    const uint32_t bbuf_bytes = uint32_t(chunks) * kPieceB, v_bytes = uint32_t(chunks) * kPieceV, part = bbuf + kBufs * bbuf_bytes;
     const uint32_t rank = cluster_rank(), blocks = cluster_size();
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kAbort);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kSlot);
@@ -238,20 +271,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const int t0 = found[0], live = found[1], j = found[2];
     const bool work = live > 0 && j >= 0;
-    const int row_chunks = (p.rows + kRows - 1) / kRows, halves = (live + kHalf - 1) / kHalf;
+    const int row_chunks = (p.rows + kRows - 1) / kRows;
     const int depths = (p.n + kDepth - 1) / kDepth, d0 = int(int64_t(depths) * rank / blocks), d1 = int(int64_t(depths) * (rank + 1) / blocks);
+    const int turn = int((blockIdx.x / blocks) % unsigned(row_chunks));
+    auto chunk = [&](int c) { return c + turn < row_chunks ? c + turn : c + turn - row_chunks; };
     bool lost = false;
 
     if (!work) {
-        constexpr int size = TYPE == FRX_F32 ? 4 : 2;
-        using Element = std::conditional_t<size == 4, uint32_t, uint16_t>;
-        if (live > 0 && p.out != p.y) {   // no adapter: y as it is
-            for (int t = int(rank); t < live; t += int(blocks)) {
-                const Element* from = static_cast<const Element*>(p.y) + (t0 + t) * p.ldy;
-                Element* to = static_cast<Element*>(p.out) + (t0 + t) * p.ldo;
-                for (int i = threadIdx.x; i < p.rows; i += kThreads) to[i] = from[i];
-            }
-        }
+        // no adapter: y as it is
+        if (live > 0 && p.out != p.y) copy_rows<TYPE == FRX_F32 ? 4 : 2>(p.y, p.ldy, p.out, p.ldo, t0, live, p.rows, int(rank) * (kThreads / 32) + warp, int(blocks) * (kThreads / 32));
     } else if (warp == kWarpLoad) {
         // ---------------- loads: the first product's stages, and this block's rows of B_j as soon as there is room
         const int boxes = (live + p.box - 1) / p.box;
@@ -264,7 +292,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
             const uint32_t full = bars + (kBarBFull + buf) * 8, to = bbuf + buf * bbuf_bytes;
             if (lane == 0) {
                 mbar_expect_tx(full, bbuf_bytes);
-                for (int i = 0; i < chunks; ++i) tma_3d(to + i * kPiece, &b_map, i * 64, c * kRows, j, full);
+                for (int i = 0; i < chunks; ++i) {
+                    if (p.whole) {
+                        constexpr int kGroup = TYPE == FRX_F32 ? 8 : 16;
+                        for (int m = 0; m < kRows; m += 4 * kGroup) tma_5d(to + i * kPieceB + m * 128, &b_map, i * 64, 0, (chunk(c) * kRows + m) / kGroup, 0, j, full);
+                    } else {
+                        tma_3d(to + i * kPieceB, &b_map, i * 64, chunk(c) * kRows, j, full);
+                    }
+                }
             }
             __syncwarp();
             c += int(blocks);
@@ -279,8 +314,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                 tma_3d(a, &a_map, s * kDepth, 0, j, full);
             }
             __syncwarp();
-            if (++st == kStages) st = 0, phase ^= 1u;
-            if (s - d0 == kStages - 1)
+            if (++st == uint32_t(p.stages)) st = 0, phase ^= 1u;
+            if (s - d0 == p.stages - 1)
                 for (int i = 0; i < kBufs && c < row_chunks && ok; ++i) rows_of_b();
         }
         while (c < row_chunks && ok) rows_of_b();
@@ -303,35 +338,51 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                 if (s + 1 == d1) umma_commit(bars + kBarV * 8);
             }
             __syncwarp();
-            if (++st == kStages) st = 0, phase ^= 1u;
+            if (++st == uint32_t(p.stages)) st = 0, phase ^= 1u;
         }
         ok = ok && warp_wait(bars + kBarVIn * 8, 0, abort, p.wait_ns);
         uint32_t buf = 0, bphase = 0, set = 0, dphase = 1;
+        const uint32_t id = p.idesc | uint32_t(kRows >> 3) << 17;
         for (int c = int(rank); c < row_chunks && ok; c += int(blocks)) {
             if (!(ok = warp_wait(bars + (kBarBFull + buf) * 8, bphase, abort, p.wait_ns))) break;
-            for (int h = 0; h < halves; ++h) {
-                if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
-                tc_fence_after_sync();
-                const uint32_t width = uint32_t((min(kHalf, live - h * kHalf) + 15) & ~15), id = p.idesc | (width >> 3) << 17;
-                if (elect_one()) {
-                    for (int q = 0; q < 3; ++q)
-                        for (int k = 0; k < p.rank16; k += 16) {
-                            const uint32_t at = uint32_t(k >> 6) * kPiece, in = uint32_t(k & 63) * 2;
-                            umma_f16(tmem + kColD + set * kHalf, umma_desc_sw128(bbuf + buf * bbuf_bytes + at) + (in >> 4),
-                                     umma_desc_sw128(ring + q * bbuf_bytes + at + h * kHalf * 128) + (in >> 4), id, q + k > 0);
-                        }
-                    if (h + 1 == halves) umma_commit(bars + (kBarBFree + buf) * 8);
-                    umma_commit(bars + (kBarDFull + set) * 8);
-                }
-                __syncwarp();
-                set ^= 1u;
-                if (set == 0) dphase ^= 1u;
+            if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
+            tc_fence_after_sync();
+            if (elect_one()) {
+                for (int q = 0; q < 3; ++q)
+                    for (int k = 0; k < p.rank16; k += 16) {
+                        const uint32_t in = uint32_t(k & 63) * 2;
+                        umma_f16(tmem + set * kRows, umma_desc_sw128(ring + q * v_bytes + uint32_t(k >> 6) * kPieceV) + (in >> 4),
+                                 umma_desc_sw128(bbuf + buf * bbuf_bytes + uint32_t(k >> 6) * kPieceB) + (in >> 4), id, q + k > 0);
+                    }
+                umma_commit(bars + (kBarBFree + buf) * 8);
+                umma_commit(bars + (kBarDFull + set) * 8);
             }
+            __syncwarp();
+            set ^= 1u;
+            if (set == 0) dphase ^= 1u;
             if (++buf == kBufs) buf = 0, bphase ^= 1u;
         }
     } else {
         const int quarter = warp & 3, side = warp >> 2, token = quarter * 32 + lane;
         const uint32_t lanes = uint32_t(quarter * 32) << 16;
+        // In the second product a warp has 16 of the tokens (of which there are two of 64 lanes) and 64 of the 128 columns, a lane two of these tokens, eight apart, and 16 columns
+        // of each; where y and out do not allow that, a lane is a token and a warp has 32 of them and 32 columns.
+        constexpr int size = TYPE == FRX_F32 ? 4 : 2, kAhead = TYPE == FRX_F32 ? 1 : 2, kPer = 32 / size, kAccesses = 16 / kPer;   // values of an access, accesses of 16 values
+        const int t = p.whole ? (quarter & 1) * 32 + side * 16 + lane / 4 : (quarter & 1) * 32 + lane;
+        const int col = p.whole ? (quarter >> 1) * 64 + (lane & 3) * kPer : (quarter >> 1) * 64 + side * 32;
+        const uint8_t* y = static_cast<const uint8_t*>(p.y) + ((t0 + t) * p.ldy + col) * size;
+        uint8_t* out = static_cast<uint8_t*>(p.out) + ((t0 + t) * p.ldo + col) * size;
+        uint32_t old[kAhead][2][8 * kAccesses] = {};
+        auto read_ahead = [&](uint32_t (&w)[2][8 * kAccesses], int c) {
+            if (c >= row_chunks || !p.whole) return;
+            const int first = chunk(c) * kRows;
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int q = 0; q < kAccesses; ++q) load_if(w[r] + 8 * q, y + (8 * r * p.ldy + first + 4 * q * kPer) * size, t + 8 * r < live && first + col + 4 * q * kPer < p.rows);
+        };
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) read_ahead(old[d], int(rank) + d * int(blocks));
         // ---------------- v: a lane is a token, a warp has half of the rank
         const int half = p.rank16 / 2, k0 = side * half;
         const bool empty = d0 == d1;   // no part of the depth here
@@ -339,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
             lost = !warp_wait(bars + kBarV * 8, 0, abort, p.wait_ns);
             tc_fence_after_sync();
         }
-        const uint32_t mine = part + uint32_t(token * p.rank16) * 4;
+        const uint32_t mine = part + uint32_t(token * (p.rank16 + 4)) * 4;   // (rows 16 bytes off a multiple of the banks)
         if (blocks > 1) {
             for (int k = k0; k < k0 + half; k += 8) {
                 float v[8];
@@ -383,14 +434,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
 #pragma unroll
                 for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i] * scale));
             }
-            tok_max[side * kTok + token] = most;
+            if (token < kTok) tok_max[side * kTok + token] = most;
             named_bar_sync(1, 32 * kWarpsEpi);
-            most = fmaxf(tok_max[token], tok_max[kTok + token]);
+            if (token < kTok) most = fmaxf(tok_max[token], tok_max[kTok + token]);
             const uint32_t e = __float_as_uint(most) >> 23;   // its exponent + 127
             // 2^(141 - e) and back, within what 32 bits hold; nothing for zeros, infinities and NaN
             const uint32_t f = e == 255u || most == 0.0f ? 127u : min(max(268u - e, 1u), 253u);
             up = __uint_as_float(f << 23);
-            if (side == 0) tok_scale[token] = __uint_as_float((254u - f) << 23);
+            if (side == 0 && token < kTok) tok_scale[token] = __uint_as_float((254u - f) << 23);
         }
         for (int k = k0; k < k0 + half; k += 8) {
             float v[8];
@@ -405,46 +456,66 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                     bits[q][i / 2] = i & 1 ? bits[q][i / 2] | b << 16 : b;
                 }
             }
-            const uint32_t at = ring + uint32_t(k >> 6) * kPiece + uint32_t(token) * 128 + uint32_t(((k & 63) >> 3) ^ (token & 7)) * 16;   // (the 128-byte swizzle)
+            const uint32_t at = ring + uint32_t(k >> 6) * kPieceV + uint32_t(token) * 128 + uint32_t(((k & 63) >> 3) ^ (token & 7)) * 16;   // (the 128-byte swizzle)
 #pragma unroll
-            for (int q = 0; q < 3; ++q)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + q * bbuf_bytes), "r"(bits[q][0]), "r"(bits[q][1]), "r"(bits[q][2]), "r"(bits[q][3]) : "memory");
+            for (int q = 0; q < 6 && token < kTok; ++q)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (q % 3) * v_bytes + (q / 3) * kTok * 128), "r"(bits[q % 3][0]), "r"(bits[q % 3][1]), "r"(bits[q % 3][2]),
+                             "r"(bits[q % 3][3])
+                             : "memory");
         }
         fence_async_smem();   // generic-proxy writes: visible to the tensor core
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kBarVIn * 8);
-        if (XTYPE == FRX_F16) named_bar_sync(1, 32 * kWarpsEpi);   // tok_scale is there
-        // ---------------- the second product's sums: a lane is a row of y, a warp has 32 of 64 tokens
-        constexpr int size = TYPE == FRX_F32 ? 4 : 2;
-        const bool pairs = TYPE != FRX_F32 && p.rows % 2 == 0 && p.ldy % 2 == 0 && p.ldo % 2 == 0 && (reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.out)) % 4 == 0;
+        float down = 1.0f, down8 = 1.0f;   // of the lane's tokens
+        if (XTYPE == FRX_F16) {
+            named_bar_sync(1, 32 * kWarpsEpi);
+            down = tok_scale[t];
+            down8 = tok_scale[min(t + 8, kTok - 1)];
+        }
+        // ---------------- the second product's sums
         uint32_t set = 0, phase = 0;
-        for (int c = int(rank); c < row_chunks; c += int(blocks)) {
-            const int row = c * kRows + quarter * 32 + lane;
-            const bool have = row < p.rows;
-            for (int h = 0; h < halves; ++h) {
-                const int tok = h * kHalf + side * 32, count = live - tok;   // the warp's first token, and tokens from it on
-                const uint8_t* y = static_cast<const uint8_t*>(p.y) + ((t0 + tok) * p.ldy + row) * size;
-                uint8_t* out = static_cast<uint8_t*>(p.out) + ((t0 + tok) * p.ldo + row) * size;
-                Ahead<TYPE> old[2];
+        for (int c0 = int(rank); c0 < row_chunks; c0 += kAhead * int(blocks)) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) old[q].load(y + q * 16 * p.ldy * size, p.ldy, count - q * 16, have, pairs);
+            for (int d = 0; d < kAhead; ++d) {
+                const int c = c0 + d * int(blocks);
+                if (c >= row_chunks) continue;
+                const int first = chunk(c) * kRows;
                 lost = !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns) || lost;
                 tc_fence_after_sync();
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float v[8];
-                    if (q * 8 >= count) break;
+                const uint32_t sums = tmem + lanes + set * kRows;
+                if (p.whole) {
+                    uint32_t v[8][4];
                     if (lost) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fffffffu);
+                        for (int i = 0; i < 32; ++i) v[i / 4][i % 4] = 0x7fffffffu;
                     } else {
-                        tmem_ld8(tmem + lanes + kColD + set * kHalf + side * 32 + q * 8, v);
+                        tmem_ld_16x256(sums + (uint32_t(side * 16) << 16) + (quarter >> 1) * 64, v);
                     }
-                    if (XTYPE == FRX_F16) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] *= tok_scale[tok + q * 8 + i];
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int q = 0; q < kAccesses; ++q) {
+                            float f[kPer];
+#pragma unroll
+                            for (int i = 0; i < kPer; ++i) f[i] = __uint_as_float(v[q * kPer / 2 + i / 2][2 * r + i % 2]) * (r ? down8 : down);   // (exact; by 1 for bfloat16)
+                            if (t + 8 * r < live && first + col + 4 * q * kPer < p.rows)
+                                add_and_store<TYPE>(f, old[d][r] + 8 * q, out + (8 * r * p.ldo + first + 4 * q * kPer) * size);
+                        }
+                    read_ahead(old[d], c + kAhead * int(blocks));
+                } else {
+                    for (int h = 0; h < 32; h += 16) {
+                        uint32_t v[2][8];
+                        float f[16];
+                        if (lost) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = 0x7fffffffu;
+                        } else {
+                            tmem_ld16(sums + col + h, v);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i / 8][i % 8]) * down;
+                        if (t < live) add_and_store_each<TYPE>(f, y + (first + h) * size, out + (first + h) * size, p.rows - first - col - h);
                     }
-                    add_and_store8<TYPE>(v, old[q / 2], q & 1, out + q * 8 * p.ldo * size, p.ldo, count - q * 8, have, pairs);
                 }
                 tc_fence_before_sync();
                 __syncwarp();
@@ -468,21 +539,33 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
     if (blocks > 1) cluster_sync_all();   // the others have read what they needed of this block's shared memory
 }
 
+// b for the second product: 128 rows a load, or, with a group, four groups of so many rows, in the order in which a thread finds its columns side by side
+int second_map(CUtensorMap& map, const void* b, int64_t ldb, int64_t stride_b, int dtype, int L, int rows, int rank, int group) {
+    if (!group) return matrices_map(map, b, ldb, stride_b, dtype, L, rows, rank, kRows);
+    const cuuint64_t dims[5] = {cuuint64_t(rank), 2, cuuint64_t(rows / group), cuuint64_t(group / 2), cuuint64_t(L)};
+    const cuuint64_t strides[4] = {cuuint64_t(ldb) * 2, cuuint64_t(ldb) * 2 * group, cuuint64_t(ldb) * 4, cuuint64_t(stride_b) * 2};
+    const cuuint32_t boxes[5] = {64, 2, 4, cuuint32_t(group / 2), 1};
+    return encode_tensor_map(map, map_type(dtype), 5, b, dims, strides, boxes);
+}
+
 template <int XTYPE, int TYPE>
 int launch_typed(Adapters& p, const CUtensorMap& x_map, const CUtensorMap& a_map, const CUtensorMap& b_map, cudaStream_t stream) {
     int rc = allow_smem<k_adapter<XTYPE, TYPE>>();
     if (rc != FRX_OK) return rc;
     const int chunks = p.rank16 > 64 ? 2 : 1;
-    const int64_t tiles = int64_t(p.T) / kTok + std::min(p.R, p.T);   // of any requests that do not overlap
-    // as many blocks a tile as run at the same time (two an SM, one where the rank is more than 64)
+    const int64_t requests = std::min(p.R, p.T), tiles = (p.T - requests) / kTok + requests;   // of any requests that do not overlap
+    // As many blocks a tile as run at the same time (two an SM, one where the rank is more than 64), and as many stages as that leaves room for.
     unsigned blocks = 8;
     while (blocks > 1 && tiles * blocks > int64_t(sm_count()) * (chunks == 1 ? 2 : 1)) blocks /= 2;
     if (tiles * blocks > 0x7fff0000) return fail(FRX_ERR_SHAPE, "adapters: %lld tiles", (long long)tiles);
     p.stage_bytes = kTok * 128 + p.rank16 * 128;
-    p.ring_bytes = std::max(kStages * p.stage_bytes, 3 * chunks * kPiece);
-    const size_t smem = size_t(kHead) + p.ring_bytes + kBufs * chunks * kPiece + (blocks > 1 ? size_t(kTok) * p.rank16 * 4 : 0);
-    static_assert(kHead + 3 * 2 * kPiece + kBufs * 2 * kPiece + kTok * 128 * 4 <= kSmemMost, "the largest rank");
-    static_assert(3 * (kHead + kStages * (kTok + 16) * 128 + kBufs * kPiece) > 228 * 1024, "no third block an SM, which would wait for tensor memory");
+    const int rest = kHead + kBufs * chunks * kPieceB + (blocks > 1 ? kTok * (p.rank16 + 4) * 4 : 0);
+    static_assert(kHead + kBufs * kPieceB + kTok * 68 * 4 + std::max(kMinStages * (kTok + 64) * 128, 3 * kPieceV) <= kSmemTwo, "two blocks an SM up to a rank of 64");
+    static_assert(kHead + kBufs * 2 * kPieceB + kTok * 132 * 4 + std::max(kMinStages * (kTok + 128) * 128, 3 * 2 * kPieceV) <= int(kSmemMost), "the largest rank");
+    p.stages = std::min(kMaxStages, ((chunks == 1 ? kSmemTwo : int(kSmemMost)) - rest) / p.stage_bytes);
+    p.ring_bytes = std::max(p.stages * p.stage_bytes, 3 * chunks * kPieceV);
+    // (more than a third of an SM's shared memory, whatever the rank: a third block would wait for tensor memory)
+    const size_t smem = std::max(size_t(rest + p.ring_bytes), size_t(78 * 1024));
     p.wait_ns = wait_limit_ns();
     FRX_LAUNCH(kKGateUp, stream, launch_pdl_cluster(k_adapter<XTYPE, TYPE>, dim3(unsigned(tiles) * blocks), dim3(kThreads), smem, stream, blocks, p, x_map, a_map, b_map));
     FRX_CUDA(cudaGetLastError());
@@ -537,9 +620,11 @@ extern "C" int frx_adapter_add(frx_stream_t stream, const void* x, int64_t ldx, 
     p.rank16 = (rank + 15) & ~15;
     p.box = T / R >= 64 ? 64 : 16;   // rows of a load: few where most requests have a token or two
     p.idesc = f16_idesc(dtype, false, false);
+    const int64_t size = dtype_size(y_dtype);
+    p.whole = rows * size % 32 == 0 && aligned(y, 32) && aligned(out, 32) && ldy * size % 32 == 0 && ldo * size % 32 == 0;
     CUtensorMap xm, am, bm;
     if ((rc = rows_map(xm, x, ldx, dtype, T, n, p.box)) != FRX_OK || (rc = matrices_map(am, a, lda, stride_a, dtype, L, rank, n, p.rank16)) != FRX_OK ||
-        (rc = matrices_map(bm, b, ldb, stride_b, dtype, L, rows, rank, kRows)) != FRX_OK)
+        (rc = second_map(bm, b, ldb, stride_b, dtype, L, rows, rank, p.whole ? 32 / dtype_size(y_dtype) : 0)) != FRX_OK)
         return rc;
     return dtype == FRX_BF16 ? launch<FRX_BF16>(p, y_dtype, xm, am, bm, stream) : launch<FRX_F16>(p, y_dtype, xm, am, bm, stream);
 }

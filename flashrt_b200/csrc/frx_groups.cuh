@@ -206,7 +206,7 @@ inline int encode_tensor_map(CUtensorMap& map, CUtensorMapDataType type, int ran
         if (found != cudaDriverEntryPointSuccess || !fn) return fail(FRX_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
         entry.store(fn, std::memory_order_release);
     }
-    const cuuint32_t steps[3] = {1, 1, 1};
+    const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
     const CUresult r = reinterpret_cast<Encode>(fn)(&map, type, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FRX_OK : fail(FRX_ERR_CUDA, "cuTensorMapEncodeTiled: error %d (%llu rows of %llu elements)", int(r), (unsigned long long)dims[1], (unsigned long long)dims[0]);
