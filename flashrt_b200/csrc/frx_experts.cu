@@ -15,13 +15,18 @@ namespace {
 // them. Operands come by TMA in the 128-byte swizzle as they lie in memory: a side whose index is contiguous there is the instruction's MN-major form, so no
 // operand is ever transposed. A stage is 64 of depth. What lies beyond a matrix, or beyond all rows, arrives as zeros. Rows of the next expert that a box brings along fill
 // columns of D that are not stored; in the third form, where they would be summed, they are zeroed in shared memory first.
+//
+// Two blocks on neighbouring SMs (a cluster) share a tile of 256 lanes by up to 256 columns: the instruction (cta_group::2) takes 128 lanes and half of the columns from the shared memory of
+// each and leaves 128 lanes of all columns in the tensor memory of each. So 32 KB a stage and SM feed 512 clocks of products, 64 bytes a clock; one block's tile of 128 x 256 wanted
+// 96, and the L2 gives some 55 to 60 (131,072 rows of 2,048 by 1,024 in 712 us so). The first block of a pair issues; both load their own operands, whose bytes are counted on the
+// first one's barriers, and both write their own lanes.
 enum Form { kForward, kGradX, kGradW };
 
-constexpr int kTileM = 128, kDepth = 64, kTileN = 256;
-constexpr int kStageA = kTileM * kDepth * 2, kChunk = 64 * kDepth * 2;   // bytes of a stage's lanes side; of 64 contiguous elements x 64 of an MN-major side
+constexpr int kTileM = 256, kLanes = 128, kDepth = 64, kTileN = 256, kUnitN = 32;   // lanes of a tile, of a block; columns of a tile at most, what they are a multiple of
+constexpr int kStageA = kLanes * kDepth * 2, kChunk = 64 * kDepth * 2;   // bytes of a stage's lanes side; of 64 contiguous elements x 64 of an MN-major side
 constexpr int kMaxStages = 10;
-constexpr int kWarpsEpi = 8, kWarpLoad = 8, kWarpMma = 9, kThreads = 32 * 10;
-constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBars = kBarDFree + 2;
+constexpr int kWarpsEpi = 8, kWarpLoad = 8, kWarpMma = 9, kWarpTail = 10, kThreads = 32 * 11;
+constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBarTail = kBarDFree + 2, kBars = kBarTail + kMaxStages;
 constexpr int kAbort = 512, kSlot = 516, kSums = 640, kHead = 1024;
 static_assert(kBars * 8 <= kAbort && kSums + 8 * kThreads / 32 <= kHead, "the block's head");
 
@@ -42,6 +47,33 @@ struct Product {
 // Shared-memory descriptor of an operand whose rows of 128 bytes run along its own index (64 elements) and not along the depth: 128-byte swizzle, eight of depth
 // 1024 bytes apart, the next 64 elements a chunk further.
 __device__ __forceinline__ uint64_t umma_desc_mn(uint32_t smem_addr) { return umma_desc(smem_addr, kChunk, 1024) | (uint64_t(2) << 61); }
+
+// Loads of a pair: into this block's shared memory, counted on a barrier of the first block (at its address in the cluster)
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+// 256 lanes x N x 16 of depth, operands at the same places in both blocks' shared memory
+__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// An arrival at this barrier of both blocks when every MMA issued so far by this thread has completed
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3)) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result, uint32_t cols) {   // by one warp of each block
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free_pair(uint32_t base, uint32_t cols) { asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory"); }
 
 // what is there, added to eight columns of this lane (32 bits, before the one rounding)
 template <int TYPE>
@@ -65,30 +97,30 @@ template <int FORM>
 struct Tiles {
     GroupWalk g;
     int tile, per, across;   // third form: the tile, tiles of a matrix, of them along the columns
-    int e, lane0, col0, live, width;   // expert; first of the lanes side; first column, columns, their number rounded up to 16
+    int e, lane0, col0, live, width;   // expert; first of the tile's lanes side; first column, columns, their number rounded up to 32
     int row0, steps, last;   // first row of the expert; stages; depth of the last one
     __device__ __forceinline__ void begin(const Product& p, const GroupTables& tab, int experts) {
         if (FORM == kGradW) {
             g.tab = tab;
             across = (p.cols + kTileN - 1) / kTileN;
             per = across * ((p.lanes + kTileM - 1) / kTileM);
-            tile = int(blockIdx.x) - int(gridDim.x);
+            tile = int(blockIdx.x >> 1) - int(gridDim.x >> 1);
         } else {
-            g.begin(tab, experts);
+            g.begin(tab, experts, int(blockIdx.x >> 1), int(gridDim.x >> 1));
             steps = (p.depth + kDepth - 1) / kDepth;
             last = p.depth - (steps - 1) * kDepth;
         }
     }
     __device__ __forceinline__ bool next(const Product& p) {
         if (FORM == kGradW) {
-            tile += int(gridDim.x);
+            tile += int(gridDim.x >> 1);
             e = tile / per;
             if (e >= p.E) return false;
             const int local = tile - e * per, m = local / across;
             lane0 = m * kTileM;
             col0 = (local - m * across) * kTileN;
             live = min(kTileN, p.cols - col0);
-            width = (live + 15) & ~15;
+            width = (live + kUnitN - 1) & -kUnitN;
             row0 = g.tab.first[e];
             const int count = g.tab.count[e];
             steps = (count + kDepth - 1) / kDepth;
@@ -100,7 +132,7 @@ struct Tiles {
         lane0 = g.rp * kTileM;
         row0 = col0 = g.row0;
         live = g.live;
-        width = g.width;
+        width = __shfl_sync(0xffffffffu, (live + kUnitN - 1) & -kUnitN, 0);
         return true;
     }
 };
@@ -110,6 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t s0 = smem_u32(smem), stages0 = s0 + kHead, bars = s0, abort = s0 + kAbort, n_stages = uint32_t(p.stages), stage_bytes = uint32_t(p.stage_bytes);
+    const uint32_t rank = cluster_rank(), bars_first = peer_addr(bars, 0);   // the barriers of the pair's first block
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kAbort);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kSlot);
     GroupTables tab;
@@ -120,25 +153,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
     if (threadIdx.x == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(smem);
         for (int i = 0; i < kMaxStages; ++i) {
-            mbar_init(b + kBarFull + i, 1);
+            mbar_init(b + kBarFull + i, FORM == kGradW ? 2 : 1);   // the first block with the bytes of both; where a block may have to zero something, each of them
             mbar_init(b + kBarFree + i, 1);
+            mbar_init(b + kBarTail + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(b + kBarDFull + i, 1);
-            mbar_init(b + kBarDFree + i, kWarpsEpi);
+            mbar_init(b + kBarDFree + i, 2 * kWarpsEpi);
         }
         asm volatile("prefetch.tensormap [%0];" ::"l"(&lanes_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&cols_map) : "memory");
         *abort_flag = 0;
         mbar_fence_init();
     }
-    if (warp == kWarpMma) tmem_alloc(tmem_slot, 512);
+    if (warp == kWarpMma) tmem_alloc_pair(tmem_slot, 512);
     pdl_wait();
     pdl_trigger();
-    const long long tiles = group_tables<kThreads>(tab, p.offsets, p.E, p.S, p.width, (p.lanes + kTileM - 1) / kTileM, reinterpret_cast<long long*>(smem + kSums));
+    const long long tiles = group_tables<kThreads, kUnitN>(tab, p.offsets, p.E, p.S, p.width, (p.lanes + kTileM - 1) / kTileM, reinterpret_cast<long long*>(smem + kSums));
     const int experts = FORM != kGradW && tiles > p.most ? 0 : p.E;   // offsets that do not ascend: nothing is computed
     tc_fence_before_sync();
-    __syncthreads();
+    __syncwarp();
+    cluster_sync_all();   // the barriers of both blocks are there
     tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     Tiles<FORM> t;
@@ -146,75 +181,98 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
 
     // "free" barriers are waited on with the parity of the phase before the one about to be used, which a fresh barrier reports as complete
     if (warp == kWarpLoad) {
+        // ---------------- loads: this block's 128 lanes and its half of the columns
         uint32_t st = 0, phase = 1;
         bool ok = true;
         while (ok && t.next(p)) {
-            const int box = FORM == kGradW ? 64 : p.box, boxes = (t.width + box - 1) / box, box_bytes = box * 128;
-            const int halves = FORM == kForward || p.lanes - t.lane0 <= 64 ? 1 : 2;   // chunks of the lanes side
-            const uint32_t bytes = (FORM == kForward ? kStageA : uint32_t(halves * kChunk)) + uint32_t(boxes * box_bytes);
+            const int half = t.width / 2, box = FORM == kGradW ? 64 : p.box, boxes = (half + box - 1) / box, box_bytes = box * 128;
+            const int lane0 = t.lane0 + int(rank) * kLanes, col0 = t.col0 + int(rank) * half;
+            const uint32_t bytes = uint32_t(kStageA + boxes * box_bytes);
             for (int s = 0; s < t.steps; ++s) {
                 if (!(ok = warp_wait(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns))) break;
-                const uint32_t full = bars + (kBarFull + st) * 8, a = stages0 + st * stage_bytes, b = a + kStageA;
+                const uint32_t a = stages0 + st * stage_bytes, b = a + kStageA;
+                // rows of the next expert have to be zeroed in the last stage: its bytes are counted here, and kWarpTail reports to the first block
+                const bool tail = FORM == kGradW && s + 1 == t.steps && t.last % 16 != 0;
+                const uint32_t full = tail ? peer_addr(bars + (kBarTail + st) * 8, rank) : bars_first + (kBarFull + st) * 8;
                 if (lane == 0) {
-                    mbar_expect_tx(full, bytes);
+                    if (tail)
+                        mbar_expect_tx(bars + (kBarTail + st) * 8, bytes);
+                    else if (rank == 0)
+                        mbar_expect_tx(bars + (kBarFull + st) * 8, 2 * bytes);
+                    else if (FORM == kGradW)
+                        mbar_arrive_peer(full);
                     if (FORM == kForward) {
-                        tma_3d(a, &lanes_map, s * kDepth, t.lane0, t.e, full);
+                        tma_3d_pair(a, &lanes_map, s * kDepth, lane0, t.e, full);
                     } else {
-                        for (int i = 0; i < halves; ++i) {
+                        for (int i = 0; i < 2; ++i) {
                             if (FORM == kGradX)
-                                tma_3d(a + i * kChunk, &lanes_map, t.lane0 + 64 * i, s * kDepth, t.e, full);
+                                tma_3d_pair(a + i * kChunk, &lanes_map, lane0 + 64 * i, s * kDepth, t.e, full);
                             else
-                                tma_2d(a + i * kChunk, &lanes_map, t.lane0 + 64 * i, t.row0 + s * kDepth, full);
+                                tma_2d_pair(a + i * kChunk, &lanes_map, lane0 + 64 * i, t.row0 + s * kDepth, full);
                         }
                     }
                     for (int i = 0; i < boxes; ++i) {
                         if (FORM == kGradW)
-                            tma_2d(b + i * kChunk, &cols_map, t.col0 + 64 * i, t.row0 + s * kDepth, full);
+                            tma_2d_pair(b + i * kChunk, &cols_map, col0 + 64 * i, t.row0 + s * kDepth, full);
                         else
-                            tma_2d(b + i * box_bytes, &cols_map, s * kDepth, t.col0 + i * box, full);
+                            tma_2d_pair(b + i * box_bytes, &cols_map, s * kDepth, col0 + i * box, full);
                     }
                 }
                 __syncwarp();
                 if (++st == n_stages) st = 0, phase ^= 1u;
             }
         }
-    } else if (warp == kWarpMma) {
-        uint32_t st = 0, phase = 0, set = 0, dphase = 1;
-        bool ok = true;
-        while (ok && t.next(p)) {
-            const uint32_t idesc = p.idesc | uint32_t(t.width >> 3) << 17;
-            if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
-            tc_fence_after_sync();   // behind the epilogue's loads of these accumulators
-            const uint32_t acc = tmem + set * kTileN;
-            for (int s = 0; s < t.steps; ++s) {
-                if (!(ok = warp_wait(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns))) break;
-                const uint32_t a = stages0 + st * stage_bytes, b = a + kStageA;
-                const int depth = s + 1 < t.steps ? kDepth : t.last;
-                if (FORM == kGradW && depth % 16) {
-                    // the rows behind the expert's last one, up to the next 16: zeros (a row of depth is 128 bytes in every chunk, whatever the swizzle)
-                    const int extra = 16 - depth % 16, chunks = 2 + (t.width + 63) / 64;
+    } else if (warp == kWarpTail) {
+        // ---------------- third form: the rows behind the expert's last one, up to the next 16, to zeros in both operands (a row of depth is 128 bytes in every chunk, whatever the swizzle)
+        if (FORM == kGradW) {
+            uint32_t st = 0, phases = 0;   // a stage's barrier is used again only when its products are done: a phase bit each
+            while (t.next(p)) {
+                st += uint32_t(t.steps);
+                if (t.steps && t.last % 16) {
+                    const uint32_t stage = (st - 1) % n_stages;
+                    if (!warp_wait(bars + (kBarTail + stage) * 8, phases >> stage & 1u, abort, p.wait_ns)) break;
+                    phases ^= 1u << stage;
+                    const uint32_t a = stages0 + stage * stage_bytes;
+                    const int extra = 16 - t.last % 16, chunks = 2 + (t.width / 2 + 63) / 64;
                     for (int i = lane; i < chunks * extra * 8; i += 32) {
                         const int r = i >> 3, c = r / extra;
-                        const uint32_t at = (c < 2 ? a + c * kChunk : b + (c - 2) * kChunk) + uint32_t(depth + r - c * extra) * 128 + (i & 7) * 16;
+                        const uint32_t at = a + uint32_t(c * kChunk + (t.last + r - c * extra) * 128 + (i & 7) * 16);   // (the lanes side's two chunks, then the columns')
                         asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
                     }
                     fence_async_smem();   // generic-proxy writes: visible to the tensor core
                     __syncwarp();
+                    if (lane == 0) mbar_arrive_peer(bars_first + (kBarFull + stage) * 8);
                 }
+                st %= n_stages;
+            }
+        }
+    } else if (warp == kWarpMma) {
+        // ---------------- MMA: the first block's warp, one elected lane
+        uint32_t st = 0, phase = 0, set = 0, dphase = 1;
+        bool ok = rank == 0;
+        while (ok && t.next(p)) {
+            const uint32_t idesc = p.idesc | uint32_t(t.width >> 3) << 17;
+            if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
+            tc_fence_after_sync();   // behind the epilogues' loads of these accumulators
+            const uint32_t acc = tmem + set * kTileN;
+            for (int s = 0; s < t.steps; ++s) {
+                if (!(ok = warp_wait_cluster(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns))) break;
+                const uint32_t a = stages0 + st * stage_bytes, b = a + kStageA;
+                const int depth = s + 1 < t.steps ? kDepth : t.last;
                 if (elect_one()) {
                     const uint64_t da = FORM == kForward ? umma_desc_sw128(a) : umma_desc_mn(a), db = FORM == kGradW ? umma_desc_mn(b) : umma_desc_sw128(b);
                     constexpr uint64_t kStepK = 32 >> 4, kStepMn = 16 * 128 >> 4;   // 16 of depth
 #pragma unroll
                     for (int k = 0; k < kDepth / 16; ++k) {
                         if (k * 16 >= depth) break;
-                        umma_f16(acc, da + k * (FORM == kForward ? kStepK : kStepMn), db + k * (FORM == kGradW ? kStepMn : kStepK), idesc, s + k > 0);
+                        umma_f16_pair(acc, da + k * (FORM == kForward ? kStepK : kStepMn), db + k * (FORM == kGradW ? kStepMn : kStepK), idesc, s + k > 0);
                     }
-                    umma_commit(bars + (kBarFree + st) * 8);
+                    umma_commit_pair(bars + (kBarFree + st) * 8);
                 }
                 __syncwarp();
                 if (++st == n_stages) st = 0, phase ^= 1u;
             }
-            if (ok && elect_one()) umma_commit(bars + (kBarDFull + set) * 8);
+            if (ok && elect_one()) umma_commit_pair(bars + (kBarDFull + set) * 8);
             __syncwarp();
             set ^= 1u;
             if (set == 0) dphase ^= 1u;
@@ -230,8 +288,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
             lost = lost || !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);
             tc_fence_after_sync();
             const uint32_t acc = tmem + (uint32_t(quarter * 32) << 16) + set * kTileN;
-            const bool have = t.lane0 + m < p.lanes, empty = FORM == kGradW && t.steps == 0;
-            uint8_t* y = static_cast<uint8_t*>(p.y) + ((FORM == kGradW ? t.e * p.ldye : 0) + t.col0 * p.ldy + t.lane0 + m) * size;
+            const int at_lane = t.lane0 + int(rank) * kLanes + m;
+            const bool have = at_lane < p.lanes, empty = FORM == kGradW && t.steps == 0;
+            uint8_t* y = static_cast<uint8_t*>(p.y) + ((FORM == kGradW ? t.e * p.ldye : 0) + t.col0 * p.ldy + at_lane) * size;
             for (int c = part * 16; c < t.width && !(empty && p.add); c += 32) {
                 uint32_t v[2][8];
                 if (lost || empty) {
@@ -250,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
             if (!lost) {
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bars + (kBarDFree + set) * 8);
+                if (lane == 0) mbar_arrive_peer(bars_first + (kBarDFree + set) * 8);
             }
             set ^= 1u;
             if (set == 0) phase ^= 1u;
@@ -266,7 +325,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
         }
         __syncthreads();
     }
-    if (warp == kWarpMma) tmem_free(tmem, 512);
+    cluster_sync_all();   // neither block's shared or tensor memory is used by the other any more
+    if (warp == kWarpMma) tmem_free_pair(tmem, 512);
 }
 
 template <int FORM, int TYPE>
@@ -279,10 +339,11 @@ int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& co
     if (most > 0x7fff0000 || p.S / 16 >= (1 << 24)) return fail(FRX_ERR_SHAPE, "product by expert: %lld tiles of %d rows", (long long)most, p.S);
     p.most = int(most);
     p.stages = int(std::min<size_t>(kMaxStages, (kSmemMost - kHead - tables) / size_t(p.stage_bytes)));
-    static_assert((kSmemMost - kHead - 4096 * 16) / (kStageA + kTileN * kDepth * 2) >= 3, "stages beside the tables of 4096 experts");
+    static_assert((kSmemMost - kHead - 4096 * 16) / (kStageA + kTileN / 2 * kDepth * 2) >= 4, "stages beside the tables of 4096 experts");
     p.wait_ns = wait_limit_ns();
-    const unsigned grid = unsigned(std::min<int64_t>(sm_count(), std::max<int64_t>(1, most)));
-    FRX_LAUNCH(kKGateUp, stream, launch_pdl(k_moe_product<FORM, TYPE>, dim3(grid), dim3(kThreads), kHead + size_t(p.stages) * p.stage_bytes + tables, stream, p, lanes_map, cols_map));
+    const unsigned pairs = unsigned(std::min<int64_t>(std::max(1, sm_count() / 2), std::max<int64_t>(1, most)));
+    FRX_LAUNCH(kKGateUp, stream,
+               launch_pdl_cluster(k_moe_product<FORM, TYPE>, dim3(2 * pairs), dim3(kThreads), kHead + size_t(p.stages) * p.stage_bytes + tables, stream, 2u, p, lanes_map, cols_map));
     FRX_CUDA(cudaGetLastError());
     return FRX_OK;
 }
@@ -313,10 +374,10 @@ int result(const char* who, const char* what, const void* y, int64_t ld, int64_t
 // flight.
 void row_tiles(Product& p) {
     const int average = (p.S + p.E - 1) / p.E;
-    p.width = 16;
+    p.width = kUnitN;
     while (p.width < kTileN && p.width < 2 * average) p.width *= 2;
     p.box = p.width >= 128 ? 32 : 16;
-    p.stage_bytes = kStageA + p.width * kDepth * 2;
+    p.stage_bytes = kStageA + p.width / 2 * kDepth * 2;
 }
 
 }  // namespace
@@ -343,9 +404,9 @@ int frx_moe_matmul(frx_stream_t stream, const void* x, int64_t ldx, const void* 
     p.lanes = rows;
     p.depth = n;
     row_tiles(p);
-    p.idesc = f16_idesc(dtype, false, false);
+    p.idesc = f16_idesc(dtype, false, false, kTileM);
     CUtensorMap wm, xm;
-    if ((rc = matrices_map(wm, w, ldw, lde, dtype, E, rows, n, kTileM)) != FRX_OK || (rc = rows_map(xm, x, ldx, dtype, S, n, p.box)) != FRX_OK) return rc;
+    if ((rc = matrices_map(wm, w, ldw, lde, dtype, E, rows, n, kLanes)) != FRX_OK || (rc = rows_map(xm, x, ldx, dtype, S, n, p.box)) != FRX_OK) return rc;
     return launch<kForward>(p, out_dtype, wm, xm, stream);
 }
 
@@ -367,7 +428,7 @@ int frx_moe_matmul_backward_x(frx_stream_t stream, const void* gy, int64_t ldgy,
     p.lanes = n;
     p.depth = rows;
     row_tiles(p);
-    p.idesc = f16_idesc(dtype, true, false);
+    p.idesc = f16_idesc(dtype, true, false, kTileM);
     CUtensorMap wm, gm;
     if ((rc = matrices_map(wm, w, ldw, lde, dtype, E, rows, n, kDepth)) != FRX_OK || (rc = rows_map(gm, gy, ldgy, dtype, S, rows, p.box)) != FRX_OK) return rc;
     return launch<kGradX>(p, out_dtype, wm, gm, stream);
@@ -399,8 +460,8 @@ int frx_moe_matmul_backward_w(frx_stream_t stream, const void* gy, int64_t ldgy,
     p.cols = rows;
     p.width = kTileN;
     p.add = add != 0;
-    p.stage_bytes = kStageA + std::min((rows + 63) / 64, kTileN / 64) * kChunk;
-    p.idesc = f16_idesc(dtype, true, true);
+    p.stage_bytes = kStageA + std::min((rows + 127) / 128, kTileN / 128) * kChunk;
+    p.idesc = f16_idesc(dtype, true, true, kTileM);
     CUtensorMap xm, gm;
     if ((rc = rows_map(xm, x, ldx, dtype, S, n, kDepth)) != FRX_OK || (rc = rows_map(gm, gy, ldgy, dtype, S, rows, kDepth)) != FRX_OK) return rc;
     return launch<kGradW>(p, out_dtype, xm, gm, stream);

@@ -46,14 +46,16 @@ struct GroupWalk {
     int E, tile, e;
     int rp, row0, live, width;   // row pair, first y row, y rows, their number rounded up to 16
     bool alone;                  // the expert has one block of y rows: this tile's weights are read by no other
-    __device__ __forceinline__ void begin(const GroupTables& tables, int experts) {
+    int stride;                  // tiles between two of this block: as many as there are blocks, or pairs of them
+    __device__ __forceinline__ void begin(const GroupTables& tables, int experts, int block = int(blockIdx.x), int blocks = int(gridDim.x)) {
         tab = tables;
         E = experts;
-        tile = int(blockIdx.x) - int(gridDim.x);
+        tile = block - blocks;
+        stride = blocks;
         e = 0;
     }
     __device__ __forceinline__ bool next() {
-        tile += int(gridDim.x);
+        tile += stride;
         const int lane = threadIdx.x & 31;
         // 32 experts at a time, those that end at or before the tile: from the last one on, then, if all of these do, over the whole list
         // in 32 steps
@@ -82,10 +84,10 @@ struct GroupWalk {
     }
 };
 
-// Fills the tables: a thread takes a few experts in a row. blocks: tiles across the matrix; width: y rows of a tile at most (a multiple of 16, up to 256). Returns the number of
+// Fills the tables: a thread takes a few experts in a row. blocks: tiles across the matrix; width: y rows of a tile at most (a multiple of UNIT, up to 256). Returns the number of
 // tiles, which is more than there can be where offsets do not ascend. All THREADS threads of the block; sums: one a warp. The tables are
 // complete behind the next barrier of the block.
-template <int THREADS>
+template <int THREADS, int UNIT = 16>
 __device__ __forceinline__ long long group_tables(const GroupTables& tab, const int32_t* offsets, int E, int S, int width, int across, long long* sums) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = (E + THREADS - 1) / THREADS, e0 = min(E, int(threadIdx.x) * per), e1 = min(E, e0 + per);
@@ -97,7 +99,7 @@ __device__ __forceinline__ long long group_tables(const GroupTables& tab, const 
             b = min(max(__ldcg(offsets + e + 1), a), S);
         }
         const int count = b - a, blocks = (count + width - 1) / width;
-        const int w16 = blocks ? ((count + blocks - 1) / blocks + 15) >> 4 : 0;   // as even as multiples of 16 allow
+        const int w16 = blocks ? ((count + blocks - 1) / blocks + UNIT - 1) / UNIT * (UNIT / 16) : 0;   // as even as multiples of UNIT allow
         tab.first[e] = a;
         tab.count[e] = count;
         tab.blocks[e] = blocks | w16 << 24;
@@ -159,6 +161,38 @@ __device__ __forceinline__ void store8(const uint32_t (&v)[8], void* y, int64_t 
             else
                 *reinterpret_cast<__half*>(p) = __float2half_rn(__uint_as_float(v[i]));
         }
+}
+
+// ---- blocks of a cluster
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t addr) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory"); }
+// warp_wait for what other blocks of the cluster have written
+__device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity, uint32_t abort, uint64_t limit_ns) {
+    if (!warp_wait(bar, parity, abort, limit_ns)) return false;
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return __all_sync(0xffffffffu, ok != 0);
 }
 
 // ---- 16-bit operands
@@ -226,10 +260,10 @@ inline int allow_smem() {
     return FRX_OK;
 }
 
-// Instruction descriptor of kind::f16 without N: sums in 32 bits, both operands of one type (0 fp16, 1 bf16), `mn` bits where an operand is MN-major, 128 lanes
-inline uint32_t f16_idesc(int dtype, bool lanes_mn, bool cols_mn) {
+// Instruction descriptor of kind::f16 without N: sums in 32 bits, both operands of one type (0 fp16, 1 bf16), `mn` bits where an operand is MN-major
+inline uint32_t f16_idesc(int dtype, bool lanes_mn, bool cols_mn, int lanes = 128) {
     const uint32_t type = dtype == FRX_BF16;
-    return (1u << 4) | type << 7 | type << 10 | uint32_t(lanes_mn) << 15 | uint32_t(cols_mn) << 16 | uint32_t(128 >> 4) << 24;
+    return (1u << 4) | type << 7 | type << 10 | uint32_t(lanes_mn) << 15 | uint32_t(cols_mn) << 16 | uint32_t(lanes >> 4) << 24;
 }
 inline CUtensorMapDataType map_type(int dtype) { return dtype == FRX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
 
