@@ -26,7 +26,7 @@ constexpr int kTileM = 256, kLanes = 128, kDepth = 64, kTileN = 256, kUnitN = 32
 constexpr int kStageA = kLanes * kDepth * 2, kChunk = 64 * kDepth * 2;   // bytes of a stage's lanes side; of 64 contiguous elements x 64 of an MN-major side
 constexpr int kMaxStages = 10;
 constexpr int kWarpsEpi = 8, kWarpLoad = 8, kWarpMma = 9, kWarpTail = 10, kThreads = 32 * 11;
-constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBarTail = kBarDFree + 2, kBars = kBarTail + kMaxStages;
+constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBarTail = kBarDFree + 2, kBarTailPeer = kBarTail + kMaxStages, kBars = kBarTailPeer + kMaxStages;
 constexpr int kAbort = 512, kSlot = 516, kSums = 640, kHead = 1024;
 static_assert(kBars * 8 <= kAbort && kSums + 8 * kThreads / 32 <= kHead, "the block's head");
 
@@ -153,9 +153,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
     if (threadIdx.x == 0) {
         uint64_t* b = reinterpret_cast<uint64_t*>(smem);
         for (int i = 0; i < kMaxStages; ++i) {
-            mbar_init(b + kBarFull + i, FORM == kGradW ? 2 : 1);   // the first block with the bytes of both; where a block may have to zero something, each of them
+            mbar_init(b + kBarFull + i, 1);   // the first block, with the bytes of both
             mbar_init(b + kBarFree + i, 1);
             mbar_init(b + kBarTail + i, 1);
+            mbar_init(b + kBarTailPeer + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(b + kBarDFull + i, 1);
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
             for (int s = 0; s < t.steps; ++s) {
                 if (!(ok = warp_wait(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns))) break;
                 const uint32_t a = stages0 + st * stage_bytes, b = a + kStageA;
-                // rows of the next expert have to be zeroed in the last stage: its bytes are counted here, and kWarpTail reports to the first block
+                // rows of the next expert have to be zeroed in the last stage: its bytes are counted here, and kWarpTail reports
                 const bool tail = FORM == kGradW && s + 1 == t.steps && t.last % 16 != 0;
                 const uint32_t full = tail ? peer_addr(bars + (kBarTail + st) * 8, rank) : bars_first + (kBarFull + st) * 8;
                 if (lane == 0) {
@@ -199,8 +200,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
                         mbar_expect_tx(bars + (kBarTail + st) * 8, bytes);
                     else if (rank == 0)
                         mbar_expect_tx(bars + (kBarFull + st) * 8, 2 * bytes);
-                    else if (FORM == kGradW)
-                        mbar_arrive_peer(full);
                     if (FORM == kForward) {
                         tma_3d_pair(a, &lanes_map, s * kDepth, lane0, t.e, full);
                     } else {
@@ -225,13 +224,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
     } else if (warp == kWarpTail) {
         // ---------------- third form: the rows behind the expert's last one, up to the next 16, to zeros in both operands (a row of depth is 128 bytes in every chunk, whatever the swizzle)
         if (FORM == kGradW) {
-            uint32_t st = 0, phases = 0;   // a stage's barrier is used again only when its products are done: a phase bit each
+            uint32_t st = 0, phases = 0;   // a stage's barriers are used again only when its products are done: a phase bit each (one barrier for all stages could run two phases ahead of its waiter)
             while (t.next(p)) {
                 st += uint32_t(t.steps);
                 if (t.steps && t.last % 16) {
                     const uint32_t stage = (st - 1) % n_stages;
                     if (!warp_wait(bars + (kBarTail + stage) * 8, phases >> stage & 1u, abort, p.wait_ns)) break;
-                    phases ^= 1u << stage;
                     const uint32_t a = stages0 + stage * stage_bytes;
                     const int extra = 16 - t.last % 16, chunks = 2 + (t.width / 2 + 63) / 64;
                     for (int i = lane; i < chunks * extra * 8; i += 32) {
@@ -241,7 +239,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
                     }
                     fence_async_smem();   // generic-proxy writes: visible to the tensor core
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_peer(bars_first + (kBarFull + stage) * 8);
+                    if (rank == 0 && !warp_wait_cluster(bars + (kBarTailPeer + stage) * 8, phases >> stage & 1u, abort, p.wait_ns)) break;
+                    if (lane == 0) mbar_arrive_peer(bars_first + ((rank ? kBarTailPeer : kBarFull) + stage) * 8);
+                    phases ^= 1u << stage;
                 }
                 st %= n_stages;
             }
