@@ -37,7 +37,9 @@ struct Product {
     unsigned long long wait_ns;
     int E, S;
     int lanes, cols, depth;   // extents: of the lanes side; of the columns side in the third form; of the depth in the other two
-    int width, box;           // columns of a tile at most; rows of a load of the columns side in the first two forms
+    int width, box, box_small;   // columns of a tile at most; rows of a load of the columns side in the first two forms, and of a small one
+    int unit;                 // columns of a tile are a multiple of this
+    int lanes_chunks, cols_chunks;   // chunks of 64 a load of an MN-major side brings
     int stages, stage_bytes;
     int most;                 // tiles of any plan whose experts' rows do not overlap
     uint32_t idesc;           // the instruction descriptor without N
@@ -54,6 +56,11 @@ __device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map
 }
 __device__ __forceinline__ void tma_3d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_4d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int u, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(u),
+                 "r"(bar)
                  : "memory");
 }
 // 256 lanes x N x 16 of depth, operands at the same places in both blocks' shared memory
@@ -120,7 +127,7 @@ struct Tiles {
             lane0 = m * kTileM;
             col0 = (local - m * across) * kTileN;
             live = min(kTileN, p.cols - col0);
-            width = (live + kUnitN - 1) & -kUnitN;
+            width = (live + p.unit - 1) & -p.unit;
             row0 = g.tab.first[e];
             const int count = g.tab.count[e];
             steps = (count + kDepth - 1) / kDepth;
@@ -138,7 +145,8 @@ struct Tiles {
 };
 
 template <int FORM, int TYPE>
-__global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, const __grid_constant__ CUtensorMap lanes_map, const __grid_constant__ CUtensorMap cols_map) {
+__global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, const __grid_constant__ CUtensorMap lanes_map, const __grid_constant__ CUtensorMap cols_map,
+                                                              const __grid_constant__ CUtensorMap small_map) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t s0 = smem_u32(smem), stages0 = s0 + kHead, bars = s0, abort = s0 + kAbort, n_stages = uint32_t(p.stages), stage_bytes = uint32_t(p.stage_bytes);
@@ -182,12 +190,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
 
     // "free" barriers are waited on with the parity of the phase before the one about to be used, which a fresh barrier reports as complete
     if (warp == kWarpLoad) {
-        // ---------------- loads: this block's 128 lanes and its half of the columns
+        // ---------------- loads: this block's 128 lanes and its half of the columns, in as few as possible (each costs the issuing thread some 100 clocks, whatever its size: with
+        // 5 of them a stage took 750 clocks, with two 520)
         uint32_t st = 0, phase = 1;
         bool ok = true;
         while (ok && t.next(p)) {
-            const int half = t.width / 2, box = FORM == kGradW ? 64 : p.box, boxes = (half + box - 1) / box, box_bytes = box * 128;
-            const int lane0 = t.lane0 + int(rank) * kLanes, col0 = t.col0 + int(rank) * half;
+            const int half = t.width / 2, lane0 = t.lane0 + int(rank) * kLanes, col0 = t.col0 + int(rank) * half;
+            const bool small = FORM != kGradW && half <= 3 * p.box_small;
+            const int box = FORM == kGradW ? 64 * p.cols_chunks : small ? p.box_small : p.box, boxes = (half + box - 1) / box, box_bytes = box * 128;
+            const CUtensorMap* const cols = small ? &small_map : &cols_map;
             const uint32_t bytes = uint32_t(kStageA + boxes * box_bytes);
             for (int s = 0; s < t.steps; ++s) {
                 if (!(ok = warp_wait(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns))) break;
@@ -202,6 +213,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
                         mbar_expect_tx(bars + (kBarFull + st) * 8, 2 * bytes);
                     if (FORM == kForward) {
                         tma_3d_pair(a, &lanes_map, s * kDepth, lane0, t.e, full);
+                    } else if (p.lanes_chunks == 2) {
+                        if (FORM == kGradX)
+                            tma_4d_pair(a, &lanes_map, 0, s * kDepth, lane0 / 64, t.e, full);
+                        else
+                            tma_3d_pair(a, &lanes_map, 0, t.row0 + s * kDepth, lane0 / 64, full);
                     } else {
                         for (int i = 0; i < 2; ++i) {
                             if (FORM == kGradX)
@@ -210,12 +226,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
                                 tma_2d_pair(a + i * kChunk, &lanes_map, lane0 + 64 * i, t.row0 + s * kDepth, full);
                         }
                     }
-                    for (int i = 0; i < boxes; ++i) {
-                        if (FORM == kGradW)
-                            tma_2d_pair(b + i * kChunk, &cols_map, col0 + 64 * i, t.row0 + s * kDepth, full);
-                        else
-                            tma_2d_pair(b + i * box_bytes, &cols_map, s * kDepth, col0 + i * box, full);
-                    }
+                    if (FORM == kGradW && p.cols_chunks == 2)
+                        tma_3d_pair(b, &cols_map, 0, t.row0 + s * kDepth, col0 / 64, full);
+                    else
+                        for (int i = 0; i < boxes; ++i) {
+                            if (FORM == kGradW)
+                                tma_2d_pair(b + i * kChunk, &cols_map, col0 + 64 * i, t.row0 + s * kDepth, full);
+                            else
+                                tma_2d_pair(b + i * box_bytes, cols, s * kDepth, col0 + i * box, full);
+                        }
                 }
                 __syncwarp();
                 if (++st == n_stages) st = 0, phase ^= 1u;
@@ -330,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
 }
 
 template <int FORM, int TYPE>
-int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& cols_map, cudaStream_t stream) {
+int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& cols_map, const CUtensorMap& small_map, cudaStream_t stream) {
     const size_t tables = size_t(p.E) * 16;
     int rc = allow_smem<k_moe_product<FORM, TYPE>>();
     if (rc != FRX_OK) return rc;
@@ -343,17 +362,31 @@ int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& co
     p.wait_ns = wait_limit_ns();
     const unsigned pairs = unsigned(std::min<int64_t>(std::max(1, sm_count() / 2), std::max<int64_t>(1, most)));
     FRX_LAUNCH(kKGateUp, stream,
-               launch_pdl_cluster(k_moe_product<FORM, TYPE>, dim3(2 * pairs), dim3(kThreads), kHead + size_t(p.stages) * p.stage_bytes + tables, stream, 2u, p, lanes_map, cols_map));
+               launch_pdl_cluster(k_moe_product<FORM, TYPE>, dim3(2 * pairs), dim3(kThreads), kHead + size_t(p.stages) * p.stage_bytes + tables, stream, 2u, p, lanes_map, cols_map, small_map));
     FRX_CUDA(cudaGetLastError());
     return FRX_OK;
 }
 template <int FORM>
-int launch(Product& p, int type, const CUtensorMap& lanes_map, const CUtensorMap& cols_map, cudaStream_t stream) {
+int launch(Product& p, int type, const CUtensorMap& lanes_map, const CUtensorMap& cols_map, const CUtensorMap& small_map, cudaStream_t stream) {
     switch (type) {
-        case FRX_F32: return launch_typed<FORM, FRX_F32>(p, lanes_map, cols_map, stream);
-        case FRX_BF16: return launch_typed<FORM, FRX_BF16>(p, lanes_map, cols_map, stream);
-        default: return launch_typed<FORM, FRX_F16>(p, lanes_map, cols_map, stream);
+        case FRX_F32: return launch_typed<FORM, FRX_F32>(p, lanes_map, cols_map, small_map, stream);
+        case FRX_BF16: return launch_typed<FORM, FRX_BF16>(p, lanes_map, cols_map, small_map, stream);
+        default: return launch_typed<FORM, FRX_F16>(p, lanes_map, cols_map, small_map, stream);
     }
+}
+
+// Sides whose index is contiguous in memory, 64 of depth a load: two chunks of 64 at once where the extent is whole chunks (the chunk is a dimension of the map then), else one
+int depth_rows_map(CUtensorMap& map, const void* x, int64_t ld, int dtype, int rows, int n, int chunks) {
+    if (chunks == 1) return rows_map(map, x, ld, dtype, rows, n, kDepth);
+    const cuuint64_t dims[3] = {64, cuuint64_t(rows), cuuint64_t(n / 64)}, strides[2] = {cuuint64_t(ld) * 2, 128};
+    const cuuint32_t boxes[3] = {64, kDepth, cuuint32_t(chunks)};
+    return encode_tensor_map(map, map_type(dtype), 3, x, dims, strides, boxes);
+}
+int depth_matrices_map(CUtensorMap& map, const void* w, int64_t ldw, int64_t lde, int dtype, int E, int rows, int n, int chunks) {
+    if (chunks == 1) return matrices_map(map, w, ldw, lde, dtype, E, rows, n, kDepth);
+    const cuuint64_t dims[4] = {64, cuuint64_t(rows), cuuint64_t(n / 64), cuuint64_t(E)}, strides[3] = {cuuint64_t(ldw) * 2, 128, cuuint64_t(lde) * 2};
+    const cuuint32_t boxes[4] = {64, kDepth, cuuint32_t(chunks), 1};
+    return encode_tensor_map(map, map_type(dtype), 4, w, dims, strides, boxes);
 }
 
 int shape(const char* who, int dtype, int out_dtype, int E, int rows, int n, int S) {
@@ -376,7 +409,8 @@ void row_tiles(Product& p) {
     const int average = (p.S + p.E - 1) / p.E;
     p.width = kUnitN;
     while (p.width < kTileN && p.width < 2 * average) p.width *= 2;
-    p.box = p.width >= 128 ? 32 : 16;
+    p.box = p.width / 2;
+    p.box_small = std::max(16, p.width / 8);
     p.stage_bytes = kStageA + p.width / 2 * kDepth * 2;
 }
 
@@ -405,9 +439,11 @@ int frx_moe_matmul(frx_stream_t stream, const void* x, int64_t ldx, const void* 
     p.depth = n;
     row_tiles(p);
     p.idesc = f16_idesc(dtype, false, false, kTileM);
-    CUtensorMap wm, xm;
-    if ((rc = matrices_map(wm, w, ldw, lde, dtype, E, rows, n, kLanes)) != FRX_OK || (rc = rows_map(xm, x, ldx, dtype, S, n, p.box)) != FRX_OK) return rc;
-    return launch<kForward>(p, out_dtype, wm, xm, stream);
+    CUtensorMap wm, xm, small;
+    if ((rc = matrices_map(wm, w, ldw, lde, dtype, E, rows, n, kLanes)) != FRX_OK || (rc = rows_map(xm, x, ldx, dtype, S, n, p.box)) != FRX_OK ||
+        (rc = rows_map(small, x, ldx, dtype, S, n, p.box_small)) != FRX_OK)
+        return rc;
+    return launch<kForward>(p, out_dtype, wm, xm, small, stream);
 }
 
 int frx_moe_matmul_backward_x(frx_stream_t stream, const void* gy, int64_t ldgy, const void* w, int64_t ldw, int64_t lde, int dtype, const int32_t* offsets, int E, int rows, int n,
@@ -429,9 +465,12 @@ int frx_moe_matmul_backward_x(frx_stream_t stream, const void* gy, int64_t ldgy,
     p.depth = rows;
     row_tiles(p);
     p.idesc = f16_idesc(dtype, true, false, kTileM);
-    CUtensorMap wm, gm;
-    if ((rc = matrices_map(wm, w, ldw, lde, dtype, E, rows, n, kDepth)) != FRX_OK || (rc = rows_map(gm, gy, ldgy, dtype, S, rows, p.box)) != FRX_OK) return rc;
-    return launch<kGradX>(p, out_dtype, wm, gm, stream);
+    p.lanes_chunks = n % 64 == 0 ? 2 : 1;
+    CUtensorMap wm, gm, small;
+    if ((rc = depth_matrices_map(wm, w, ldw, lde, dtype, E, rows, n, p.lanes_chunks)) != FRX_OK || (rc = rows_map(gm, gy, ldgy, dtype, S, rows, p.box)) != FRX_OK ||
+        (rc = rows_map(small, gy, ldgy, dtype, S, rows, p.box_small)) != FRX_OK)
+        return rc;
+    return launch<kGradX>(p, out_dtype, wm, gm, small, stream);
 }
 
 int frx_moe_matmul_backward_w(frx_stream_t stream, const void* gy, int64_t ldgy, const void* x, int64_t ldx, int dtype, const int32_t* offsets, int E, int rows, int n, int S, void* gw,
@@ -462,9 +501,12 @@ int frx_moe_matmul_backward_w(frx_stream_t stream, const void* gy, int64_t ldgy,
     p.add = add != 0;
     p.stage_bytes = kStageA + std::min((rows + 127) / 128, kTileN / 128) * kChunk;
     p.idesc = f16_idesc(dtype, true, true, kTileM);
+    p.lanes_chunks = n % 64 == 0 ? 2 : 1;
+    p.cols_chunks = rows % 64 == 0 && rows > 128 ? 2 : 1;
+    p.unit = p.cols_chunks == 2 ? 128 : kUnitN;   // (a block's half begins with a chunk)
     CUtensorMap xm, gm;
-    if ((rc = rows_map(xm, x, ldx, dtype, S, n, kDepth)) != FRX_OK || (rc = rows_map(gm, gy, ldgy, dtype, S, rows, kDepth)) != FRX_OK) return rc;
-    return launch<kGradW>(p, out_dtype, xm, gm, stream);
+    if ((rc = depth_rows_map(xm, x, ldx, dtype, S, n, p.lanes_chunks)) != FRX_OK || (rc = depth_rows_map(gm, gy, ldgy, dtype, S, rows, p.cols_chunks)) != FRX_OK) return rc;
+    return launch<kGradW>(p, out_dtype, xm, gm, gm, stream);
 }
 
 }  // extern "C"
