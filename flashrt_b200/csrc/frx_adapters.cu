@@ -16,7 +16,7 @@ namespace {
 // parts up through one another's shared memory (in the order of the blocks), and share the second product's rows. y is read two steps (32 bits: one) ahead of the sums it is added
 // to, from before the first product on.
 constexpr int kTok = 64, kRows = 128, kDepth = 64;
-constexpr int kMaxStages = 6, kMinStages = 3, kBufs = 2;
+constexpr int kMaxStages = 10, kMinStages = 3, kBufs = 2;
 constexpr int kWarpsEpi = 8, kWarpLoad = 8, kWarpMma = 9, kThreads = 32 * 10;
 constexpr int kBarFull = 0, kBarFree = kBarFull + kMaxStages, kBarBFull = kBarFree + kMaxStages, kBarBFree = kBarBFull + kBufs, kBarDFull = kBarBFree + kBufs, kBarDFree = kBarDFull + 2,
               kBarV = kBarDFree + 2, kBarVIn = kBarV + 1, kBarPart = kBarVIn + 1, kBars = kBarPart + 1;
@@ -38,7 +38,7 @@ struct Adapters {
     int64_t ldy, ldo;
     unsigned long long wait_ns;
     int T, R, L, n, rows, rank, rank16;   // rank16: the rank rounded up to 16
-    int box, stages, stage_bytes, ring_bytes;   // rows of a load of x; stages, bytes of one, of all of them (v's pieces come to the same place)
+    int box, ring_bytes;                        // rows of a load of x; bytes of the first product's stages (v's pieces come to the same place)
     uint32_t idesc;
     int whole;                                  // y and out allow accesses of 32 bytes
 };
@@ -46,6 +46,11 @@ struct Adapters {
 __device__ __forceinline__ float4 ld_peer(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_peer1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int u, int v, uint32_t bar) {
@@ -201,12 +206,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
     {   // the cluster's tile: a thread takes a few requests in a row
         const int tile = int(blockIdx.x / blocks), per = (p.R + kThreads - 1) / kThreads, r0 = min(p.R, int(threadIdx.x) * per), r1 = min(p.R, r0 + per);
         auto range = [&](int r, int& a) {   // (what the ranges say beyond the tokens that there are is left out)
-            a = min(max(__ldcg(p.offsets + r), 0), p.T);
-            return min(max(__ldcg(p.offsets + r + 1), a), p.T) - a;
+            const int from = __ldcg(p.offsets + r), to = __ldcg(p.offsets + r + 1);
+            a = min(max(from, 0), p.T);
+            return min(max(to, a), p.T) - a;
         };
-        long long sum = 0;
-        int a;
-        for (int r = r0; r < r1; ++r) sum += (range(r, a) + kTok - 1) / kTok;
+        // (of few requests a thread has one: its adapter is read along with its range)
+        int a = 0, count = 0, j = 0;
+        if (r0 < r1) {
+            j = __ldcg(p.which + r0);
+            count = range(r0, a);
+        }
+        long long sum = (count + kTok - 1) / kTok;
+        for (int r = r0 + 1; r < r1; ++r) {
+            int unused;
+            sum += (range(r, unused) + kTok - 1) / kTok;
+        }
         long long inc = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -219,17 +233,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
         long long before = inc - sum;
         for (int i = 0; i < warp; ++i) before += sums[i];
         if (tile >= before && tile < before + sum) {
-            for (int r = r0; r < r1; ++r) {
-                const int count = range(r, a), t = int(tile - before);
-                before += (count + kTok - 1) / kTok;
-                if (tile < before) {
-                    const int j = __ldcg(p.which + r);
-                    found[0] = a + t * kTok;
-                    found[1] = min(kTok, count - t * kTok);
-                    found[2] = j >= p.L ? -1 : j;
-                    break;
-                }
+            int t = int(tile - before);   // of the thread's requests
+            for (int r = r0; t >= (count + kTok - 1) / kTok && ++r < r1;) {
+                t -= (count + kTok - 1) / kTok;
+                j = __ldcg(p.which + r);
+                count = range(r, a);
             }
+            found[0] = a + t * kTok;
+            found[1] = min(kTok, count - t * kTok);
+            found[2] = j >= p.L ? -1 : j;
         }
     }
     tc_fence_before_sync();
@@ -246,6 +258,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
     const int depths = (p.n + kDepth - 1) / kDepth, d0 = int(int64_t(depths) * rank / blocks), d1 = int(int64_t(depths) * (rank + 1) / blocks);
     const int turn = int((blockIdx.x / blocks) % unsigned(row_chunks));
     auto chunk = [&](int c) { return c + turn < row_chunks ? c + turn : c + turn - row_chunks; };
+    // A stage is the tokens' rows of x, as many as the loads bring, and A_j's: of one token 4 KB instead of 10 at a rank of 16, so that most of its depth is in flight at once.
+    const int boxes = (live + p.box - 1) / p.box;
+    const uint32_t x_bytes = uint32_t(boxes * p.box) * 128, stage_bytes = x_bytes + uint32_t(p.rank16) * 128, stages = min(uint32_t(kMaxStages), uint32_t(p.ring_bytes) / max(stage_bytes, 1u));
     bool lost = false;
 
     if (!work) {
@@ -253,8 +268,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
         if (live > 0 && p.out != p.y) copy_rows<TYPE == FRX_F32 ? 4 : 2>(p.y, p.ldy, p.out, p.ldo, t0, live, p.rows, int(rank) * (kThreads / 32) + warp, int(blocks) * (kThreads / 32));
     } else if (warp == kWarpLoad) {
         // ---------------- loads: the first product's stages, and this block's rows of B_j as soon as there is room
-        const int boxes = (live + p.box - 1) / p.box;
-        const uint32_t bytes = uint32_t(boxes * p.box * 128 + p.rank16 * 128);
         uint32_t st = 0, phase = 1, buf = 0, bphase = 1;
         int c = int(rank);
         bool ok = true;
@@ -278,15 +291,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
         };
         for (int s = d0; s < d1 && ok; ++s) {
             if (!(ok = warp_wait(bars + (kBarFree + st) * 8, phase, abort, p.wait_ns))) break;
-            const uint32_t full = bars + (kBarFull + st) * 8, x = ring + st * uint32_t(p.stage_bytes), a = x + kTok * 128;
+            const uint32_t full = bars + (kBarFull + st) * 8, x = ring + st * stage_bytes, a = x + x_bytes;
             if (lane == 0) {
-                mbar_expect_tx(full, bytes);
+                mbar_expect_tx(full, stage_bytes);
                 for (int i = 0; i < boxes; ++i) tma_2d(x + i * p.box * 128, &x_map, s * kDepth, t0 + i * p.box, full);
                 tma_3d(a, &a_map, s * kDepth, 0, j, full);
             }
             __syncwarp();
-            if (++st == uint32_t(p.stages)) st = 0, phase ^= 1u;
-            if (s - d0 == p.stages - 1)
+            if (++st == stages) st = 0, phase ^= 1u;
+            if (s - d0 == int(stages) - 1)
                 for (int i = 0; i < kBufs && c < row_chunks && ok; ++i) rows_of_b();
         }
         while (c < row_chunks && ok) rows_of_b();
@@ -296,10 +309,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
         const uint32_t idesc = p.idesc | uint32_t(p.rank16 >> 3) << 17;
         for (int s = d0; s < d1; ++s) {
             if (!(ok = warp_wait(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns))) break;
-            const uint32_t x = ring + st * uint32_t(p.stage_bytes);
+            const uint32_t x = ring + st * stage_bytes;   // (lanes without a token are whatever lies behind)
             const int depth = min(kDepth, p.n - s * kDepth);
             if (elect_one()) {
-                const uint64_t da = umma_desc_sw128(x), db = umma_desc_sw128(x + kTok * 128);
+                const uint64_t da = umma_desc_sw128(x), db = umma_desc_sw128(x + x_bytes);
 #pragma unroll
                 for (int k = 0; k < kDepth / 16; ++k) {
                     if (k * 16 >= depth) break;
@@ -309,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                 if (s + 1 == d1) umma_commit(bars + kBarV * 8);
             }
             __syncwarp();
-            if (++st == uint32_t(p.stages)) st = 0, phase ^= 1u;
+            if (++st == stages) st = 0, phase ^= 1u;
         }
         ok = ok && warp_wait(bars + kBarVIn * 8, 0, abort, p.wait_ns);
         uint32_t buf = 0, bphase = 0, set = 0, dphase = 1;
@@ -363,6 +376,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
         }
         const uint32_t mine = part + uint32_t(token * (p.rank16 + 4)) * 4;   // (rows 16 bytes off a multiple of the banks)
         if (blocks > 1) {
+            float most = 0.0f;
             for (int k = k0; k < k0 + half; k += 8) {
                 float v[8];
                 if (empty || lost) {
@@ -371,11 +385,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                 } else {
                     tmem_ld8(tmem + lanes + k, v);
                 }
+                if (XTYPE == FRX_F16) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
+                }
                 if (token < live) {
                     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mine + k * 4), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
                     asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mine + k * 4 + 16), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
                 }
             }
+            if (XTYPE == FRX_F16 && token < kTok) tok_max[side * kTok + token] = most;
             __syncwarp();
             if (lane < int(blocks)) mbar_arrive_peer(peer_addr(bars + kBarPart * 8, uint32_t(lane)));
             lost = !warp_wait_cluster(bars + kBarPart * 8, 0, abort, p.wait_ns) || lost;
@@ -385,10 +404,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = 0.0f;
                 if (token < live && !lost)
-                    for (uint32_t b = 0; b < blocks; ++b) {
-                        const uint32_t at = peer_addr(mine + k * 4, b);
-                        const float4 lo = ld_peer(at), hi = ld_peer(at + 16);
-                        v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w, v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+                    for (uint32_t b = 0; b < blocks; b += 4) {   // (2, 4 or 8 blocks) the loads of four at once: each takes half a microsecond
+                        float4 lo[4], hi[4];
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (b + i < blocks) {
+                                const uint32_t at = peer_addr(mine + k * 4, b + i);
+                                lo[i] = ld_peer(at);
+                                hi[i] = ld_peer(at + 16);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[0] += lo[i].x, v[1] += lo[i].y, v[2] += lo[i].z, v[3] += lo[i].w, v[4] += hi[i].x, v[5] += hi[i].y, v[6] += hi[i].z, v[7] += hi[i].w;
                     }
             } else {
                 tmem_ld8(tmem + lanes + k, v);   // (sums that nobody has finished, where the wait ran out: the outputs are NaN then)
@@ -397,17 +425,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
         const float scale = p.scale ? __ldcg(p.scale + j) : 1.0f;
         float up = 1.0f;
         if (XTYPE == FRX_F16) {
-            // the token's largest magnitude to [2^14, 2^15): pieces of float16 then hold every bit of the others that counts
+            // the token's largest magnitude (or, of a sum over blocks, that of the parts) to [2^14, 2^15): pieces of float16 then hold every bit of the others that counts
             float most = 0.0f;
-            for (int k = k0; k < k0 + half; k += 8) {
-                float v[8];
-                take8(k, v);
+            if (blocks > 1) {
+                if (token < live && !lost)
+                    for (uint32_t b = 0; b < blocks; ++b)
+                        most += fmaxf(ld_peer1(peer_addr(s0 + kTokMax + token * 4, b)), ld_peer1(peer_addr(s0 + kTokMax + (kTok + token) * 4, b)));
+            } else {
+                for (int k = k0; k < k0 + half; k += 8) {
+                    float v[8];
+                    take8(k, v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i] * scale));
+                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
+                }
+                if (token < kTok) tok_max[side * kTok + token] = most;
+                named_bar_sync(1, 32 * kWarpsEpi);
+                if (token < kTok) most = fmaxf(tok_max[token], tok_max[kTok + token]);
             }
-            if (token < kTok) tok_max[side * kTok + token] = most;
-            named_bar_sync(1, 32 * kWarpsEpi);
-            if (token < kTok) most = fmaxf(tok_max[token], tok_max[kTok + token]);
+            most *= fabsf(scale);
             const uint32_t e = __float_as_uint(most) >> 23;   // its exponent + 127
             // 2^(141 - e) and back, within what 32 bits hold; nothing for zeros, infinities and NaN
             const uint32_t f = e == 255u || most == 0.0f ? 127u : min(max(268u - e, 1u), 253u);
@@ -525,18 +560,15 @@ int launch_typed(Adapters& p, const CUtensorMap& x_map, const CUtensorMap& a_map
     if (rc != FRX_OK) return rc;
     const int chunks = p.rank16 > 64 ? 2 : 1;
     const int64_t requests = std::min(p.R, p.T), tiles = (p.T - requests) / kTok + requests;   // of any requests that do not overlap
-    // As many blocks a tile as run at the same time (two an SM, one where the rank is more than 64), and as many stages as that leaves room for.
+    // As many blocks a tile as run at the same time (two an SM, one where the rank is more than 64), and the stages have the room that is left.
     unsigned blocks = 8;
     while (blocks > 1 && tiles * blocks > int64_t(sm_count()) * (chunks == 1 ? 2 : 1)) blocks /= 2;
     if (tiles * blocks > 0x7fff0000) return fail(FRX_ERR_SHAPE, "adapters: %lld tiles", (long long)tiles);
-    p.stage_bytes = kTok * 128 + p.rank16 * 128;
     const int rest = kHead + kBufs * chunks * kPieceB + (blocks > 1 ? kTok * (p.rank16 + 4) * 4 : 0);
     static_assert(kHead + kBufs * kPieceB + kTok * 68 * 4 + std::max(kMinStages * (kTok + 64) * 128, 3 * kPieceV) <= kSmemTwo, "two blocks an SM up to a rank of 64");
     static_assert(kHead + kBufs * 2 * kPieceB + kTok * 132 * 4 + std::max(kMinStages * (kTok + 128) * 128, 3 * 2 * kPieceV) <= int(kSmemMost), "the largest rank");
-    p.stages = std::min(kMaxStages, ((chunks == 1 ? kSmemTwo : int(kSmemMost)) - rest) / p.stage_bytes);
-    p.ring_bytes = std::max(p.stages * p.stage_bytes, 3 * chunks * kPieceV);
-    // (more than a third of an SM's shared memory, whatever the rank: a third block would wait for tensor memory)
-    const size_t smem = std::max(size_t(rest + p.ring_bytes), size_t(78 * 1024));
+    p.ring_bytes = std::max(((chunks == 1 ? kSmemTwo : int(kSmemMost)) - rest) / 1024 * 1024, 3 * chunks * kPieceV);
+    const size_t smem = size_t(rest + p.ring_bytes);   // (about half of an SM's, or all of it: a third block would wait for tensor memory)
     p.wait_ns = wait_limit_ns();
     FRX_LAUNCH(kKGateUp, stream, launch_pdl_cluster(k_adapter<XTYPE, TYPE>, dim3(unsigned(tiles) * blocks), dim3(kThreads), smem, stream, blocks, p, x_map, a_map, b_map));
     FRX_CUDA(cudaGetLastError());
