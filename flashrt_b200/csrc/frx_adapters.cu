@@ -43,11 +43,6 @@ struct Adapters {
     int whole;                                  // y and out allow accesses of 32 bytes
 };
 
-__device__ __forceinline__ float4 ld_peer(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ float ld_peer1(uint32_t addr) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -367,17 +362,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
         };
 #pragma unroll
         for (int d = 0; d < kAhead; ++d) read_ahead(old[d], int(rank) + d * int(blocks));
-        // ---------------- v: a lane is a token, a warp has half of the rank
-        const int half = p.rank16 / 2, k0 = side * half;
+        // ---------------- v: a lane is a token, a warp has every second eight of the rank (every fourth of a sum over blocks, which any warp can read)
+        const int k0 = side * 8;
         const bool empty = d0 == d1;   // no part of the depth here
         if (!empty) {
             lost = !warp_wait(bars + kBarV * 8, 0, abort, p.wait_ns);
             tc_fence_after_sync();
         }
-        const uint32_t mine = part + uint32_t(token * (p.rank16 + 4)) * 4;   // (rows 16 bytes off a multiple of the banks)
+        const uint32_t mine = part + uint32_t(token) * 4;   // token after token: a warp's read of another block's shared memory is 128 bytes (as 16 bytes a lane it was 32 requests: 3 us for eight of the rank)
         if (blocks > 1) {
             float most = 0.0f;
-            for (int k = k0; k < k0 + half; k += 8) {
+            for (int k = k0; k < p.rank16; k += 16) {
                 float v[8];
                 if (empty || lost) {
 #pragma unroll
@@ -390,8 +385,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                     for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
                 }
                 if (token < live) {
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mine + k * 4), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mine + k * 4 + 16), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + uint32_t(k + i) * kTok * 4), "f"(v[i]) : "memory");
                 }
             }
             if (XTYPE == FRX_F16 && token < kTok) tok_max[side * kTok + token] = most;
@@ -399,24 +394,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
             if (lane < int(blocks)) mbar_arrive_peer(peer_addr(bars + kBarPart * 8, uint32_t(lane)));
             lost = !warp_wait_cluster(bars + kBarPart * 8, 0, abort, p.wait_ns) || lost;
         }
+        const int taken = blocks > 1 ? (quarter & 1) * 32 + lane : token, first_k = blocks > 1 ? k0 + (quarter >> 1) * 16 : k0, step_k = blocks > 1 ? 32 : 16;   // the lane's token, and its warp's part of the rank
         auto take8 = [&](int k, float (&v)[8]) {
             if (blocks > 1) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-                if (token < live && !lost)
+                if (taken < live && !lost)
                     for (uint32_t b = 0; b < blocks; b += 4) {   // (2, 4 or 8 blocks) the loads of four at once: each takes half a microsecond
-                        float4 lo[4], hi[4];
+                        float of[4][8];
 #pragma unroll
                         for (uint32_t i = 0; i < 4; ++i) {
-                            lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            if (b + i < blocks) {
-                                const uint32_t at = peer_addr(mine + k * 4, b + i);
-                                lo[i] = ld_peer(at);
-                                hi[i] = ld_peer(at + 16);
-                            }
+                            const uint32_t at = peer_addr(part + uint32_t(k * kTok + taken) * 4, min(b + i, blocks - 1));
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) of[i][c] = b + i < blocks ? ld_peer1(at + c * kTok * 4) : 0.0f;
                         }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[0] += lo[i].x, v[1] += lo[i].y, v[2] += lo[i].z, v[3] += lo[i].w, v[4] += hi[i].x, v[5] += hi[i].y, v[6] += hi[i].z, v[7] += hi[i].w;
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) v[c] += of[i][c];
                     }
             } else {
                 tmem_ld8(tmem + lanes + k, v);   // (sums that nobody has finished, where the wait ran out: the outputs are NaN then)
@@ -428,11 +423,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
             // the token's largest magnitude (or, of a sum over blocks, that of the parts) to [2^14, 2^15): pieces of float16 then hold every bit of the others that counts
             float most = 0.0f;
             if (blocks > 1) {
-                if (token < live && !lost)
+                if (taken < live && !lost)
                     for (uint32_t b = 0; b < blocks; ++b)
-                        most += fmaxf(ld_peer1(peer_addr(s0 + kTokMax + token * 4, b)), ld_peer1(peer_addr(s0 + kTokMax + (kTok + token) * 4, b)));
+                        most += fmaxf(ld_peer1(peer_addr(s0 + kTokMax + taken * 4, b)), ld_peer1(peer_addr(s0 + kTokMax + (kTok + taken) * 4, b)));
             } else {
-                for (int k = k0; k < k0 + half; k += 8) {
+                for (int k = first_k; k < p.rank16; k += step_k) {
                     float v[8];
                     take8(k, v);
 #pragma unroll
@@ -447,9 +442,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
             // 2^(141 - e) and back, within what 32 bits hold; nothing for zeros, infinities and NaN
             const uint32_t f = e == 255u || most == 0.0f ? 127u : min(max(268u - e, 1u), 253u);
             up = __uint_as_float(f << 23);
-            if (side == 0 && token < kTok) tok_scale[token] = __uint_as_float((254u - f) << 23);
+            if (side == 0 && token < kTok) tok_scale[taken] = __uint_as_float((254u - f) << 23);
         }
-        for (int k = k0; k < k0 + half; k += 8) {
+        for (int k = first_k; k < p.rank16; k += step_k) {
             float v[8];
             take8(k, v);
             uint32_t bits[3][4];
@@ -462,9 +457,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                     bits[q][i / 2] = i & 1 ? bits[q][i / 2] | b << 16 : b;
                 }
             }
-            const uint32_t at = ring + uint32_t(k >> 6) * kPieceV + uint32_t(token) * 128 + uint32_t(((k & 63) >> 3) ^ (token & 7)) * 16;   // (the 128-byte swizzle)
+            const uint32_t at = ring + uint32_t(k >> 6) * kPieceV + uint32_t(taken) * 128 + uint32_t(((k & 63) >> 3) ^ (taken & 7)) * 16;   // (the 128-byte swizzle)
 #pragma unroll
-            for (int q = 0; q < 6 && token < kTok; ++q)
+            for (int q = 0; q < 6 && taken < kTok; ++q)
                 asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (q % 3) * v_bytes + (q / 3) * kTok * 128), "r"(bits[q % 3][0]), "r"(bits[q % 3][1]), "r"(bits[q % 3][2]),
                              "r"(bits[q % 3][3])
                              : "memory");
@@ -564,9 +559,9 @@ int launch_typed(Adapters& p, const CUtensorMap& x_map, const CUtensorMap& a_map
     unsigned blocks = 8;
     while (blocks > 1 && tiles * blocks > int64_t(sm_count()) * (chunks == 1 ? 2 : 1)) blocks /= 2;
     if (tiles * blocks > 0x7fff0000) return fail(FRX_ERR_SHAPE, "adapters: %lld tiles", (long long)tiles);
-    const int rest = kHead + kBufs * chunks * kPieceB + (blocks > 1 ? kTok * (p.rank16 + 4) * 4 : 0);
-    static_assert(kHead + kBufs * kPieceB + kTok * 68 * 4 + std::max(kMinStages * (kTok + 64) * 128, 3 * kPieceV) <= kSmemTwo, "two blocks an SM up to a rank of 64");
-    static_assert(kHead + kBufs * 2 * kPieceB + kTok * 132 * 4 + std::max(kMinStages * (kTok + 128) * 128, 3 * 2 * kPieceV) <= int(kSmemMost), "the largest rank");
+    const int rest = kHead + kBufs * chunks * kPieceB + (blocks > 1 ? kTok * p.rank16 * 4 : 0);
+    static_assert(kHead + kBufs * kPieceB + kTok * 64 * 4 + std::max(kMinStages * (kTok + 64) * 128, 3 * kPieceV) <= kSmemTwo, "two blocks an SM up to a rank of 64");
+    static_assert(kHead + kBufs * 2 * kPieceB + kTok * 128 * 4 + std::max(kMinStages * (kTok + 128) * 128, 3 * 2 * kPieceV) <= int(kSmemMost), "the largest rank");
     p.ring_bytes = std::max(((chunks == 1 ? kSmemTwo : int(kSmemMost)) - rest) / 1024 * 1024, 3 * chunks * kPieceV);
     const size_t smem = size_t(rest + p.ring_bytes);   // (about half of an SM's, or all of it: a third block would wait for tensor memory)
     p.wait_ns = wait_limit_ns();
