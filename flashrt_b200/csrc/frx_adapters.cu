@@ -15,7 +15,7 @@ namespace {
 // A tile (64 tokens of a request) is the work of a cluster of up to eight blocks, as many as fit the GPU at once: they share the first product's depth, add their
 // parts up through one another's shared memory (in the order of the blocks), and share the second product's rows. y is read two steps (32 bits: one) ahead of the sums it is added
 // to, from before the first product on.
-constexpr int kTok = 64, kRows = 128, kDepth = 64;
+constexpr int kTok = 64, kRows = 128, kDepth = 64, kFewRank = 16;
 constexpr int kMaxStages = 10, kMinStages = 3, kBufs = 2;
 constexpr int kWarpsEpi = 8, kWarpLoad = 8, kWarpMma = 9, kThreads = 32 * 10;
 constexpr int kBarFull = 0, kBarFree = kBarFull + kMaxStages, kBarBFull = kBarFree + kMaxStages, kBarBFree = kBarBFull + kBufs, kBarDFull = kBarBFree + kBufs, kBarDFree = kBarDFull + 2,
@@ -33,14 +33,15 @@ struct Adapters {
     const int32_t* offsets;   // [R + 1]
     const int32_t* which;     // [R]
     const float* scale;       // [L] or null
-    const void* y;
+    const void *x, *a, *b, *y;
     void* out;
-    int64_t ldy, ldo;
+    int64_t ldx, lda, stride_a, ldb, stride_b, ldy, ldo;
     unsigned long long wait_ns;
     int T, R, L, n, rows, rank, rank16;   // rank16: the rank rounded up to 16
     int box, ring_bytes;                        // rows of a load of x; bytes of the first product's stages (v's pieces come to the same place)
     uint32_t idesc;
     int whole;                                  // y and out allow accesses of 32 bytes
+    int few;                                    // tiles of one token go without the tensor cores
 };
 
 __device__ __forceinline__ float ld_peer1(uint32_t addr) {
@@ -170,6 +171,148 @@ __device__ __forceinline__ void copy_rows(const void* from, int64_t ld_from, voi
     }
 }
 
+// an element of y, of which nothing is waited for here
+template <int TYPE>
+__device__ __forceinline__ void load_one_if(uint32_t& w, const void* p, bool on) {
+    if (TYPE == FRX_F32)
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u32 %0, [%1];\n\t}" : "+r"(w) : "l"(p), "r"(uint32_t(on)));
+    else
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u16 %0, [%1];\n\t}" : "+r"(w) : "l"(p), "r"(uint32_t(on)));
+}
+// eight 16-bit elements from p on, `count` of which are there (the others 0); p on a 16-byte boundary
+struct Eight {
+    uint4 v;
+    __device__ __forceinline__ void load(const uint16_t* p, int count, bool tails) {   // tails: whether there are counts between 0 and 8 at all
+        v = make_uint4(0u, 0u, 0u, 0u);
+        asm volatile(
+            "{\n\t.reg .pred q;\n\t"
+            "setp.ge.s32 q, %5, 8;\n\t"
+            "@q ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+            : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+            : "l"(p), "r"(count));
+        if (tails && count > 0 && count < 8) {
+            uint32_t w[4] = {};
+#pragma unroll
+            for (int i = 0; i < 7; ++i)
+                if (i < count) w[i / 2] |= uint32_t(p[i]) << (i % 2 * 16);
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    template <int XTYPE>
+    __device__ __forceinline__ void wide8(float (&f)[8]) const {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = wide<XTYPE>(w[i]);
+            f[2 * i + 1] = wide<XTYPE>(w[i] >> 16);
+        }
+    }
+};
+
+// A tile of one token and a rank of up to 16 by fused multiply-adds: the steps between are fewer than by way of the tensor cores, whose instructions take 128 lanes and 16 columns
+// whatever there is (64 users 12.9 -> 9.7 us, 256 31 -> 18; of a rank of 32 12.3 and 12.5, of 64 16 and 21: these stay there). First product: a warp has two rows of A_j, the lanes the columns
+// of this block's part of the depth. Second: two lanes have a row of B_j, eight of the rank each; its rows and y's elements are read four steps ahead, the
+// first before v is there.
+template <int XTYPE, int TYPE>
+__device__ __forceinline__ void one_token(const Adapters& p, uint32_t bars, uint32_t abort, float* part, uint32_t part_addr, float* v, int t0, int j, int c0, int c1, uint32_t rank, uint32_t blocks) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kWarps = kThreads / 32, kAhead = 4, size = TYPE == FRX_F32 ? 4 : 2;
+    const uint16_t* x = static_cast<const uint16_t*>(p.x) + int64_t(t0) * p.ldx;
+    const uint16_t* a = static_cast<const uint16_t*>(p.a) + int64_t(j) * p.stride_a;
+    const uint16_t* b = static_cast<const uint16_t*>(p.b) + int64_t(j) * p.stride_b;
+    static_assert(2 * kWarps >= kFewRank, "two rows a warp");
+    {
+        float acc[2] = {};
+        const bool first = warp < p.rank, second = warp + kWarps < p.rank, tails = p.n % 8 != 0;
+#pragma unroll 4
+        for (int c = c0 + lane * 8; c < c1; c += 256) {
+            const int count = min(8, c1 - c);
+            Eight av[2], xv;
+            av[0].load(a + int64_t(warp) * p.lda + c, first ? count : 0, tails);
+            av[1].load(a + int64_t(warp + kWarps) * p.lda + c, second ? count : 0, tails);
+            xv.load(x + c, count, tails);
+            float af[2][8], xf[8];
+            av[0].wide8<XTYPE>(af[0]);
+            av[1].wide8<XTYPE>(af[1]);
+            xv.wide8<XTYPE>(xf);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                acc[0] = fmaf(xf[i], af[0][i], acc[0]);
+                acc[1] = fmaf(xf[i], af[1][i], acc[1]);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
+            if (lane == 0 && (m ? second : first)) part[warp + m * kWarps] = acc[m];
+        }
+    }
+    constexpr int kPer = 16, kSteps = kRows / kPer;   // rows a warp's step; steps of a chunk of rows
+    const int q = lane & 1;
+    const int row_chunks = (p.rows + kRows - 1) / kRows, count = int(rank) < row_chunks ? ((row_chunks - 1 - int(rank)) / int(blocks) + 1) * kSteps : 0;   // steps of this block
+    auto row_of = [&](int i) { return (int(rank) + i / kSteps * int(blocks)) * kRows + i % kSteps * kPer + lane / 2; };
+    Eight bv[kAhead];
+    uint32_t yv[kAhead] = {};
+    auto read = [&](int m, int i) {
+        const int row = row_of(i);
+        const bool have = i < count && row < p.rows;
+        bv[m].load(b + int64_t(row) * p.ldb + q * 8, have ? min(8, p.rank - q * 8) : 0, p.rank % 8 != 0);
+        load_one_if<TYPE>(yv[m], static_cast<const uint8_t*>(p.y) + (t0 * p.ldy + row) * size, have && q == 0);
+    };
+#pragma unroll
+    for (int m = 0; m < kAhead; ++m) read(m, warp + m * kWarps);
+    __syncthreads();
+    bool ok = true;
+    if (blocks > 1) {
+        if (warp < kWarpsEpi && lane < int(blocks)) mbar_arrive_peer(peer_addr(bars + kBarPart * 8, uint32_t(lane)));
+        ok = warp_wait_cluster(bars + kBarPart * 8, 0, abort, p.wait_ns);
+    }
+    if (threadIdx.x < kFewRank) {
+        const int k = threadIdx.x;
+        float sum = 0.0f;
+        if (k < p.rank) {
+            if (blocks > 1) {
+                float of[8];
+#pragma unroll
+                for (uint32_t m = 0; m < 8; ++m) of[m] = m < blocks ? ld_peer1(peer_addr(part_addr + uint32_t(k) * 4, m)) : 0.0f;
+#pragma unroll
+                for (int m = 0; m < 8; ++m) sum += of[m];
+            } else {
+                sum = part[k];
+            }
+            sum *= p.scale ? __ldcg(p.scale + j) : 1.0f;
+        }
+        v[k] = sum;
+    }
+    __syncthreads();
+    ok = ok && lds32(abort) == 0;   // (whoever's wait ran out, its sums are everybody's)
+    float vf[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vf[i] = v[q * 8 + i];
+    for (int i0 = warp; i0 < count; i0 += kAhead * kWarps) {
+#pragma unroll
+        for (int m = 0; m < kAhead; ++m) {
+            const int i = i0 + m * kWarps, row = row_of(i);
+            float bf[8], sum = 0.0f;
+            bv[m].wide8<XTYPE>(bf);
+            const uint32_t old = yv[m];
+            read(m, i + kAhead * kWarps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = q * 8 + e < p.rank ? fmaf(bf[e], vf[e], sum) : sum;   // (nothing beyond the rank, were v infinite)
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            if (!ok) sum = __uint_as_float(0x7fffffffu);   // a wait ran out
+            if (i < count && row < p.rows && q == 0) {
+                uint8_t* to = static_cast<uint8_t*>(p.out) + (t0 * p.ldo + row) * size;
+                if (TYPE == FRX_F32)
+                    *reinterpret_cast<float*>(to) = sum + __uint_as_float(old);
+                else
+                    *reinterpret_cast<uint16_t*>(to) = uint16_t(narrow2<TYPE>(sum + wide<TYPE>(old), 0.0f));
+            }
+        }
+    }
+}
+
 template <int XTYPE, int TYPE>
 __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap a_map,
                                                          const __grid_constant__ CUtensorMap b_map) {
@@ -261,6 +404,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
     if (!work) {
         // no adapter: y as it is
         if (live > 0 && p.out != p.y) copy_rows<TYPE == FRX_F32 ? 4 : 2>(p.y, p.ldy, p.out, p.ldo, t0, live, p.rows, int(rank) * (kThreads / 32) + warp, int(blocks) * (kThreads / 32));
+    } else if (live == 1 && p.few) {
+        float* v = reinterpret_cast<float*>(smem + kHead + 32 * 1024);   // (the ring's room has 48 KB and more)
+        float* sums = reinterpret_cast<float*>(smem + (blocks > 1 ? part - s0 : uint32_t(kHead)));
+        const uint32_t sums_addr = blocks > 1 ? part : ring;
+        const int c0 = d0 * kDepth, c1 = min(p.n, d1 * kDepth);
+        one_token<XTYPE, TYPE>(p, bars, abort, sums, sums_addr, v, t0, j, c0, c1, rank, blocks);
     } else if (warp == kWarpLoad) {
         // ---------------- loads: the first product's stages, and this block's rows of B_j as soon as there is room
         uint32_t st = 0, phase = 1, buf = 0, bphase = 1;
@@ -605,6 +754,14 @@ extern "C" int frx_adapter_add(frx_stream_t stream, const void* x, int64_t ldx, 
     p.offsets = offsets;
     p.which = which;
     p.scale = scale;
+    p.x = x;
+    p.a = a;
+    p.b = b;
+    p.ldx = ldx;
+    p.lda = lda;
+    p.stride_a = stride_a;
+    p.ldb = ldb;
+    p.stride_b = stride_b;
     p.y = y;
     p.out = out;
     p.ldy = ldy;
@@ -617,6 +774,7 @@ extern "C" int frx_adapter_add(frx_stream_t stream, const void* x, int64_t ldx, 
     p.rank = rank;
     p.rank16 = (rank + 15) & ~15;
     p.box = T / R >= 64 ? 64 : 16;   // rows of a load: few where most requests have a token or two
+    p.few = p.rank16 == 16;
     p.idesc = f16_idesc(dtype, false, false);
     const int64_t size = dtype_size(y_dtype);
     p.whole = rows * size % 32 == 0 && aligned(y, 32) && aligned(out, 32) && ldy * size % 32 == 0 && ldo * size % 32 == 0;
