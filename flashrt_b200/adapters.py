@@ -20,16 +20,20 @@ def add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, offs
     if stream is not None and out is None:
         return _on(stream, add, y, x, a, b, offsets, which, scale=scale, out=out)
     _on_device(y, x, a, b, offsets, which, scale, out)
-    ldx, code = _matrix("x", x), _half("x", x)
-    T, n = x.shape
-    L, rank, _, lda, stride_a = _matrices("a", a, x.dtype)
-    rows = y.shape[-1]
-    ldy = _matrix("y", y, None, (T, rows))
-    if a.shape[2] != n or b.shape != (L, rows, rank):
-        raise FrxError(_l.ERR_ARG, f"adapters {tuple(a.shape)}, {tuple(b.shape)} for rows of {n} values and results of {rows}: [L][rank][n] and [L][rows][rank] are wanted")
-    _, _, _, ldb, stride_b = _matrices("b", b, x.dtype)
+    code = _half("x", x)
+    try:
+        (T, n), (L, rank, columns), (count, rows, inner) = x.shape, a.shape, b.shape
+    except ValueError:
+        raise FrxError(_l.ERR_ARG, f"x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)}: [T][n], [L][rank][n] and [L][rows][rank] are wanted") from None
+    if columns != n or count != L or inner != rank or y.shape != (T, rows):
+        raise FrxError(_l.ERR_ARG, f"adapters {tuple(a.shape)}, {tuple(b.shape)} for rows of {n} values and results {tuple(y.shape)}: [L][rank][n], [L][rows][rank] and [T][rows] are wanted")
+    if a.dtype != x.dtype or b.dtype != x.dtype:
+        raise FrxError(_l.ERR_ARG, f"adapters of {a.dtype} and {b.dtype} for rows of {x.dtype}")
+    ldx, ldy = _matrix("x", x), _matrix("y", y)
+    lda, stride_a = (n, rank * n) if a.is_contiguous() else _matrices("a", a)[3:]
+    ldb, stride_b = (rank, rows * rank) if b.is_contiguous() else _matrices("b", b)[3:]
     R = which.numel()
-    _typed("which", which, torch.int32, (R,))
+    _typed("which", which, torch.int32)
     _typed("offsets", offsets, torch.int32, (R + 1,))
     if scale is not None:
         _typed("scale", scale, torch.float32, (L,))

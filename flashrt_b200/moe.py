@@ -290,7 +290,9 @@ def _matrix(name: str, t: torch.Tensor, dtype=None, shape=None) -> int:
     size = t.shape
     if len(size) != 2 or t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype) or (shape is not None and size != shape):
         raise FrxError(_l.ERR_ARG, f"{name}: rows of {'float32, bfloat16 or float16' if dtype is None else dtype}{'' if shape is None else f', {tuple(shape)},'} are wanted")
-    if size[0] <= 1 or t.is_contiguous():
+    if t.is_contiguous():
+        return size[1]
+    if size[0] <= 1:
         if size[1] <= 1 or t.stride(1) == 1:
             return size[1]
     elif (size[1] <= 1 or t.stride(1) == 1) and t.stride(0) >= size[1]:
