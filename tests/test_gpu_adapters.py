@@ -263,6 +263,32 @@ def test_adapters_in_the_order_of_a_sort():
     assert ((back.double().cpu() - want).abs() <= tol)[live].all()
 
 
+@pytest.mark.parametrize("lengths,rank", [([1], 8), ([3], 16), ([40, 1, 30], 64)])
+def test_a_wait_that_runs_out_leaves_nan(lengths, rank):
+    """A row of half a million values keeps the rest of a tile waiting, and the other blocks of its cluster; with a limit of one microsecond (a token alone is quick) it gives up. Nothing
+    hangs, no wrong number is left, and the next call is as if nothing had been."""
+    T, n, rows = sum(lengths), 1 << 19, 400
+    g = gen(3)
+    x, a = torch.randn(T, n, generator=g).to(BF16).cuda(), (torch.randn(3, rank, n, generator=g) / n ** 0.5).to(BF16).cuda()
+    b, y = torch.randn(3, rows, rank, generator=g).to(BF16).cuda(), torch.randn(T, rows, generator=g).cuda()
+    offsets = torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+    which = torch.arange(len(lengths), dtype=torch.int32, device="cuda")
+    want = adapters.add(y, x, a, b, offsets, which)
+    torch.cuda.synchronize()
+    lost = torch.zeros_like(y, dtype=torch.bool)
+    try:
+        L.check(L.lib.frx_debug_set_wait_limit_ns(1_000))
+        for _ in range(5):
+            got = adapters.add(y, x, a, b, offsets, which)
+            torch.cuda.synchronize()
+            lost |= got.isnan()
+            assert bool((got.isnan() | (got == want)).all())
+    finally:
+        L.check(L.lib.frx_debug_set_wait_limit_ns(0))
+    assert bool(lost.any()) or lengths == [1], "no wait ran out"
+    assert torch.equal(adapters.add(y, x, a, b, offsets, which), want)
+
+
 def test_refusals():
     c = Case([2, 3], 64, 32, 16)
     y, x, a, b, offsets, which = c.args()
