@@ -43,6 +43,7 @@ struct Product {
     int stages, stage_bytes;
     int most;                 // tiles of any plan whose experts' rows do not overlap
     uint32_t idesc;           // the instruction descriptor without N
+    int run;                  // stages whose products are summed by the tensor cores
     int add;                  // third form: added to what is there
 };
 
@@ -271,67 +272,83 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
         bool ok = rank == 0;
         while (ok && t.next(p)) {
             const uint32_t idesc = p.idesc | uint32_t(t.width >> 3) << 17;
-            if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
-            tc_fence_after_sync();   // behind the epilogues' loads of these accumulators
-            const uint32_t acc = tmem + set * kTileN;
-            for (int s = 0; s < t.steps; ++s) {
-                if (!(ok = warp_wait_cluster(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns))) break;
-                const uint32_t a = stages0 + st * stage_bytes, b = a + kStageA;
-                const int depth = s + 1 < t.steps ? kDepth : t.last;
-                if (elect_one()) {
-                    const uint64_t da = FORM == kForward ? umma_desc_sw128(a) : umma_desc_mn(a), db = FORM == kGradW ? umma_desc_mn(b) : umma_desc_sw128(b);
-                    constexpr uint64_t kStepK = 32 >> 4, kStepMn = 16 * 128 >> 4;   // 16 of depth
+            for (int first = 0; first == 0 || first < t.steps; first += p.run) {   // (an expert without rows has one run of nothing)
+                if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
+                tc_fence_after_sync();   // behind the epilogues' loads of these accumulators
+                const uint32_t acc = tmem + set * kTileN;
+                const int end = min(t.steps, first + p.run);
+                for (int s = first; s < end; ++s) {
+                    if (!(ok = warp_wait_cluster(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns))) break;
+                    const uint32_t a = stages0 + st * stage_bytes, b = a + kStageA;
+                    const int depth = s + 1 < t.steps ? kDepth : t.last;
+                    if (elect_one()) {
+                        const uint64_t da = FORM == kForward ? umma_desc_sw128(a) : umma_desc_mn(a), db = FORM == kGradW ? umma_desc_mn(b) : umma_desc_sw128(b);
+                        constexpr uint64_t kStepK = 32 >> 4, kStepMn = 16 * 128 >> 4;   // 16 of depth
 #pragma unroll
-                    for (int k = 0; k < kDepth / 16; ++k) {
-                        if (k * 16 >= depth) break;
-                        umma_f16_pair(acc, da + k * (FORM == kForward ? kStepK : kStepMn), db + k * (FORM == kGradW ? kStepMn : kStepK), idesc, s + k > 0);
+                        for (int k = 0; k < kDepth / 16; ++k) {
+                            if (k * 16 >= depth) break;
+                            umma_f16_pair(acc, da + k * (FORM == kForward ? kStepK : kStepMn), db + k * (FORM == kGradW ? kStepMn : kStepK), idesc, s - first + k > 0);
+                        }
+                        umma_commit_pair(bars + (kBarFree + st) * 8);
                     }
-                    umma_commit_pair(bars + (kBarFree + st) * 8);
+                    __syncwarp();
+                    if (++st == n_stages) st = 0, phase ^= 1u;
                 }
+                if (!ok) break;
+                if (elect_one()) umma_commit_pair(bars + (kBarDFull + set) * 8);
                 __syncwarp();
-                if (++st == n_stages) st = 0, phase ^= 1u;
+                set ^= 1u;
+                if (set == 0) dphase ^= 1u;
             }
-            if (ok && elect_one()) umma_commit_pair(bars + (kBarDFull + set) * 8);
-            __syncwarp();
-            set ^= 1u;
-            if (set == 0) dphase ^= 1u;
         }
     } else {
-        // ---------------- epilogue: a warp has a quarter of the lanes and every second 16 columns
+        // ---------------- epilogue: a warp has a quarter of the lanes and every second 16 columns, whose sums it keeps in registers
         const int quarter = warp & 3, part = warp >> 2, m = quarter * 32 + lane;
-        constexpr int size = TYPE == FRX_F32 ? 4 : 2;
+        constexpr int size = TYPE == FRX_F32 ? 4 : 2, kSixteens = kTileN / 32;
         uint32_t set = 0, phase = 0;
         const bool pairs = TYPE != FRX_F32 && p.lanes % 2 == 0 && p.ldy % 2 == 0 && (FORM != kGradW || p.ldye % 2 == 0) && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
         bool lost = false;   // a wait ran out: NaN, not a wrong number, and no more waits
         while (t.next(p)) {
-            lost = lost || !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);
-            tc_fence_after_sync();
-            const uint32_t acc = tmem + (uint32_t(quarter * 32) << 16) + set * kTileN;
+            uint32_t sums[kSixteens][2][8] = {};
+            for (int first = 0; first == 0 || first < t.steps; first += p.run) {
+                lost = lost || !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);
+                tc_fence_after_sync();
+                const uint32_t acc = tmem + (uint32_t(quarter * 32) << 16) + set * kTileN;
+#pragma unroll
+                for (int c = 0; c < kSixteens; ++c)
+                    if (c * 32 + part * 16 < t.width && t.steps && !lost) {
+                        uint32_t v[2][8];
+                        tmem_ld16(acc + c * 32 + part * 16, v);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sums[c][i / 8][i % 8] = __float_as_uint(__uint_as_float(sums[c][i / 8][i % 8]) + __uint_as_float(v[i / 8][i % 8]));
+                    }
+                if (!lost) {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_peer(bars_first + (kBarDFree + set) * 8);
+                }
+                set ^= 1u;
+                if (set == 0) phase ^= 1u;
+            }
             const int at_lane = t.lane0 + int(rank) * kLanes + m;
-            const bool have = at_lane < p.lanes, empty = FORM == kGradW && t.steps == 0;
+            const bool have = at_lane < p.lanes;
+            if (FORM == kGradW && p.add && t.steps == 0 && !lost) continue;
             uint8_t* y = static_cast<uint8_t*>(p.y) + ((FORM == kGradW ? t.e * p.ldye : 0) + t.col0 * p.ldy + at_lane) * size;
-            for (int c = part * 16; c < t.width && !(empty && p.add); c += 32) {
-                uint32_t v[2][8];
-                if (lost || empty) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[0][i] = v[1][i] = lost ? 0x7fffffffu : 0u;
-                } else {
-                    tmem_ld16(acc + c, v);
-                }
+            for (int c = 0; c < kSixteens; ++c)
+                if (c * 32 + part * 16 < t.width) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint8_t* at = y + (c + 8 * h) * p.ldy * size;
-                    if (FORM == kGradW && p.add) add8<TYPE>(v[h], at, p.ldy, t.live - c - 8 * h, have);
-                    store8<TYPE>(v[h], at, p.ldy, t.live - c - 8 * h, have, pairs);
+                    for (int h = 0; h < 2; ++h) {
+                        const int col = c * 32 + part * 16 + 8 * h;
+                        uint8_t* at = y + col * p.ldy * size;
+                        if (lost) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) sums[c][h][i] = 0x7fffffffu;
+                        }
+                        if (FORM == kGradW && p.add) add8<TYPE>(sums[c][h], at, p.ldy, t.live - col, have);
+                        store8<TYPE>(sums[c][h], at, p.ldy, t.live - col, have, pairs);
+                    }
                 }
-            }
-            if (!lost) {
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_peer(bars_first + (kBarDFree + set) * 8);
-            }
-            set ^= 1u;
-            if (set == 0) phase ^= 1u;
         }
     }
     tc_fence_before_sync();
@@ -359,6 +376,10 @@ int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& co
     p.most = int(most);
     p.stages = int(std::min<size_t>(kMaxStages, (kSmemMost - kHead - tables) / size_t(p.stage_bytes)));
     static_assert((kSmemMost - kHead - 4096 * 16) / (kStageA + kTileN / 2 * kDepth * 2) >= 4, "stages beside the tables of 4096 experts");
+    // The tensor cores add to their sums by cutting off, half a step of 2^-23 of the sum so far on average and always towards zero: 128 additions (2,048 of depth) leave 2.1e-6 of a result. What
+    // is returned in 32 bits they sum over 256 of depth at a time, which the epilogue adds up rounded to nearest (1e-7, as a plain sum in 32 bits); 16 bits round by 2^-9 and 2^-12
+    // themselves, there it is 8,192.
+    p.run = TYPE == FRX_F32 ? 4 : 128;
     p.wait_ns = wait_limit_ns();
     const unsigned pairs = unsigned(std::min<int64_t>(std::max(1, sm_count() / 2), std::max<int64_t>(1, most)));
     FRX_LAUNCH(kKGateUp, stream,
