@@ -399,6 +399,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
     // A stage is the tokens' rows of x, as many as the loads bring, and A_j's: of one token 4 KB instead of 10 at a rank of 16, so that most of its depth is in flight at once.
     const int boxes = (live + p.box - 1) / p.box;
     const uint32_t x_bytes = uint32_t(boxes * p.box) * 128, stage_bytes = x_bytes + uint32_t(p.rank16) * 128, stages = min(uint32_t(kMaxStages), uint32_t(p.ring_bytes) / max(stage_bytes, 1u));
+    // The tensor cores add to their sums by cutting off (half a step of 2^-23 each time on average, towards zero): the first product's depth goes into several sums, some 256 of it each as far as
+    // tensor memory has room, which are added up rounded to nearest; of the second product's pieces the smallest come first.
+    const int room = kCols / p.rank16, part_depths = max(4, (d1 - d0 + min(room, 8) - 1) / min(room, 8)), parts = (d1 - d0 + part_depths - 1) / part_depths;
     bool lost = false;
 
     if (!work) {
@@ -454,13 +457,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
         for (int s = d0; s < d1; ++s) {
             if (!(ok = warp_wait(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns))) break;
             const uint32_t x = ring + st * stage_bytes;   // (lanes without a token are whatever lies behind)
-            const int depth = min(kDepth, p.n - s * kDepth);
+            const int depth = min(kDepth, p.n - s * kDepth), in_part = (s - d0) % part_depths;
+            const uint32_t acc = tmem + uint32_t((s - d0) / part_depths * p.rank16);
             if (elect_one()) {
                 const uint64_t da = umma_desc_sw128(x), db = umma_desc_sw128(x + x_bytes);
 #pragma unroll
                 for (int k = 0; k < kDepth / 16; ++k) {
                     if (k * 16 >= depth) break;
-                    umma_f16(tmem, da + k * 2, db + k * 2, idesc, s + k > d0);
+                    umma_f16(acc, da + k * 2, db + k * 2, idesc, in_part + k > 0);
                 }
                 umma_commit(bars + (kBarFree + st) * 8);
                 if (s + 1 == d1) umma_commit(bars + kBarV * 8);
@@ -476,11 +480,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
             if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
             tc_fence_after_sync();
             if (elect_one()) {
-                for (int q = 0; q < 3; ++q)
+                for (int q = 2; q >= 0; --q)
                     for (int k = 0; k < p.rank16; k += 16) {
                         const uint32_t in = uint32_t(k & 63) * 2;
                         umma_f16(tmem + set * kRows, umma_desc_sw128(ring + q * v_bytes + uint32_t(k >> 6) * kPieceV) + (in >> 4),
-                                 umma_desc_sw128(bbuf + buf * bbuf_bytes + uint32_t(k >> 6) * kPieceB) + (in >> 4), id, q + k > 0);
+                                 umma_desc_sw128(bbuf + buf * bbuf_bytes + uint32_t(k >> 6) * kPieceB) + (in >> 4), id, q < 2 || k > 0);
                     }
                 umma_commit(bars + (kBarBFree + buf) * 8);
                 umma_commit(bars + (kBarDFull + set) * 8);
@@ -519,6 +523,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
             tc_fence_after_sync();
         }
         const uint32_t mine = part + uint32_t(token) * 4;   // token after token: a warp's read of another block's shared memory is 128 bytes (as 16 bytes a lane it was 32 requests: 3 us for eight of the rank)
+        auto sum_parts = [&](int k, float (&v)[8]) {
+            tmem_ld8(tmem + lanes + k, v);
+            for (int g = 1; g < parts; ++g) {
+                float more[8];
+                tmem_ld8(tmem + lanes + g * p.rank16 + k, more);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] += more[i];
+            }
+        };
         if (blocks > 1) {
             float most = 0.0f;
             for (int k = k0; k < p.rank16; k += 16) {
@@ -527,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = lost ? __uint_as_float(0x7fffffffu) : 0.0f;
                 } else {
-                    tmem_ld8(tmem + lanes + k, v);
+                    sum_parts(k, v);
                 }
                 if (XTYPE == FRX_F16) {
 #pragma unroll
@@ -563,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                             for (int c = 0; c < 8; ++c) v[c] += of[i][c];
                     }
             } else {
-                tmem_ld8(tmem + lanes + k, v);   // (sums that nobody has finished, where the wait ran out: the outputs are NaN then)
+                sum_parts(k, v);   // (sums that nobody has finished, where the wait ran out: the outputs are NaN then)
             }
         };
         const float scale = p.scale ? __ldcg(p.scale + j) : 1.0f;

@@ -24,9 +24,9 @@ enum Form { kForward, kGradX, kGradW };
 
 constexpr int kTileM = 256, kLanes = 128, kDepth = 64, kTileN = 256, kUnitN = 32;   // lanes of a tile, of a block; columns of a tile at most, what they are a multiple of
 constexpr int kStageA = kLanes * kDepth * 2, kChunk = 64 * kDepth * 2;   // bytes of a stage's lanes side; of 64 contiguous elements x 64 of an MN-major side
-constexpr int kMaxStages = 10;
+constexpr int kMaxStages = 10, kMaxSets = 8;
 constexpr int kWarpsEpi = 8, kWarpLoad = 8, kWarpMma = 9, kWarpTail = 10, kThreads = 32 * 11;
-constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + 2, kBarTail = kBarDFree + 2, kBarTailPeer = kBarTail + kMaxStages, kBars = kBarTailPeer + kMaxStages;
+constexpr int kBarFull = 0, kBarFree = kMaxStages, kBarDFull = 2 * kMaxStages, kBarDFree = kBarDFull + kMaxSets, kBarTail = kBarDFree + kMaxSets, kBarTailPeer = kBarTail + kMaxStages, kBars = kBarTailPeer + kMaxStages;
 constexpr int kAbort = 512, kSlot = 516, kSums = 640, kHead = 1024;
 static_assert(kBars * 8 <= kAbort && kSums + 8 * kThreads / 32 <= kHead, "the block's head");
 
@@ -44,6 +44,7 @@ struct Product {
     int most;                 // tiles of any plan whose experts' rows do not overlap
     uint32_t idesc;           // the instruction descriptor without N
     int run;                  // stages whose products are summed by the tensor cores
+    int sets;                 // of accumulators, `width` columns each
     int add;                  // third form: added to what is there
 };
 
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
             mbar_init(b + kBarTail + i, 1);
             mbar_init(b + kBarTailPeer + i, 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kMaxSets; ++i) {
             mbar_init(b + kBarDFull + i, 1);
             mbar_init(b + kBarDFree + i, 2 * kWarpsEpi);
         }
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
             for (int first = 0; first == 0 || first < t.steps; first += p.run) {   // (an expert without rows has one run of nothing)
                 if (!(ok = warp_wait(bars + (kBarDFree + set) * 8, dphase, abort, p.wait_ns))) break;
                 tc_fence_after_sync();   // behind the epilogues' loads of these accumulators
-                const uint32_t acc = tmem + set * kTileN;
+                const uint32_t acc = tmem + set * uint32_t(p.width);
                 const int end = min(t.steps, first + p.run);
                 for (int s = first; s < end; ++s) {
                     if (!(ok = warp_wait_cluster(bars + (kBarFull + st) * 8, phase, abort, p.wait_ns))) break;
@@ -297,8 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
                 if (!ok) break;
                 if (elect_one()) umma_commit_pair(bars + (kBarDFull + set) * 8);
                 __syncwarp();
-                set ^= 1u;
-                if (set == 0) dphase ^= 1u;
+                if (++set == uint32_t(p.sets)) set = 0, dphase ^= 1u;
             }
         }
     } else {
@@ -308,47 +308,63 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
         uint32_t set = 0, phase = 0;
         const bool pairs = TYPE != FRX_F32 && p.lanes % 2 == 0 && p.ldy % 2 == 0 && (FORM != kGradW || p.ldye % 2 == 0) && reinterpret_cast<uintptr_t>(p.y) % 4 == 0;
         bool lost = false;   // a wait ran out: NaN, not a wrong number, and no more waits
+        // a run's sums are there; they have been read
+        auto wait_for_sums = [&]() {
+            lost = lost || !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);
+            tc_fence_after_sync();
+            return tmem + (uint32_t(quarter * 32) << 16) + set * uint32_t(p.width);
+        };
+        auto give_back = [&]() {
+            if (!lost) {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_peer_relaxed(bars_first + (kBarDFree + set) * 8);   // (tensor memory alone has been read: nothing of memory to wait for)
+            }
+            if (++set == uint32_t(p.sets)) set = 0, phase ^= 1u;
+        };
         while (t.next(p)) {
+            const int at_lane = t.lane0 + int(rank) * kLanes + m;
+            const bool have = at_lane < p.lanes;
+            uint8_t* y = static_cast<uint8_t*>(p.y) + ((FORM == kGradW ? t.e * p.ldye : 0) + t.col0 * p.ldy + at_lane) * size;
+            auto store16 = [&](uint32_t (&v)[2][8], int c) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint8_t* at = y + (c + 8 * h) * p.ldy * size;
+                    if (lost) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[h][i] = 0x7fffffffu;
+                    }
+                    if (FORM == kGradW && p.add) add8<TYPE>(v[h], at, p.ldy, t.live - c - 8 * h, have);
+                    store8<TYPE>(v[h], at, p.ldy, t.live - c - 8 * h, have, pairs);
+                }
+            };
+            if (t.steps <= p.run) {   // one run: from tensor memory to y
+                const uint32_t acc = wait_for_sums();
+                const bool empty = FORM == kGradW && t.steps == 0;
+                for (int c = part * 16; c < t.width && !(empty && p.add && !lost); c += 32) {
+                    uint32_t v[2][8] = {};
+                    if (!lost && !empty) tmem_ld16(acc + c, v);
+                    store16(v, c);
+                }
+                give_back();
+                continue;
+            }
             uint32_t sums[kSixteens][2][8] = {};
-            for (int first = 0; first == 0 || first < t.steps; first += p.run) {
-                lost = lost || !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);
-                tc_fence_after_sync();
-                const uint32_t acc = tmem + (uint32_t(quarter * 32) << 16) + set * kTileN;
+            for (int first = 0; first < t.steps; first += p.run) {
+                const uint32_t acc = wait_for_sums();
 #pragma unroll
                 for (int c = 0; c < kSixteens; ++c)
-                    if (c * 32 + part * 16 < t.width && t.steps && !lost) {
+                    if (c * 32 + part * 16 < t.width && !lost) {
                         uint32_t v[2][8];
                         tmem_ld16(acc + c * 32 + part * 16, v);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) sums[c][i / 8][i % 8] = __float_as_uint(__uint_as_float(sums[c][i / 8][i % 8]) + __uint_as_float(v[i / 8][i % 8]));
                     }
-                if (!lost) {
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_peer(bars_first + (kBarDFree + set) * 8);
-                }
-                set ^= 1u;
-                if (set == 0) phase ^= 1u;
+                give_back();
             }
-            const int at_lane = t.lane0 + int(rank) * kLanes + m;
-            const bool have = at_lane < p.lanes;
-            if (FORM == kGradW && p.add && t.steps == 0 && !lost) continue;
-            uint8_t* y = static_cast<uint8_t*>(p.y) + ((FORM == kGradW ? t.e * p.ldye : 0) + t.col0 * p.ldy + at_lane) * size;
 #pragma unroll
             for (int c = 0; c < kSixteens; ++c)
-                if (c * 32 + part * 16 < t.width) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int col = c * 32 + part * 16 + 8 * h;
-                        uint8_t* at = y + col * p.ldy * size;
-                        if (lost) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) sums[c][h][i] = 0x7fffffffu;
-                        }
-                        if (FORM == kGradW && p.add) add8<TYPE>(sums[c][h], at, p.ldy, t.live - col, have);
-                        store8<TYPE>(sums[c][h], at, p.ldy, t.live - col, have, pairs);
-                    }
-                }
+                if (c * 32 + part * 16 < t.width) store16(sums[c], c * 32 + part * 16);
         }
     }
     tc_fence_before_sync();
@@ -376,10 +392,12 @@ int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& co
     p.most = int(most);
     p.stages = int(std::min<size_t>(kMaxStages, (kSmemMost - kHead - tables) / size_t(p.stage_bytes)));
     static_assert((kSmemMost - kHead - 4096 * 16) / (kStageA + kTileN / 2 * kDepth * 2) >= 4, "stages beside the tables of 4096 experts");
-    // The tensor cores add to their sums by cutting off, half a step of 2^-23 of the sum so far on average and always towards zero: 128 additions (2,048 of depth) leave 2.1e-6 of a result. What
-    // is returned in 32 bits they sum over 256 of depth at a time, which the epilogue adds up rounded to nearest (1e-7, as a plain sum in 32 bits); 16 bits round by 2^-9 and 2^-12
-    // themselves, there it is 8,192.
+    // The tensor cores add to their sums by cutting off, half a step of 2^-23 of the sum so far on average and always towards zero: 128 additions (2,048 of depth) leave a relative error of
+    // 2.1e-6 in the root mean square. What is returned in 32 bits they sum over 256 of depth at a time, which the epilogue adds up rounded to nearest: 2.4e-7 (over 512 4.7e-7; a plain sum in 32
+    // bits leaves 1e-7). It costs nothing where matrices are the traffic, and a tenth where the tensor cores are busy (131,072 rows of 2,048 by 1,024 523 instead of 469 us). 16 bits round by
+    // 2^-9 and 2^-12 themselves: there it is 8,192 of depth.
     p.run = TYPE == FRX_F32 ? 4 : 128;
+    p.sets = std::min(kMaxSets, 512 / p.width);
     p.wait_ns = wait_limit_ns();
     const unsigned pairs = unsigned(std::min<int64_t>(std::max(1, sm_count() / 2), std::max<int64_t>(1, most)));
     FRX_LAUNCH(kKGateUp, stream,

@@ -181,6 +181,7 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
     return r;
 }
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t addr) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory"); }
+__device__ __forceinline__ void mbar_arrive_peer_relaxed(uint32_t addr) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory"); }
 // warp_wait for what other blocks of the cluster have written
 __device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity, uint32_t abort, uint64_t limit_ns) {
     if (!warp_wait(bar, parity, abort, limit_ns)) return false;
