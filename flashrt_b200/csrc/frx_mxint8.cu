@@ -1,6 +1,7 @@
 // MXINT8: activations kept in 8 bits for a backward pass. Rows to 8 bits and back, SwiGLU that keeps its gate and up rows in 8 bits in the same pass, and its
 // gradient from what was kept (frx_mxint8_* in frx.h).
 #include <algorithm>
+#include <type_traits>
 
 #include "frx_mx.cuh"
 #include "frx_rows.cuh"
@@ -29,34 +30,60 @@ __device__ __forceinline__ void put8(T* p, const float (&f)[kPer]) {
     }
 }
 
-// A quarter of a block of 32 to its codes; the block's four lanes get the scale byte, the exponent field of its largest magnitude (0 for a subnormal one: 2^-127), 255 where
-// there is a NaN or an infinity. v / 2^e is exact wherever the code is not 0 (v * 2^-e falls below 2^-126 only far below half a step), and so is the multiplication by 64: one rounding.
-__device__ __forceinline__ uint2 codes8(const float (&f)[kPer], uint32_t& byte) {
-    uint32_t amax = 0;
+// The bits of the largest magnitude of a thread's values as a 32-bit float, infinity above all numbers and NaN above that. Pairs of 16-bit elements are compared as they are.
+template <class T>
+__device__ __forceinline__ uint32_t largest(const T (&v)[kPer]) {
+    if constexpr (sizeof(T) == 4) {
+        uint32_t amax = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) amax = max(amax, __float_as_uint(f[j]) & 0x7fffffffu);   // (the bits of magnitudes are in their order, infinity and NaN on top)
+        for (int j = 0; j < kPer; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+        return amax;
+    } else {
+        using Two = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+        const Two* two = reinterpret_cast<const Two*>(v);
+        Two top = __habs2(two[0]);
+#pragma unroll
+        for (int j = 1; j < kPer / 2; ++j) top = __hmax2_nan(top, __habs2(two[j]));
+        return __float_as_uint(to_float(__hmax_nan(top.x, top.y))) & 0x7fffffffu;
+    }
+}
+
+// A quarter of a block of 32 to its codes; amax: `largest` of the quarter. The block's four lanes get the scale byte, the exponent field of its largest magnitude (0 for a subnormal one:
+// 2^-127), 255 where there is a NaN or an infinity. One rounding: the value times 2^(6 - e), plus 1.5 * 2^23, is rounded to an integer, ties to even, in one fused step, and the code is its low
+// byte (the conversion instructions have a quarter of the rate). A magnitude beyond 127.5 steps gives 128, the byte 0x80, which no other value has: these few are formed again, within +-127.
+__device__ __forceinline__ uint2 codes8(const float (&f)[kPer], uint32_t amax, uint32_t& byte) {
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     byte = amax >> 23;
     if (byte == 255u) return make_uint2(0u, 0u);
-    const float inv = byte == 254u ? __uint_as_float(0x00400000u) : __uint_as_float((254u - byte) << 23);   // 2^(127 - byte)
-    int q[kPer];
+    constexpr float kRound = 12582912.0f;   // 1.5 * 2^23
+    const float inv = __uint_as_float((260u - max(byte, 6u)) << 23);   // 2^(133 - byte), which 32 bits hold from a byte of 6 on
+    float v[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) q[j] = min(max(__float2int_rn(f[j] * inv * 64.0f), -127), 127);
+    for (int j = 0; j < kPer; ++j) v[j] = fmaf(f[j], inv, kRound);
     auto word = [&](int j) {
-        return uint32_t(__byte_perm(__byte_perm(uint32_t(q[j]), uint32_t(q[j + 1]), 0x0040), __byte_perm(uint32_t(q[j + 2]), uint32_t(q[j + 3]), 0x0040), 0x5410));
+        return __byte_perm(__byte_perm(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), 0x0040), __byte_perm(__float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]), 0x0040), 0x5410);
     };
-    return make_uint2(word(0), word(4));
+    uint2 w = make_uint2(word(0), word(4));
+    auto minus128 = [](uint32_t x) { return x & ~((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) & 0x80808080u; };   // a byte's top bit where the byte is 0x80
+    if (byte < 6u || (minus128(w.x) | minus128(w.y)) != 0) {
+        const float two = byte < 6u ? __uint_as_float((254u - byte) << 23) : 1.0f, one = byte < 6u ? 64.0f : inv;   // (two exact steps for a scale of the lowest ones)
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) v[j] = fminf(fmaxf(fmaf(f[j] * two, one, kRound), kRound - 127.0f), kRound + 127.0f);
+        w = make_uint2(word(0), word(4));
+    }
+    return w;
 }
 // and back: q * 2^(byte - 133), exact
 __device__ __forceinline__ void values8(uint2 codes, uint32_t byte, float (&f)[kPer]) {
-    const float s = mx_scale(byte);
+    const float s = mx_scale(byte) * 0.015625f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) f[j] = float(int8_t((j < 4 ? codes.x : codes.y) >> (8 * (j & 3)))) * 0.015625f * s;
+    for (int j = 0; j < kPer; ++j) f[j] = float(int8_t((j < 4 ? codes.x : codes.y) >> (8 * (j & 3)))) * s;
 }
 
 // s = 1 / (1 + exp(-g)) and c = 1 - s, neither by a difference. For 16-bit results the hardware's exponential and reciprocal: relative errors of 2^-22 + |g| 1.25 * 2^-24 and 2^-23; 0 where exp(-|g|)
-// is below 2^-126. (The passes are bounded by memory only as long as a pair of values takes some 45 instructions; for 32-bit results, which move twice the bytes, the functions of the library.)
+// is below 2^-126. (The passes are bounded by memory only as long as a pair of values takes some 40 instructions, of which every one counts: with five more, and conversion instructions for the codes, SwiGLU took 60
+// us instead of 53; for 32-bit results, which move twice the bytes, the functions of the library.)
 template <class T>
 __device__ __forceinline__ void sigmoid(float g, float& s, float& c) {
     float e, r;
@@ -92,7 +119,7 @@ __global__ void __launch_bounds__(256) k_int8_quantize(const T* x, int64_t ldx, 
 #pragma unroll
         for (int j = 0; j < kPer; ++j) f[j] = to_float(v[q][j]);
         uint32_t byte;
-        const uint2 c = codes8(f, byte);   // (whole blocks: pieces is a multiple of four)
+        const uint2 c = codes8(f, largest(v[q]), byte);   // (whole blocks: pieces is a multiple of four)
         if (i < pieces) {
             codes[i] = c;
             if ((i & 3u) == 0) scales[i >> 2] = uint8_t(byte);
@@ -152,7 +179,7 @@ __global__ void __launch_bounds__(256) k_int8_swiglu(const T* gu, int64_t ldgu, 
             o[j] = g[j] * s * u[j];
         }
         uint32_t byte_g, byte_u;
-        const uint2 cg = codes8(g, byte_g), cu = codes8(u, byte_u);
+        const uint2 cg = codes8(g, largest(v[q][0]), byte_g), cu = codes8(u, largest(v[q][1]), byte_u);
         if (i < pieces) {
             put8<T, VEC>(h + int64_t(t) * ldh + c * kPer, o);
             const size_t at = size_t(t) * 2 * per_row + c;   // in pieces
@@ -213,7 +240,7 @@ __global__ void __launch_bounds__(256) k_int8_swiglu_grad(const T* gh, int64_t l
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 // f(T(), whether accesses of 16 bytes are possible, how many pieces a thread has in flight): of 16-bit elements four where that leaves blocks enough for every SM, of 32-bit ones two.
-// 81,920 rows of 2 x 512 bf16: SwiGLU 64 / 60 / 60 us, its gradient 69 / 70 / 67 with 1 / 2 / 4 (5.6 and 6.3 TB/s); f32 89 / 91 / 120 and 116 / 116 / 120 (6.5 TB/s).
+// 81,920 rows of 2 x 512 bf16: SwiGLU 53 us, its gradient 67 (70 with two; 6.3 TB/s of what has to move, a copy 6.4); f32 89 and 116 (6.6 TB/s; with four 120 and 120).
 template <class F>
 void with_type(int dtype, bool vec, uint64_t pieces, F f) {
     auto flight = [&](auto v, auto wide) {
