@@ -6,20 +6,25 @@
 namespace frx {
 namespace {
 
-// Three forms of one kernel. D is the tensor core's 128 x N block of sums (N a multiple of 16 up to 256); its lanes are the index that is contiguous in what
+// Three forms of one kernel. D is the tensor core's 256 x N block of sums (N a multiple of 32 up to 256); its lanes are the index that is contiguous in what
 // is written, so that a warp's stores of a column are whole sectors and need no exchange through shared memory:
 //   forward  y[r][m]     = sum_k W_e[m][k] x[r][k]     lanes: matrix rows m, columns: rows r of expert e, depth: n
 //   grad x   gx[r][m]    = sum_k W_e[k][m] gy[r][k]    lanes: matrix columns m, columns: rows r of expert e, depth: rows of the matrix
 //   grad w   gW_e[c][m]  = sum_t gy[t][c] x[t][m]      lanes: matrix columns m, columns: matrix rows c, depth: the rows t of expert e
-// The rows of an expert are the N side in the first two, so that few rows waste nothing (N is that of the tile, not of the kernel), and the matrix is read once per 256 of
-// them. Operands come by TMA in the 128-byte swizzle as they lie in memory: a side whose index is contiguous there is the instruction's MN-major form, so no
+// The rows of an expert are the N side in the first two, so that few rows waste little (N is that of the tile, not of the kernel), and the matrix is read once per 256 of
+// them. Operands come by TMA in the 128-byte swizzle as they lie in memory: a side whose index is contiguous there is the instruction's MN-major form, which is as fast, so no
 // operand is ever transposed. A stage is 64 of depth. What lies beyond a matrix, or beyond all rows, arrives as zeros. Rows of the next expert that a box brings along fill
 // columns of D that are not stored; in the third form, where they would be summed, they are zeroed in shared memory first.
 //
 // Two blocks on neighbouring SMs (a cluster) share a tile of 256 lanes by up to 256 columns: the instruction (cta_group::2) takes 128 lanes and half of the columns from the shared memory of
-// each and leaves 128 lanes of all columns in the tensor memory of each. So 32 KB a stage and SM feed 512 clocks of products, 64 bytes a clock; one block's tile of 128 x 256 wanted
-// 96, and the L2 gives some 55 to 60 (131,072 rows of 2,048 by 1,024 in 712 us so). The first block of a pair issues; both load their own operands, whose bytes are counted on the
-// first one's barriers, and both write their own lanes.
+// each and leaves 128 lanes of all columns in the tensor memory of each: 32 KB a stage and SM for 512 clocks of products where one block's tile of 128 x 256 takes 48. The
+// first block of a pair issues; both load their own operands, whose bytes are counted on the first one's barriers, and both write their own lanes. 131,072 rows of 2,048 by 1,024: 712 us with
+// single blocks, 593 with pairs, 521 with two loads a stage instead of five.
+//
+// What bounds it. 65,536 rows of 64 equal experts, 2,048 by 1,024: 207 us, gradients 221 and 219 (1,330, 1,240 and 1,250 TFLOP/s; the library's batched product of the same matrices, equal
+// experts alone, takes 202): 17,300 clocks a tile of 16,400 that the tensor cores need, at 1.1 to 1.3 GHz, which is what the power limit leaves; experts of different sizes cost another tenth (tiles of
+// fewer than 256 columns wait for their loads). A row or two an expert: the matrices. 64 tokens of ten experts out of 512: 1.54 GB in 230 us, 6.8 TB/s of what has to move. One token: 40 tiles, 8.5 of 15 us
+// for 512 KB a block, the rest is start, tables and end. Gradients of matrices with few rows: what is written (1.68 GB in 32 bits, 330 us).
 enum Form { kForward, kGradX, kGradW };
 
 constexpr int kTileM = 256, kLanes = 128, kDepth = 64, kTileN = 256, kUnitN = 32;   // lanes of a tile, of a block; columns of a tile at most, what they are a multiple of
@@ -178,13 +183,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
         mbar_fence_init();
     }
     if (warp == kWarpMma) tmem_alloc_pair(tmem_slot, 512);
+    __syncwarp();
+    cluster_sync_all();   // the barriers of both blocks are there
     pdl_wait();
     pdl_trigger();
     const long long tiles = group_tables<kThreads, kUnitN>(tab, p.offsets, p.E, p.S, p.width, (p.lanes + kTileM - 1) / kTileM, reinterpret_cast<long long*>(smem + kSums));
     const int experts = FORM != kGradW && tiles > p.most ? 0 : p.E;   // offsets that do not ascend: nothing is computed
     tc_fence_before_sync();
-    __syncwarp();
-    cluster_sync_all();   // the barriers of both blocks are there
+    __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     Tiles<FORM> t;
@@ -419,13 +425,13 @@ int depth_rows_map(CUtensorMap& map, const void* x, int64_t ld, int dtype, int r
     if (chunks == 1) return rows_map(map, x, ld, dtype, rows, n, kDepth);
     const cuuint64_t dims[3] = {64, cuuint64_t(rows), cuuint64_t(n / 64)}, strides[2] = {cuuint64_t(ld) * 2, 128};
     const cuuint32_t boxes[3] = {64, kDepth, cuuint32_t(chunks)};
-    return encode_tensor_map(map, map_type(dtype), 3, x, dims, strides, boxes);
+    return encode_16(map, dtype, 3, x, dims, strides, boxes);
 }
 int depth_matrices_map(CUtensorMap& map, const void* w, int64_t ldw, int64_t lde, int dtype, int E, int rows, int n, int chunks) {
     if (chunks == 1) return matrices_map(map, w, ldw, lde, dtype, E, rows, n, kDepth);
     const cuuint64_t dims[4] = {64, cuuint64_t(rows), cuuint64_t(n / 64), cuuint64_t(E)}, strides[3] = {cuuint64_t(ldw) * 2, 128, cuuint64_t(lde) * 2};
     const cuuint32_t boxes[4] = {64, kDepth, cuuint32_t(chunks), 1};
-    return encode_tensor_map(map, map_type(dtype), 4, w, dims, strides, boxes);
+    return encode_16(map, dtype, 4, w, dims, strides, boxes);
 }
 
 int shape(const char* who, int dtype, int out_dtype, int E, int rows, int n, int S) {

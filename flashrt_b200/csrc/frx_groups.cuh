@@ -237,7 +237,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[2][8]) {
 
 // A tensor map with the 128-byte swizzle (box[0] elements are 128 bytes) over rows of dims[0] elements; strides in bytes, of the dimensions from the second on. What
 // lies outside reads as zeros.
-inline int encode_tensor_map(CUtensorMap& map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+inline int encode_tensor_map(CUtensorMap& map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                             CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_128B) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static std::atomic<void*> entry{nullptr};   // the driver's function: looked up once
@@ -250,7 +251,7 @@ inline int encode_tensor_map(CUtensorMap& map, CUtensorMapDataType type, int ran
     }
     const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
     const CUresult r = reinterpret_cast<Encode>(fn)(&map, type, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                                    CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FRX_OK : fail(FRX_ERR_CUDA, "cuTensorMapEncodeTiled: error %d (%llu rows of %llu elements)", int(r), (unsigned long long)dims[1], (unsigned long long)dims[0]);
 }
 
@@ -273,18 +274,22 @@ inline uint32_t f16_idesc(int dtype, bool lanes_mn, bool cols_mn, int lanes = 12
     const uint32_t type = dtype == FRX_BF16;
     return (1u << 4) | type << 7 | type << 10 | uint32_t(lanes_mn) << 15 | uint32_t(cols_mn) << 16 | uint32_t(lanes >> 4) << 24;
 }
-inline CUtensorMapDataType map_type(int dtype) { return dtype == FRX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
+// A map of 16-bit elements. The 128 bytes of a row that a box brings come into the L2 with their neighbours, which the next stage reads (1.5 GB of matrices by a row or two each 247 -> 228 us, by
+// sixty 151 -> 140).
+inline int encode_16(CUtensorMap& map, int dtype, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    return encode_tensor_map(map, dtype == FRX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, base, dims, strides, box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
 
 // rows of n elements, `box` of them a load
 inline int rows_map(CUtensorMap& map, const void* x, int64_t ld, int dtype, int rows, int n, int box) {
     const cuuint64_t dims[2] = {cuuint64_t(n), cuuint64_t(rows)}, strides[1] = {cuuint64_t(ld) * 2};
     const cuuint32_t boxes[2] = {64, cuuint32_t(box)};
-    return encode_tensor_map(map, map_type(dtype), 2, x, dims, strides, boxes);
+    return encode_16(map, dtype, 2, x, dims, strides, boxes);
 }
 inline int matrices_map(CUtensorMap& map, const void* w, int64_t ldw, int64_t lde, int dtype, int E, int rows, int n, int box) {
     const cuuint64_t dims[3] = {cuuint64_t(n), cuuint64_t(rows), cuuint64_t(E)}, strides[2] = {cuuint64_t(ldw) * 2, cuuint64_t(lde) * 2};
     const cuuint32_t boxes[3] = {64, cuuint32_t(box), 1};
-    return encode_tensor_map(map, map_type(dtype), 3, w, dims, strides, boxes);
+    return encode_16(map, dtype, 3, w, dims, strides, boxes);
 }
 
 inline bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
