@@ -275,7 +275,7 @@ def _on_device(*ts):
     """The tensors are on the current device, whose stream the call goes to."""
     dev = _current_device() if _current_device else None
     for t in ts:
-        if t is not None and not (t.is_cuda and t.get_device() == dev):
+        if t is not None and t.get_device() != dev:   # (-1 of a tensor in host memory)
             raise FrxError(_l.ERR_ARG, "tensors must be CUDA tensors of the current device")
 
 
@@ -434,9 +434,10 @@ def _matrices(name: str, w: torch.Tensor, dtype=None, shape=None):
 
 
 def _half(name: str, t: torch.Tensor) -> int:
-    if t.dtype != torch.bfloat16 and t.dtype != torch.float16:
+    code = DTYPES.get(t.dtype)
+    if not code:   # (float32 is 0)
         raise FrxError(_l.ERR_ARG, f"{name}: bfloat16 or float16 is wanted, not {t.dtype}")
-    return DTYPES[t.dtype]
+    return code
 
 
 def moe_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor | None = None, dtype: torch.dtype | None = None, stream=None) -> torch.Tensor:
