@@ -104,6 +104,14 @@ def test_ranks(rank, lengths):
     Case(LENGTHS[lengths], 384, 300, rank, before=4).check()
 
 
+@pytest.mark.parametrize("rank", [3, 16, 17, 24, 32, 33, 48, 63, 64, 100])
+@pytest.mark.parametrize("users,n,rows", [(1, 2048, 2048), (1, 8, 3), (5, 1000, 257), (40, 2560, 384), (150, 72, 1030), (300, 520, 64)])
+def test_a_token_each(users, n, rows, rank):
+    """A decode batch: as many requests as tokens, few and many blocks a tile."""
+    dtype = BF16 if rank % 2 else F16
+    Case([1] * users, n, rows, rank, dtype=dtype, out=(F32, dtype)[rows % 2], behind=0, before=2 if users > 4 else 0).check()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("out", [F32, BF16, F16])
 @pytest.mark.parametrize("n,rows,rank", [(1, 1, 1), (8, 3, 8), (63, 129, 20), (1000, 257, 72), (512, 512, 16)])
@@ -130,10 +138,11 @@ def test_without_scale_and_rows_apart():
         assert torch.equal(view[:live], want[:live]) and (buf[3:].view(T, 265)[:, 264] == 7).all() and (buf[:3] == 7).all() and (view[live:] == 7).all()
 
 
+@pytest.mark.parametrize("lengths,rank", [([1, 40, 200], 16), ([1] * 30, 16), ([1] * 30, 40)])
 @pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** 12])
-def test_small_and_large_values_in_float16(size):
+def test_small_and_large_values_in_float16(size, lengths, rank):
     """A x far below and far above what float16 holds: it stays in 32 bits. (B takes the opposite size, so that the result is ordinary.)"""
-    c = Case([1, 40, 200], 512, 256, 16, dtype=F16, out=F32, none=0.0)
+    c = Case(lengths, 512, 256, rank, dtype=F16, out=F32, none=0.0)
     c.a = (c.a.double() * size).to(F16)          # (small: subnormals, exact as they are)
     c.x = (c.x.double() * (64 if size > 1 else 2.0 ** -4)).to(F16)
     c.b = (c.b.double() / 16).to(F16) if size > 1 else c.b
@@ -164,6 +173,27 @@ def test_nan_and_infinity_stay_with_their_tokens():
     a2[0] = float("nan")
     got = adapters.add(y, x, a2, b2, offsets, which)
     assert got[:30].isnan().all() and got[159:229].isnan().all() and torch.equal(got[30:159], want[30:159]) and torch.equal(got[229:], want[229:])
+
+
+@pytest.mark.parametrize("rank", [8, 40])
+def test_nan_and_infinity_of_a_token_each(rank):
+    c = Case([1] * 50, 264, 300, rank, none=0.0, behind=0, count=50)
+    c.which = torch.arange(50, dtype=torch.int32)
+    y, x, a, b, offsets, which = c.args()
+    want = adapters.add(y, x, a, b, offsets, which)
+    for t in (0, 7, 49):
+        for bad in (float("nan"), float("inf")):
+            for spoil in range(3):
+                x2, a2, b2 = x.clone(), a.clone(), b.clone()
+                if spoil == 0:
+                    x2[t, 200] = bad
+                elif spoil == 1:
+                    a2[t, rank - 1, 3] = bad
+                else:
+                    b2[t, :, 2] = bad
+                got = adapters.add(y, x2, a2, b2, offsets, which)
+                others = torch.arange(c.T) != t
+                assert torch.equal(got[others], want[others]) and not torch.isfinite(got[t]).any()
 
 
 def test_nothing_to_do():
@@ -263,9 +293,9 @@ def test_adapters_in_the_order_of_a_sort():
     assert ((back.double().cpu() - want).abs() <= tol)[live].all()
 
 
-@pytest.mark.parametrize("lengths,rank", [([1], 8), ([3], 16), ([40, 1, 30], 64)])
+@pytest.mark.parametrize("lengths,rank", [([1], 8), ([20], 16), ([40, 1, 30], 64)])
 def test_a_wait_that_runs_out_leaves_nan(lengths, rank):
-    """A row of half a million values keeps the rest of a tile waiting, and the other blocks of its cluster; with a limit of one microsecond (a token alone is quick) it gives up. Nothing
+    """A row of half a million values keeps the rest of a tile waiting, and the other blocks of its cluster; with a limit of one microsecond (a few tokens are quick) it gives up. Nothing
     hangs, no wrong number is left, and the next call is as if nothing had been."""
     T, n, rows = sum(lengths), 1 << 19, 400
     g = gen(3)
