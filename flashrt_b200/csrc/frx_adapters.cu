@@ -398,6 +398,7 @@ __device__ __forceinline__ void one_token_of_rank(const Adapters& p, uint32_t ba
                 for (int e = 0; e < 4; ++e) sum[e] += d[e], d[e] = 0.0f;
             }
         }
+        fetch_wait<0>();   // (those from behind the depth write zeros to the places of the next: copies have no order among themselves)
     }
     // the second product's first rows are on their way while the parts are added up
     const int all16 = (p.rows + 15) / 16, from16 = int(int64_t(all16) * rank / blocks), count = int(int64_t(all16) * (rank + 1) / blocks) - from16;   // this block's rows, 16 a step

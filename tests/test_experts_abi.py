@@ -188,3 +188,13 @@ def test_loads_behind_the_wait_are_ordinary_ones(source, least):
         seen += 1
         assert not re.search(r"\bconst\b[^,]*\*\s*__restrict__", params) and "__ldg(" not in body, name
     assert seen >= least
+
+
+def test_places_are_free_before_the_second_product_fills_them():
+    """Asynchronous copies have no order among themselves: those that the first product of a single token still has in flight (zeros from behind its depth) have to be waited for
+    before the second product's rows go to the same places."""
+    from pathlib import Path
+    text = (Path(moe.__file__).parent / "csrc" / "frx_adapters.cu").read_text()
+    body = text[text.index("void one_token_of_rank("):]
+    last, first = body.index("fetch(at);"), body.index("fetch(mine + i * 2 * NB * kSlotBytes);")   # the first product's last, the second's first
+    assert last < first and "fetch_wait<0>();" in body[last:first]
