@@ -980,6 +980,7 @@ extern "C" int frx_adapter_add(frx_stream_t stream, const void* x, int64_t ldx, 
     if (!offsets || !which || !y || !out) return fail(FRX_ERR_ARG, "%s: null pointer", who);
     if (ldy < rows || ldo < rows) return fail(FRX_ERR_ARG, "%s: rows of y and out are %lld and %lld elements apart and %d long", who, (long long)ldy, (long long)ldo, rows);
     if (!rows_aligned(y, dtype_size(y_dtype)) || !rows_aligned(out, dtype_size(y_dtype))) return fail(FRX_ERR_ARG, "%s: misaligned pointer", who);
+    if (out == y && ldo != ldy && T > 1) return fail(FRX_ERR_ARG, "%s: out is y, with rows %lld instead of %lld elements apart", who, (long long)ldo, (long long)ldy);
     int rc;
     if ((rc = operand(who, "x", x, ldx, T, n)) != FRX_OK || (rc = operand(who, "a", a, lda, rank, n)) != FRX_OK || (rc = operand(who, "b", b, ldb, rows, rank)) != FRX_OK ||
         (rc = operand(who, "a (its matrices)", a, stride_a, L, (rank - 1) * lda + n)) != FRX_OK ||

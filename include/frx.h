@@ -246,7 +246,7 @@ int frx_moe_matmul_backward_w(frx_stream_t stream, const void* gy, int64_t ldgy,
 
 /* ---- low-rank adapters of many requests beside a shared projection (whatever computes that: frx_mxfp4_matmul, frx_moe_matmul, a library; the reference has no counterpart)
  *   out[t] = y[t] + scale[j] * B_j (A_j x[t])   for the tokens t = offsets[i] .. offsets[i + 1] - 1 of request i, j = which[i]
- * and out[t] = y[t] for the tokens of a request whose which is negative (or L or more). y: what the projection gave; out may be y. x [T] rows of n; a: L matrices of `rank` rows of n
+ * and out[t] = y[t] for the tokens of a request whose which is negative (or L or more). y: what the projection gave; out may be y (with ldo = ldy), and else overlaps nothing that is read. x [T] rows of n; a: L matrices of `rank` rows of n
  * elements, lda apart, matrices stride_a apart; b: L matrices of `rows` rows of `rank` elements, ldb and stride_b apart; scale [L], or null for 1; y, out [T] rows of `rows` elements of
  * y_dtype. dtype (FRX_BF16 or FRX_F16) is that of x, a and b. Adapters of a smaller rank are filled up with zeros. Products are exact, both sums are formed in 32 bits on the tensor cores,
  * A_j x is kept in 32 bits between them, and out is rounded once; where A_j x holds infinities out may be NaN. x, a and b begin every row on a 16-byte boundary (ld* multiples of 8); y

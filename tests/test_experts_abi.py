@@ -198,3 +198,8 @@ def test_places_are_free_before_the_second_product_fills_them():
     body = text[text.index("void one_token_of_rank("):]
     last, first = body.index("fetch(at);"), body.index("fetch(mine + i * 2 * NB * kSlotBytes);")   # the first product's last, the second's first
     assert last < first and "fetch_wait<0>();" in body[last:first]
+
+
+def test_adapter_result_in_place_has_the_rows_of_y(L):
+    ok = [None, P, 64, P, 64, 64 * 16, P, 16, 16 * 40, 1, 5, 16, 64, 40, P, P, 3, None, 7, P, 40, P, 40, 1]
+    refused(L.lib.frx_adapter_add, ok, ((20, 48, L.ERR_ARG), (22, 48, L.ERR_ARG)))
