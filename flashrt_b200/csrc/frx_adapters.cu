@@ -842,7 +842,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                              "r"(bits[q % 3][3])
                              : "memory");
         }
-        fence_async_smem();   // generic-proxy writes: visible to the tensor core
+        fence_async_smem();       // generic-proxy writes: visible to the tensor core
+        tc_fence_before_sync();   // behind the loads of the first product's sums, whose columns the second product's take
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + kBarVIn * 8);
         float down = 1.0f, down8 = 1.0f;   // of the lane's tokens

@@ -333,3 +333,16 @@ def test_refusals():
                  lambda: f(y, x, a[:1].expand(5, 16, 64), b, offsets, which)):
         with pytest.raises(L.FrxError):
             call()
+
+
+@pytest.mark.parametrize("rank", [64, 128])
+@pytest.mark.parametrize("lengths", [[64] * 3, [50] * 400])
+def test_sums_are_read_before_their_columns_are_used_again(lengths, rank):
+    """The first product's parts fill tensor memory (512 of depth: as many parts as there is room for) and the second product's sums take the same columns: a tile over a cluster and tiles of
+    a block each give the same bits in every one of many launches, and the formula's values."""
+    c = Case(lengths, 512, 256, rank, out=F32, behind=0)
+    y, *rest = c.args()
+    c.check(scaled=False)
+    want = adapters.add(y, *rest)
+    got = [adapters.add(y, *rest) for _ in range(40)]
+    assert all(torch.equal(g, want) for g in got)
