@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
             if (blocks > 1) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-                if (taken < live && !lost)
+                if (taken < live)
                     for (uint32_t b = 0; b < blocks; b += 4) {   // (2, 4 or 8 blocks) the loads of four at once: each takes half a microsecond
                         float of[4][8];
 #pragma unroll
@@ -794,7 +794,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                             for (int c = 0; c < 8; ++c) v[c] += of[i][c];
                     }
             } else {
-                sum_parts(k, v);   // (sums that nobody has finished, where the wait ran out: the outputs are NaN then)
+                sum_parts(k, v);
             }
         };
         const float scale = p.scale ? __ldcg(p.scale + j) : 1.0f;
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                     for (uint32_t b = 0; b < blocks; ++b)
                         most += fmaxf(ld_peer1(peer_addr(s0 + kTokMax + taken * 4, b)), ld_peer1(peer_addr(s0 + kTokMax + (kTok + taken) * 4, b)));
             } else {
-                for (int k = first_k; k < p.rank16; k += step_k) {
+                for (int k = first_k; k < p.rank16 && !lost; k += step_k) {
                     float v[8];
                     take8(k, v);
 #pragma unroll
@@ -822,7 +822,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
             up = power_up(most, down);
             if (side == 0 && token < kTok) tok_scale[taken] = down;
         }
-        for (int k = first_k; k < p.rank16; k += step_k) {
+        // Where a wait ran out nothing is written, since the first product may still use its stages, and the arrival is left out: other warps, whose outputs need this warp's part of v, may
+        // have been in time. There is no second product then, and all waits for its sums run out.
+        for (int k = first_k; k < p.rank16 && !lost; k += step_k) {
             float v[8];
             take8(k, v);
             uint32_t bits[3][4];
@@ -845,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
         fence_async_smem();       // generic-proxy writes: visible to the tensor core
         tc_fence_before_sync();   // behind the loads of the first product's sums, whose columns the second product's take
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kBarVIn * 8);
+        if (lane == 0 && !lost) mbar_arrive(bars + kBarVIn * 8);
         float down = 1.0f, down8 = 1.0f;   // of the lane's tokens
         if (XTYPE == FRX_F16) {
             named_bar_sync(1, 32 * kWarpsEpi);
@@ -860,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
                 const int c = c0 + d * int(blocks);
                 if (c >= row_chunks) continue;
                 const int first = chunk(c) * kRows;
-                lost = !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns) || lost;
+                lost = lost || !warp_wait(bars + (kBarDFull + set) * 8, phase, abort, p.wait_ns);
                 tc_fence_after_sync();
                 const uint32_t sums = tmem + lanes + set * kRows;
                 if (p.whole) {

@@ -346,3 +346,30 @@ def test_sums_are_read_before_their_columns_are_used_again(lengths, rank):
     want = adapters.add(y, *rest)
     got = [adapters.add(y, *rest) for _ in range(40)]
     assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tiles,rank,depths", [(18, 64, (86016, 92160, 94208, 96256, 98304, 100352)), (320, 16, (9728, 10752, 11264, 11776, 12288, 15872))])
+def test_a_wait_that_runs_out_in_some_warps_leaves_no_wrong_number(tiles, rank, depths, dtype):
+    """Depths at which the first product is done just as the warps that wait for it give up: in some the wait has run out, in others not. What these write is NaN too, or right: each of their
+    outputs needs the whole of A x. (A wait ends at the earliest after some polls of a few microseconds each, so these depths are some tens of microseconds of work, with clusters and without.)"""
+    g, most = torch.Generator(device="cuda").manual_seed(4), max(depths)
+    x, a = torch.randn(64 * tiles, most, generator=g, device="cuda").to(dtype), (torch.randn(3, rank, most, generator=g, device="cuda") / most ** 0.5).to(dtype)
+    b, y = torch.randn(3, 400, rank, generator=g, device="cuda").to(dtype), torch.randn(64 * tiles, 400, generator=g, device="cuda")
+    offsets = torch.arange(tiles + 1, dtype=torch.int32, device="cuda") * 64
+    which = (torch.arange(tiles, device="cuda") % 3).int()
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    for n in depths:
+        args = y, x[:, :n], a[:, :, :n], b, offsets, which
+        want = adapters.add(*args)
+        torch.cuda.synchronize()
+        try:
+            L.check(L.lib.frx_debug_set_wait_limit_ns(1))
+            for _ in range(100):
+                got = adapters.add(*args)
+                wrong += (~got.isnan() & (got != want)).any()
+            torch.cuda.synchronize()
+        finally:
+            L.check(L.lib.frx_debug_set_wait_limit_ns(0))
+        assert torch.equal(adapters.add(*args), want)
+    assert int(wrong) == 0, f"{int(wrong)} calls left a finite number that is wrong"
