@@ -947,7 +947,7 @@ int launch_as(Adapters& p, const CUtensorMap& x_map, const CUtensorMap& a_map, c
     p.ring_bytes = std::max(((chunks == 1 ? kSmemTwo : int(kSmemMost)) - rest) / 1024 * 1024, 3 * chunks * kPieceV);
     const size_t smem = size_t(rest + p.ring_bytes);   // (about half of an SM's, or all of it: a third block would wait for tensor memory)
     p.wait_ns = wait_limit_ns();
-    FRX_LAUNCH(kKGateUp, stream, launch_pdl_cluster(k_adapter<XTYPE, TYPE, SINGLES>, dim3(unsigned(tiles) * blocks), dim3(kThreads), smem, stream, blocks, p, x_map, a_map, b_map));
+    FRX_LAUNCH(kKAdapter, stream, launch_pdl_cluster(k_adapter<XTYPE, TYPE, SINGLES>, dim3(unsigned(tiles) * blocks), dim3(kThreads), smem, stream, blocks, p, x_map, a_map, b_map));
     FRX_CUDA(cudaGetLastError());
     return FRX_OK;
 }

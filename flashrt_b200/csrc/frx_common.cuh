@@ -48,7 +48,7 @@ bool prefill_stream_fits(int n, int ff);   // whether the streaming kernels have
 
 // Optional per-kernel timing (frx_profile_begin / frx_profile_end): when switched on, every
 // launch made through FRX_LAUNCH is bracketed by two CUDA events on its own stream.
-enum KernelClass : int { kKRoute = 0, kKQuant, kKGroup, kKGateUp, kKDown, kKCombine, kKLayout, kKPrologue, kKFfn, kNumKernelClasses };
+enum KernelClass : int { kKRoute = 0, kKQuant, kKGroup, kKGateUp, kKDown, kKCombine, kKLayout, kKPrologue, kKFfn, kKProduct, kKAdapter, kKSwiglu, kNumKernelClasses };
 extern bool g_profile_on;
 void profile_mark(int cls, cudaStream_t stream, bool start);
 #define FRX_LAUNCH(cls, stream, ...)                                   \

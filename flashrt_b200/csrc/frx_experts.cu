@@ -406,7 +406,7 @@ int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& co
     p.sets = std::min(kMaxSets, 512 / p.width);
     p.wait_ns = wait_limit_ns();
     const unsigned pairs = unsigned(std::min<int64_t>(std::max(1, sm_count() / 2), std::max<int64_t>(1, most)));
-    FRX_LAUNCH(kKGateUp, stream,
+    FRX_LAUNCH(kKProduct, stream,
                launch_pdl_cluster(k_moe_product<FORM, TYPE>, dim3(2 * pairs), dim3(kThreads), kHead + size_t(p.stages) * p.stage_bytes + tables, stream, 2u, p, lanes_map, cols_map, small_map));
     FRX_CUDA(cudaGetLastError());
     return FRX_OK;

@@ -328,7 +328,7 @@ int frx_mxint8_swiglu(frx_stream_t stream, const void* gu, int64_t ldgu, int dty
     with_type(dtype, rows_vec16(gu, ldgu, ff, size) && rows_vec16(h, ldh, ff, size), pieces, [&](auto v, auto vec, auto u) {
         using V = decltype(v);
         constexpr int U = decltype(u)::value;
-        FRX_LAUNCH(kKQuant, stream, launch_pdl(k_int8_swiglu<V, decltype(vec)::value, U>, grid_of<U>(pieces), dim3(256), 0, stream, static_cast<const V*>(gu), ldgu, uint32_t(pieces),
+        FRX_LAUNCH(kKSwiglu, stream, launch_pdl(k_int8_swiglu<V, decltype(vec)::value, U>, grid_of<U>(pieces), dim3(256), 0, stream, static_cast<const V*>(gu), ldgu, uint32_t(pieces),
                                                uint32_t(ff / kPer), static_cast<uint2*>(codes), static_cast<uint8_t*>(scales), static_cast<V*>(h), ldh));
     });
     FRX_CUDA(cudaGetLastError());
@@ -348,7 +348,7 @@ int frx_mxint8_swiglu_backward(frx_stream_t stream, const void* gh, int64_t ldgh
     with_type(dtype, rows_vec16(gh, ldgh, ff, size) && rows_vec16(ggu, ldggu, ff, size) && (!h || rows_vec16(h, ldh, ff, size)), pieces, [&](auto v, auto vec, auto u) {
         using V = decltype(v);
         constexpr int U = decltype(u)::value;
-        FRX_LAUNCH(kKQuant, stream, launch_pdl(k_int8_swiglu_grad<V, decltype(vec)::value, U>, grid_of<U>(pieces), dim3(256), 0, stream, static_cast<const V*>(gh), ldgh,
+        FRX_LAUNCH(kKSwiglu, stream, launch_pdl(k_int8_swiglu_grad<V, decltype(vec)::value, U>, grid_of<U>(pieces), dim3(256), 0, stream, static_cast<const V*>(gh), ldgh,
                                                static_cast<const uint2*>(codes), static_cast<const uint8_t*>(scales), uint32_t(pieces), uint32_t(ff / kPer), static_cast<V*>(ggu), ldggu,
                                                static_cast<V*>(h), ldh));
     });

@@ -58,8 +58,9 @@ const char* frx_last_error(void);
  * Between frx_profile_begin() and frx_profile_end(), every kernel the library launches is bracketed
  * by two CUDA events on its stream. frx_profile_end waits for them and returns, per kernel class c
  * (frx_profile_class_name(c): "route_topk", "quant_q8", "group", "gate_up", "down", "combine",
- * "layout"), the summed device time ms[c] and the launch count launches[c]. Not for use while a
- * stream is being captured into a CUDA graph. */
+ * "layout", "route_group_quant", "ffn", "moe_product" (frx_moe_matmul*), "adapter", "swiglu"
+ * (frx_mxint8_swiglu*); "" behind the last), the summed device time ms[c] and the launch count
+ * launches[c]. Not for use while a stream is being captured into a CUDA graph. */
 int frx_profile_begin(void);
 int frx_profile_end(float* ms, int* launches, int n_classes);
 const char* frx_profile_class_name(int cls);

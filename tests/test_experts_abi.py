@@ -203,3 +203,11 @@ def test_places_are_free_before_the_second_product_fills_them():
 def test_adapter_result_in_place_has_the_rows_of_y(L):
     ok = [None, P, 64, P, 64, 64 * 16, P, 16, 16 * 40, 1, 5, 16, 64, 40, P, P, 3, None, 7, P, 40, P, 40, 1]
     refused(L.lib.frx_adapter_add, ok, ((20, 48, L.ERR_ARG), (22, 48, L.ERR_ARG)))
+
+
+def test_timings_name_these_kernels(L):
+    names, c = [], 0
+    while name := L.lib.frx_profile_class_name(c):
+        names.append(name.decode())
+        c += 1
+    assert len(set(names)) == len(names) and {"gate_up", "quant_q8", "moe_product", "adapter", "swiglu"} <= set(names) and L.lib.frx_profile_class_name(-1) == b""

@@ -296,3 +296,26 @@ def test_refusals():
                  lambda: bw(gy, x, od, out=torch.zeros(1, 32, 64, device="cuda").expand(2, 32, 64))):
         with pytest.raises(L.FrxError):
             call()
+
+
+def test_timings_are_kept_apart():
+    """Each of these kernels is counted in a class of its own, not with the expert layer's gate and up product or its quantizer."""
+    import ctypes as C
+
+    from flashrt_b200 import adapters, mxint8
+    x, w, od = torch.zeros(6, 64, dtype=BF16, device="cuda"), torch.zeros(2, 32, 64, dtype=BF16, device="cuda"), torch.tensor([0, 2, 6], dtype=torch.int32, device="cuda")
+    gy, a, b = torch.zeros(6, 32, dtype=BF16, device="cuda"), torch.zeros(2, 16, 64, dtype=BF16, device="cuda"), torch.zeros(2, 32, 16, dtype=BF16, device="cuda")
+    ms, launches = (C.c_float * 32)(), (C.c_int * 32)()
+    L.check(L.lib.frx_profile_begin())
+    try:
+        moe.moe_matmul(x, w, od)
+        moe.moe_matmul_backward_x(gy, w, od)
+        moe.moe_matmul_backward_w(gy, x, od)
+        adapters.add(gy, x, a, b, od, od[:2])
+        h, codes, scales = mxint8.swiglu(x)
+        mxint8.swiglu_backward(h, codes, scales)
+        mxint8.dequantize(*mxint8.quantize(x))
+    finally:
+        L.check(L.lib.frx_profile_end(ms, launches, 32))
+    counted = {L.lib.frx_profile_class_name(i).decode(): launches[i] for i in range(32) if launches[i]}
+    assert counted == {"moe_product": 3, "adapter": 1, "swiglu": 2, "quant_q8": 2}
