@@ -359,18 +359,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
             for (int first = 0; first < t.steps; first += p.run) {
                 const uint32_t acc = wait_for_sums();
 #pragma unroll
-                for (int c = 0; c < kSixteens; ++c)
-                    if (c * 32 + part * 16 < t.width && !lost) {
-                        uint32_t v[2][8];
-                        tmem_ld16(acc + c * 32 + part * 16, v);
+                for (int c = 0; c < kSixteens; ++c) {
+                    if (c * 32 + part * 16 >= t.width || lost) break;
+                    uint32_t v[2][8];
+                    tmem_ld16(acc + c * 32 + part * 16, v);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) sums[c][i / 8][i % 8] = __float_as_uint(__uint_as_float(sums[c][i / 8][i % 8]) + __uint_as_float(v[i / 8][i % 8]));
-                    }
+                    for (int i = 0; i < 16; ++i) sums[c][i / 8][i % 8] = __float_as_uint(__uint_as_float(sums[c][i / 8][i % 8]) + __uint_as_float(v[i / 8][i % 8]));
+                }
                 give_back();
             }
 #pragma unroll
-            for (int c = 0; c < kSixteens; ++c)
-                if (c * 32 + part * 16 < t.width) store16(sums[c], c * 32 + part * 16);
+            for (int c = 0; c < kSixteens; ++c) {
+                if (c * 32 + part * 16 >= t.width) break;   // (instructions that are not reached are not fetched either)
+                store16(sums[c], c * 32 + part * 16);
+            }
         }
     }
     tc_fence_before_sync();
@@ -399,10 +401,10 @@ int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& co
     p.stages = int(std::min<size_t>(kMaxStages, (kSmemMost - kHead - tables) / size_t(p.stage_bytes)));
     static_assert((kSmemMost - kHead - 4096 * 16) / (kStageA + kTileN / 2 * kDepth * 2) >= 4, "stages beside the tables of 4096 experts");
     // The tensor cores add to their sums by cutting off, half a step of 2^-23 of the sum so far on average and always towards zero: 128 additions (2,048 of depth) leave a relative error of
-    // 2.1e-6 in the root mean square. What is returned in 32 bits they sum over 256 of depth at a time, which the epilogue adds up rounded to nearest: 2.4e-7 (over 512 4.7e-7; a plain sum in 32
-    // bits leaves 1e-7). It costs nothing where matrices are the traffic, and a tenth where the tensor cores are busy (131,072 rows of 2,048 by 1,024 523 instead of 469 us). 16 bits round by
-    // 2^-9 and 2^-12 themselves: there it is 8,192 of depth.
-    p.run = TYPE == FRX_F32 ? 4 : 128;
+    // 2.1e-6 in the root mean square. So they sum over a part of the depth at a time, and the epilogue adds these sums up rounded to nearest: 256 of depth for what is returned in 32 bits, 2.4e-7 (a
+    // plain sum in 32 bits leaves 1e-7 to 4e-7, by its order), 512 for what is rounded to 16 bits, by up to 2^-8 and 2^-11, afterwards: 4.7e-7. It costs nothing where matrices are the traffic, and where
+    // the tensor cores are busy a tenth in 32 bits (131,072 rows of 2,048 by 1,024 523 instead of 469 us) and 3 % in 16 (546 instead of 531; by 256 as well it would be another tenth).
+    p.run = TYPE == FRX_F32 ? 4 : 8;
     p.sets = std::min(kMaxSets, 512 / p.width);
     p.wait_ns = wait_limit_ns();
     const unsigned pairs = unsigned(std::min<int64_t>(std::max(1, sm_count() / 2), std::max<int64_t>(1, most)));
