@@ -403,7 +403,7 @@ int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& co
     // The tensor cores add to their sums by cutting off, half a step of 2^-23 of the sum so far on average and always towards zero: 128 additions (2,048 of depth) leave a relative error of
     // 2.1e-6 in the root mean square. So they sum over a part of the depth at a time, and the epilogue adds these sums up rounded to nearest: 256 of depth for what is returned in 32 bits, 2.4e-7 (a
     // plain sum in 32 bits leaves 1e-7 to 4e-7, by its order), 512 for what is rounded to 16 bits, by up to 2^-8 and 2^-11, afterwards: 4.7e-7. It costs nothing where matrices are the traffic, and where
-    // the tensor cores are busy a tenth in 32 bits (131,072 rows of 2,048 by 1,024 523 instead of 469 us) and 3 % in 16 (546 instead of 531; by 256 as well it would be another tenth).
+    // the tensor cores are busy a tenth in 32 bits (131,072 rows of 2,048 by 1,024 523 instead of 469 us) and 3 % in 16 (546 instead of 531).
     p.run = TYPE == FRX_F32 ? 4 : 8;
     p.sets = std::min(kMaxSets, 512 / p.width);
     p.wait_ns = wait_limit_ns();
