@@ -111,11 +111,6 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 template <int TYPE>
-__device__ __forceinline__ float wide(uint32_t bits) {   // of the low half
-    if (TYPE == FRX_BF16) return __uint_as_float(bits << 16);
-    return __half2float(__ushort_as_half(uint16_t(bits)));
-}
-template <int TYPE>
 __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
     if (TYPE == FRX_BF16) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -174,14 +169,6 @@ __device__ __forceinline__ void copy_rows(const void* from, int64_t ld_from, voi
     }
 }
 
-// an element of y, of which nothing is waited for here
-template <int TYPE>
-__device__ __forceinline__ void load_one_if(uint32_t& w, const void* p, bool on) {
-    if (TYPE == FRX_F32)
-        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u32 %0, [%1];\n\t}" : "+r"(w) : "l"(p), "r"(uint32_t(on)));
-    else
-        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u16 %0, [%1];\n\t}" : "+r"(w) : "l"(p), "r"(uint32_t(on)));
-}
 // eight 16-bit elements from p on, `count` of which are there (the others 0); p on a 16-byte boundary
 struct Eight {
     uint4 v;

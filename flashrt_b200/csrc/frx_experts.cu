@@ -89,21 +89,15 @@ __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result, uint32_t 
 }
 __device__ __forceinline__ void tmem_free_pair(uint32_t base, uint32_t cols) { asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory"); }
 
-// what is there, added to eight columns of this lane (32 bits, before the one rounding)
+// what is there, added to 16 columns of this lane (32 bits, before the one rounding): all of them are on their way at once
 template <int TYPE>
-__device__ __forceinline__ void add8(uint32_t (&v)[8], const void* y, int64_t ldy, int live, bool have) {
+__device__ __forceinline__ void add16(uint32_t (&v)[2][8], const uint8_t* y, int64_t ldy, int live, bool have) {
+    constexpr int size = TYPE == FRX_F32 ? 4 : 2;
+    uint32_t old[16] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < live && have) {
-            float old;
-            if (TYPE == FRX_F32)
-                old = static_cast<const float*>(y)[i * ldy];
-            else if (TYPE == FRX_BF16)
-                old = __bfloat162float(static_cast<const __nv_bfloat16*>(y)[i * ldy]);
-            else
-                old = __half2float(static_cast<const __half*>(y)[i * ldy]);
-            v[i] = __float_as_uint(__uint_as_float(v[i]) + old);
-        }
+    for (int i = 0; i < 16; ++i) load_one_if<TYPE>(old[i], y + i * ldy * size, i < live && have);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = __float_as_uint(__uint_as_float(v[i / 8][i % 8]) + (TYPE == FRX_F32 ? __uint_as_float(old[i]) : wide<TYPE>(old[i])));
 }
 
 // The tiles of a block. First two forms: those of GroupWalk (expert, lanes tile, block of its rows). Third form: every matrix has as many.
@@ -333,16 +327,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_product(const Product p, co
             const bool have = at_lane < p.lanes;
             uint8_t* y = static_cast<uint8_t*>(p.y) + ((FORM == kGradW ? t.e * p.ldye : 0) + t.col0 * p.ldy + at_lane) * size;
             auto store16 = [&](uint32_t (&v)[2][8], int c) {
+                if (lost) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint8_t* at = y + (c + 8 * h) * p.ldy * size;
-                    if (lost) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[h][i] = 0x7fffffffu;
-                    }
-                    if (FORM == kGradW && p.add) add8<TYPE>(v[h], at, p.ldy, t.live - c - 8 * h, have);
-                    store8<TYPE>(v[h], at, p.ldy, t.live - c - 8 * h, have, pairs);
+                    for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = 0x7fffffffu;
                 }
+                if (FORM == kGradW && p.add) add16<TYPE>(v, y + c * p.ldy * size, p.ldy, t.live - c, have);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) store8<TYPE>(v[h], y + (c + 8 * h) * p.ldy * size, p.ldy, t.live - c - 8 * h, have, pairs);
             };
             if (t.steps <= p.run) {   // one run: from tensor memory to y
                 const uint32_t acc = wait_for_sums();
@@ -401,10 +392,11 @@ int launch_typed(Product& p, const CUtensorMap& lanes_map, const CUtensorMap& co
     p.stages = int(std::min<size_t>(kMaxStages, (kSmemMost - kHead - tables) / size_t(p.stage_bytes)));
     static_assert((kSmemMost - kHead - 4096 * 16) / (kStageA + kTileN / 2 * kDepth * 2) >= 4, "stages beside the tables of 4096 experts");
     // The tensor cores add to their sums by cutting off, half a step of 2^-23 of the sum so far on average and always towards zero: 128 additions (2,048 of depth) leave a relative error of
-    // 2.1e-6 in the root mean square. So they sum over a part of the depth at a time, and the epilogue adds these sums up rounded to nearest: 256 of depth for what is returned in 32 bits, 2.4e-7 (a
-    // plain sum in 32 bits leaves 1e-7 to 4e-7, by its order), 512 for what is rounded to 16 bits, by up to 2^-8 and 2^-11, afterwards: 4.7e-7. It costs nothing where matrices are the traffic, and where
-    // the tensor cores are busy a tenth in 32 bits (131,072 rows of 2,048 by 1,024 523 instead of 469 us) and 3 % in 16 (546 instead of 531).
-    p.run = TYPE == FRX_F32 ? 4 : 8;
+    // 2.1e-6 in the root mean square. So they sum over a part of the depth at a time, and the epilogue adds these sums up rounded to nearest. What is returned in 32 bits: 256 of depth, 2.4e-7 (a plain
+    // sum in 32 bits leaves 1e-7 to 1e-6, by its order and depth). What is rounded to 16 bits afterwards, by up to 2^-8 or 2^-11: 1,024 of depth, 1.0e-6. It costs nothing where matrices are the
+    // traffic; where the tensor cores are busy a tenth in 32 bits (131,072 rows of 2,048 by 1,024 523 instead of 469 us) and 1 to 2 % in 16 (the same 545 instead of 538 in a stream of such, 65,536 rows 211
+    // instead of 207; with 512 of depth 550 and 217: an epilogue that writes has two runs' time before the tensor cores wait for it).
+    p.run = TYPE == FRX_F32 ? 4 : 16;
     p.sets = std::min(kMaxSets, 512 / p.width);
     p.wait_ns = wait_limit_ns();
     const unsigned pairs = unsigned(std::min<int64_t>(std::max(1, sm_count() / 2), std::max<int64_t>(1, most)));

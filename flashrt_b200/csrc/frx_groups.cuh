@@ -170,6 +170,20 @@ __device__ __forceinline__ void store8(const uint32_t (&v)[8], void* y, int64_t 
         }
 }
 
+// An element of rows that are added to, of which nothing is waited for here (as a conditional assignment the load becomes a branch that is waited for)
+template <int TYPE>
+__device__ __forceinline__ void load_one_if(uint32_t& w, const void* p, bool on) {
+    if (TYPE == FRX_F32)
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u32 %0, [%1];\n\t}" : "+r"(w) : "l"(p), "r"(uint32_t(on)));
+    else
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u16 %0, [%1];\n\t}" : "+r"(w) : "l"(p), "r"(uint32_t(on)));
+}
+template <int TYPE>
+__device__ __forceinline__ float wide(uint32_t bits) {   // of the low half
+    if (TYPE == FRX_BF16) return __uint_as_float(bits << 16);
+    return __half2float(__ushort_as_half(uint16_t(bits)));
+}
+
 // ---- blocks of a cluster
 
 __device__ __forceinline__ uint32_t cluster_rank() {
