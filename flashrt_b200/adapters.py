@@ -15,7 +15,9 @@ def add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, offs
     """out[t] = y[t] + scale[j] * B_j (A_j x[t]) for the tokens t = offsets[i] .. offsets[i + 1] - 1 of each request i, j = which[i]; y[t] alone where that is negative.
 
     y [T][rows]: what the shared projection of x [T][n] gave, float32, bfloat16 or float16; a [L][rank][n], b [L][rows][rank] and x bfloat16 or float16, rank up to 128 (adapters of
-    a smaller one filled up with zeros); offsets int32 [R + 1], which int32 [R], scale float32 [L] or None for 1. Rows of x, a and b on 16-byte boundaries. `out`: y itself, or another
+    a smaller one filled up with zeros); offsets int32 [R + 1], which int32 [R], scale float32 [L] or None for 1. Rows of x, a and b on 16-byte boundaries: a `b` of a rank that is not a
+    multiple of 8 is the first columns of a wider one (`wide[:, :, :4]` of [L][rows][8]); contiguous it is refused. Rows of y and `out` that are not whole multiples of 32 bytes, 32 bytes aligned,
+    are slow for requests of several tokens (ten times at 16,384 tokens). `out`: y itself, or another
     tensor of its shape and type, or None for a new one; tokens of no request are left as they were (in a new one: anything). A decode batch is R = T requests of a token each."""
     if stream is not None and out is None:
         return _on(stream, add, y, x, a, b, offsets, which, scale=scale, out=out)

@@ -30,9 +30,12 @@ constexpr int kSmemTwo = 228 * 512 - 1024;   // shared memory of a block of whic
 // lane). The sums come out of tensor memory in the form of 16 lanes x 8 columns, in which a thread has columns 2 i, 2 i + 1 (i = lane % 4) of every eight: so the rows of B_j go into shared memory in
 // the order that makes these consecutive. Of G = 16 (32-bit y: 8) rows an access, column 8 k + 2 i + b of 4 G columns is row G i + 2 k + b: three dimensions of the tensor map.
 //
-// What bounds it. 16,384 tokens, rank 32, 2,048 by 2,048: 46 us for 204 MB (a copy takes 31): the two halves of the kernel, x in (15 us) and y through (25), each near the rate of memory, follow
-// one another, and 3 us of start and end. 1,000 tokens of 41 users, rank 64: 26 us, a chain of 10 KB stages, the exchange between four blocks, and five steps over rows of y. 64
-// users, rank 16: 8.6 us, one: 6.1 (and 9 for the call from Python).
+// What bounds it. 16,384 tokens, rank 32, 2,048 by 2,048: 47 to 50 us for 204 MB (a copy takes 31): the two halves of the kernel, x in (15 us) and y through (25), each near the rate of memory, follow
+// one another, and 3 us of start and end. 1,000 tokens of 41 users, rank 64, 32-bit y: 27 us, a chain of 16 KB stages, three in flight, the exchange between four blocks, and five steps over rows of y.
+// 64 users, rank 16: 8.6 us, one: 5.9 (8.5 for the call from Python).
+// Where y and out do not allow accesses of 32 bytes (rows, distances or addresses that are not multiples of 32 bytes) a lane adds element by element, each behind the store of the last: ten
+// times as long for 16,384 tokens (2,040 rows instead of 2,048: 496 us instead of 48), seven for the 1,000 with 16-bit y (128 instead of 18.5), nothing for tiles of single tokens up to a rank of 64.
+// Every block looks through all requests: 64 tokens at a time of thousands of them are bound by that (1,024 single tokens of rank 16 50 us, 4,096 229, 16,384 2.8 ms).
 struct Adapters {
     const int32_t* offsets;   // [R + 1]
     const int32_t* which;     // [R]
@@ -339,7 +342,7 @@ __device__ __forceinline__ float power_up(float most, float& down) {
 // The same of a rank of 17 to 64, by warps' own matrix instructions (16 rows of a matrix by 8 tokens, of which there is one): a lane's eight elements of a row come in one asynchronous copy to a
 // place of the lane's own, kSlots of which it has, so that nothing is waited for but its own copies and none take registers. (The order of the depth inside an instruction is free as long as
 // both operands have the same.) First product: a warp has 16 rows of A_j and every so many-th 32 of this block's depth, summed over 128 from zero and added up rounded to nearest. Second: a warp has 16
-// rows of B_j a step, y read four steps ahead. NB: the rank in 32s. 256 users, rank 32: 23 us instead of 36, rank 64: 34 instead of 46.
+// rows of B_j a step, y read four steps ahead. NB: the rank in 32s. 256 users, rank 32: 20 us (36 as tiles of 64 tokens), rank 64: 31 (46); 64 users 11 and 14.
 constexpr int kSlots = 15, kSlotBytes = kThreads * 16;
 template <int XTYPE, int TYPE, int NB>
 __device__ __forceinline__ void one_token_of_rank(const Adapters& p, uint32_t bars, uint32_t abort, uint32_t slots, float* own, float* part, uint32_t part_addr, float* v, int t0, int j, int c0, int c1, uint32_t rank,
@@ -601,7 +604,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter(const Adapters p, const
     const int boxes = (live + p.box - 1) / p.box;
     const uint32_t x_bytes = uint32_t(boxes * p.box) * 128, stage_bytes = x_bytes + uint32_t(p.rank16) * 128, stages = min(uint32_t(kMaxStages), uint32_t(p.ring_bytes) / max(stage_bytes, 1u));
     // The tensor cores add to their sums by cutting off (half a step of 2^-23 each time on average, towards zero): the first product's depth goes into several sums, some 256 of it each as far as
-    // tensor memory has room, which are added up rounded to nearest; of the second product's pieces the smallest come first.
+    // tensor memory has room (eight sums up to a rank of 32, four of 64, two of 128: 1,024 each of a depth of 2,048 in one block), which are added up rounded to nearest; of the second product's
+    // pieces the smallest come first. 32-bit results of 1,000 tokens, rank 64, y among them, are off by 2.2e-7 in the root mean square (plain products in 32 bits: 1.5e-7).
     const int room = kCols / p.rank16, part_depths = max(4, (d1 - d0 + min(room, 8) - 1) / min(room, 8)), parts = (d1 - d0 + part_depths - 1) / part_depths;
     bool lost = false;
 

@@ -21,10 +21,12 @@ namespace {
 // first block of a pair issues; both load their own operands, whose bytes are counted on the first one's barriers, and both write their own lanes. 131,072 rows of 2,048 by 1,024: 712 us with
 // single blocks, 593 with pairs, 521 with two loads a stage instead of five.
 //
-// What bounds it. 65,536 rows of 64 equal experts, 2,048 by 1,024: 207 us, gradients 221 and 219 (1,330, 1,240 and 1,250 TFLOP/s; the library's batched product of the same matrices, equal
-// experts alone, takes 202): 17,300 clocks a tile of 16,400 that the tensor cores need, at 1.1 to 1.3 GHz, which is what the power limit leaves; experts of different sizes cost another tenth (tiles of
-// fewer than 256 columns wait for their loads). A row or two an expert: the matrices. 64 tokens of ten experts out of 512: 1.54 GB in 230 us, 6.8 TB/s of what has to move. One token: 40 tiles, 8.5 of 15 us
-// for 512 KB a block, the rest is start, tables and end. Gradients of matrices with few rows: what is written (1.68 GB in 32 bits, 330 us).
+// What bounds it. 65,536 rows of 64 equal experts, 2,048 by 1,024: 212 us, gradients 221 and 216 (1,300, 1,240 and 1,270 TFLOP/s; the library's batched product of the same matrices, equal
+// experts alone, takes 202): some 17,300 clocks a tile of 16,400 that the tensor cores need, at 1.1 to 1.3 GHz, which is what the power limit leaves. Experts of 1,030 rows instead of 1,024, whose five
+// tiles of 224 columns wait for their loads: 244, 254 and 253. 131,072 rows of 128 experts of a skewed routing: 542, 28 % more than twice the 212. A row or two an expert: the matrices. 64 tokens of
+// ten experts out of 512: 1.54 GB in 226 us, 6.8 TB/s of what has to move. One token: 40 tiles, 8.5 of 15 us for 512 KB a block, the rest is start, tables and end. Gradients of matrices with few rows:
+// what is written (128 of 2,560 by 1,280 in 32 bits, 1.68 GB, 280 us). Added to what is there (65,536 rows): 297 us, in 32 bits 396 instead of 265: a lane's 16 elements are read at once, but
+// none before the sums are there.
 enum Form { kForward, kGradX, kGradW };
 
 constexpr int kTileM = 256, kLanes = 128, kDepth = 64, kTileN = 256, kUnitN = 32;   // lanes of a tile, of a block; columns of a tile at most, what they are a multiple of

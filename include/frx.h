@@ -233,7 +233,9 @@ int frx_moe_unsort_rows_backward(frx_stream_t stream, const void* gout, int64_t 
  *   backward_x:  gx[r] = W_e^T gy[r]         gy [S] rows of `rows`, gx [S] rows of n
  *   backward_w:  gW_e  = sum over the rows r of e of gy[r] x[r]^T: `rows` rows of n, ldgw apart, matrices ldge apart; zeros for an expert without
  *                rows. With add it is added to what gw holds (and experts without rows are left as they were).
- * dtype (FRX_BF16 or FRX_F16) is that of x, w and gy; out_dtype any. Products are exact, sums are formed in 32 bits on the tensor cores and rounded once. What is
+ * dtype (FRX_BF16 or FRX_F16) is that of x, w and gy; out_dtype any. Products are exact. Sums are formed in 32 bits by the tensor cores, which cut off
+ * (towards zero, by half a step of 2^-23 of the sum on average) where they add to it, over 256 of depth where out_dtype is FRX_F32 and 1,024 else; the sums of these are added rounded to nearest,
+ * with add what gw holds to the last of them, and the result is rounded to out_dtype once: relative errors of 2.4e-7 and, in front of that rounding, 1.0e-6 in the root mean square. What is
  * read (x, gy, w) begins every row on a 16-byte boundary: aligned bases and ld* multiples of 8 elements; n and `rows` are any (up to 2^20). What is written has any alignment of an
  * element. Rows that no expert has (behind offsets[E]) are neither read into a sum nor written. offsets lie in [0, S] and ascend: what lies outside is left out, and offsets
  * that descend may leave everything out. The same inputs give the same bits. Buffers do not overlap. E <= 4096. A device-side wait that runs out (2 s,
@@ -249,9 +251,11 @@ int frx_moe_matmul_backward_w(frx_stream_t stream, const void* gy, int64_t ldgy,
  *   out[t] = y[t] + scale[j] * B_j (A_j x[t])   for the tokens t = offsets[i] .. offsets[i + 1] - 1 of request i, j = which[i]
  * and out[t] = y[t] for the tokens of a request whose which is negative (or L or more). y: what the projection gave; out may be y (with ldo = ldy), and else overlaps nothing that is read. x [T] rows of n; a: L matrices of `rank` rows of n
  * elements, lda apart, matrices stride_a apart; b: L matrices of `rows` rows of `rank` elements, ldb and stride_b apart; scale [L], or null for 1; y, out [T] rows of `rows` elements of
- * y_dtype. dtype (FRX_BF16 or FRX_F16) is that of x, a and b. Adapters of a smaller rank are filled up with zeros. Products are exact, both sums are formed in 32 bits on the tensor cores,
- * A_j x is kept in 32 bits between them, and out is rounded once; where A_j x holds infinities out may be NaN. x, a and b begin every row on a 16-byte boundary (ld* multiples of 8); y
- * and out have any alignment of an element. offsets [R + 1] lie in [0, T] and ascend: what lies outside is left out, and offsets that descend may leave out
+ * y_dtype. dtype (FRX_BF16 or FRX_F16) is that of x, a and b. Adapters of a smaller rank are filled up with zeros. Products are exact. Both sums are formed in 32 bits by the tensor cores, which cut
+ * off where they add: the first over 256 of depth at a time, or more where tensor memory holds fewer sums (up to n / 2 at a rank above 64), which are added
+ * rounded to nearest. A_j x is kept in 32 bits between them, and out is rounded to y_dtype once. Where A_j x or B_j holds infinities out may be NaN. x, a and b begin every row on a 16-byte boundary (ld*
+ * multiples of 8): of a rank that is not a multiple of 8 (4, say) b is held in wider rows, e.g. [L][rows][8] with ldb = 8, whose other elements are not read. y and out have any alignment of an
+ * element; where their addresses, distances or lengths of rows are not multiples of 32 bytes, requests of several tokens (and single tokens of a rank above 64) take up to ten times as long. offsets [R + 1] lie in [0, T] and ascend: what lies outside is left out, and offsets that descend may leave out
  * anything. Tokens of no request (behind offsets[R]) are left as they were. rank <= 128; n and rows up to 2^20. A device-side wait that runs out leaves NaN in out. */
 int frx_adapter_add(frx_stream_t stream, const void* x, int64_t ldx, const void* a, int64_t lda, int64_t stride_a, const void* b, int64_t ldb, int64_t stride_b, int dtype, int L, int rank,
                     int n, int rows, const int32_t* offsets, const int32_t* which, int R, const float* scale, int T, const void* y, int64_t ldy, void* out, int64_t ldo, int y_dtype);
